@@ -6,7 +6,8 @@
  * cudaStream_t (passed as void*; NULL = the legacy default stream). Functions return MMB200_OK (0) or a negative
  * status, never throw and never abort. Mutable state of the library: per-device function attributes that are set once;
  * the per-device memory pool, internal streams and events of mmb200_scaled_mm_host; the fixed scratch array of mmb200_scaled_mm_static with its
- * cached per-device address; the launch counter; the process-wide test hooks of mmb200_test_hooks.
+ * cached per-device address; the launch counter; the process-wide test hooks of mmb200_test_hooks; the per-device status
+ * word of the int8 kernels (mmb200_int8_status).
  *
  * Operands are FP8 code bytes: A is [M, K] row-major with leading dimension lda (bytes), B is [N, K] row-major with
  * leading dimension ldb -- that is mat2.t() of torch._scaled_mm's column-major [K, N] operand.
@@ -32,7 +33,7 @@
 extern "C" {
 #endif
 
-#define MMB200_ABI_VERSION 4
+#define MMB200_ABI_VERSION 5
 
 /* status codes */
 #define MMB200_OK 0
@@ -196,6 +197,7 @@ void mmb200_test_hooks(int wait_polls, int announce_extra_bytes);
  * runs as torch operations before mmaemu.scaled_mm; the reference has no fused counterpart. */
 #define MMB200_HP_F32 1
 #define MMB200_HP_BF16 2
+#define MMB200_HP_F16 3          /* the int8 entry points only */
 int mmb200_quantize_scaled_mm_ws(const void *X_dev, int64_t ldx, int x_dtype, const float *quant_scale_dev,
                                  void *A_codes_dev, int64_t lda, const void *B_dev, int64_t ldb, int fmt_b,
                                  void *D_dev, int64_t ldd, int out_dtype, int M, int N, int K, int nfma, int fast, int S,
@@ -224,6 +226,56 @@ int mmb200_scaled_mm_static(const void *A_dev, int64_t lda, int fmt_a, const voi
  * to 16-byte operands (the last to K a multiple of 16). Pure host logic: no CUDA call, nothing is dereferenced. It has no
  * counterpart in the reference, whose kernels each serve one format pair and one preset (mmaemu/backends/registry.py). */
 int mmb200_kernel_for(const void *A_dev, int64_t lda, const void *B_dev, int64_t ldb, int K, int nfma, int S);
+
+/* ---- Ragged groups: rows [m_0 + .. + m_{e-1}, + m_e) of A are multiplied with the weights of group e.
+ *
+ * mmb200_grouped_scaled_mm is mmb200_scaled_mm_ws for every group: group e has m_splits[e] rows of A and D, the operand
+ * B + e * group_stride_b, the scales scale_a_dev[e * sa_stride] and scale_b_dev[e * sb_stride] (stride 0: one scale for all
+ * groups) and the split decision splits[e], schemes[e] (NULL: no group is split). The result has the bits of a loop of
+ * mmb200_scaled_mm_ws calls, whatever kernel runs. m_splits, splits and schemes are HOST arrays of E entries, read during
+ * the call (the split decision of the emulated platform depends on a group's rows). Scratch memory as there:
+ * mmb200_grouped_workspace_bytes; mmb200_grouped_status synchronises `stream` and reports whether a bounded wait of the call
+ * that last used it ran out (the outputs of that group then keep their previous contents). The reference has no grouped
+ * call. */
+#define MMB200_MAX_GROUPS 4096
+size_t mmb200_grouped_workspace_bytes(const int *m_splits, const int *splits, int E, int N, int K);
+int mmb200_grouped_scaled_mm(const void *A_dev, int64_t lda, int fmt_a, const void *B_dev, int64_t ldb,
+                             int64_t group_stride_b, int fmt_b, void *D_dev, int64_t ldd, int out_dtype,
+                             const int *m_splits, const int *splits, const int *schemes, int E, int N, int K, int nfma,
+                             int fast, const float *scale_a_dev, int sa_stride, const float *scale_b_dev, int sb_stride,
+                             const float *scale_result_dev, int kernel, void *workspace_dev, size_t workspace_bytes,
+                             void *stream);
+int mmb200_grouped_status(const void *workspace_dev, void *stream);
+
+/* ---- int8. Integer tensor-core sums are exact on every GPU, so these calls emulate no platform.
+ *
+ * mmb200_quantize_int8: per row of X [rows, K] (x_dtype MMB200_HP_*, row stride ldx elements) scale = RN32(amax / 127) and
+ * the codes [rows, K] (row stride ldc): the integer nearest to 127 x / amax, ties to even, decided exactly. A zero row has
+ * scale 0; a row with a NaN or an infinity has scale NaN and codes 0. */
+int mmb200_quantize_int8(const void *X_dev, int64_t ldx, int x_dtype, int8_t *codes_dev, int64_t ldc, float *scale_dev,
+                         int64_t rows, int K, void *stream);
+
+/* D[r][n] = out(fma(RN32(acc), RN32(sa sb), bias)), acc = sum_k A[r][k] W[g][n][k] (exact; K <= MMB200_INT8_MAX_K,
+ * T <= MMB200_INT8_MAX_ROWS), rounded
+ * to fp32 and then to out_dtype (F32, BF16 or F16; canonical NaN). A is [T, K] int8 with row stride lda, W [E, N, K] with row
+ * stride ldw and group stride group_stride_w. sa = scale_a_dev[r * sa_stride], sb = scale_b_dev[g * sb_group_stride +
+ * n * sb_stride], bias = bias_dev[g * bias_group_stride + n] of bias_dtype (MMB200_HP_*; bias_dev NULL: none).
+ * offs_dev NULL: one group (E = 1) of all T rows. Else offs_dev[g] (device, int32) is the end of group g's rows; ends are
+ * taken as a running maximum and clamped to [0, T], so no value leads out of the operands. Rows behind the last group are
+ * set to zero (zero_rest != 0) or left as they are. Operands whose rows do not start on 16 bytes are copied into scratch
+ * memory of mmb200_int8_workspace_bytes first (16-byte aligned; 0 bytes: none needed). */
+#define MMB200_INT8_MAX_K 131071
+#define MMB200_INT8_MAX_ROWS (1 << 23)
+size_t mmb200_int8_workspace_bytes(const int8_t *A_dev, int64_t lda, const int8_t *W_dev, int64_t ldw,
+                                   int64_t group_stride_w, int T, int N, int K, int E);
+int mmb200_int8_scaled_mm(const int8_t *A_dev, int64_t lda, const int8_t *W_dev, int64_t ldw, int64_t group_stride_w,
+                          void *D_dev, int64_t ldd, int out_dtype, int T, int N, int K, int E, const int *offs_dev,
+                          const float *scale_a_dev, int sa_stride, const float *scale_b_dev, int64_t sb_group_stride,
+                          int sb_stride, const void *bias_dev, int bias_dtype, int64_t bias_group_stride, int zero_rest,
+                          void *workspace_dev, size_t workspace_bytes, void *stream);
+/* Synchronises `stream`, reads and clears the current device's status word of the int8 kernels: MMB200_ERR_TIMEOUT when a
+ * bounded wait has run out since the word was last read (outputs of that call are unspecified), else MMB200_OK. */
+int mmb200_int8_status(void *stream);
 
 /* Issue-rate probe for roofline denominators: launches `ctas` blocks of 256 threads in which every thread executes
  * iters x 32 independent instructions of one kind (kind 0: fma.rz.f32; kind 1: three-input integer add and three-input

@@ -29,6 +29,10 @@ _LAZY = {
     "sharded_scaled_mm": ("mmaemu_b200.sharding", "sharded_scaled_mm"),
     "scaled_mm_into": ("mmaemu_b200.api", "scaled_mm_into"),
     "scaled_mm_host": ("mmaemu_b200.api", "scaled_mm_host"),
+    "grouped_scaled_mm": ("mmaemu_b200.grouped", "grouped_scaled_mm"),
+    "quantize_int8": ("mmaemu_b200.int8", "quantize_int8"),
+    "int8_scaled_mm": ("mmaemu_b200.int8", "int8_scaled_mm"),
+    "int8_grouped_scaled_mm": ("mmaemu_b200.int8", "int8_grouped_scaled_mm"),
 }
 
 __all__ = ["__version__", *sorted(_LAZY), "MmaemuError", "ReferenceRejectsError", "UnsupportedFeatureError",

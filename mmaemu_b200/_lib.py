@@ -12,7 +12,7 @@ from pathlib import Path
 from .errors import BackendUnavailableError
 
 LIB_PATH = Path(__file__).resolve().parent / "libmmaemu_b200.so"
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 FMT_CODES = {"e4m3": 0, "e5m2": 1}
 OUT_CODES = {"float32": 0, "bfloat16": 1, "float16": 2, "float8_e4m3fn": 3, "float8_e5m2": 4}
@@ -24,7 +24,9 @@ EXPORTS = ("mmb200_abi_version", "mmb200_status_string", "mmb200_last_cuda_error
            "mmb200_chain", "mmb200_accumulate", "mmb200_scaled_mm", "mmb200_scaled_mm_host", "mmb200_kernel_for",
            "mmb200_launch_count", "mmb200_workspace_bytes", "mmb200_workspace_bytes_split", "mmb200_scaled_mm_ws", "mmb200_accumulate_ws",
            "mmb200_scaled_mm_static", "mmb200_quantize_scaled_mm_ws", "mmb200_workspace_status_offset",
-           "mmb200_workspace_status", "mmb200_scaled_mm_static_status", "mmb200_test_hooks", "mmb200_scaled_mm_peers", "mmb200_probe_issue_rate")
+           "mmb200_workspace_status", "mmb200_scaled_mm_static_status", "mmb200_test_hooks", "mmb200_scaled_mm_peers", "mmb200_probe_issue_rate",
+           "mmb200_grouped_workspace_bytes", "mmb200_grouped_scaled_mm", "mmb200_grouped_status", "mmb200_quantize_int8", "mmb200_int8_workspace_bytes",
+           "mmb200_int8_scaled_mm", "mmb200_int8_status")
 
 _lock = threading.Lock()
 _lib = None
@@ -101,6 +103,23 @@ def load():
         L.mmb200_test_hooks.restype = None
         L.mmb200_kernel_for.argtypes = [vp, i64, vp, i64, ci, ci, ci]
         L.mmb200_kernel_for.restype = ci
+        sz = ctypes.c_size_t
+        L.mmb200_grouped_workspace_bytes.argtypes = [vp, vp, ci, ci, ci]
+        L.mmb200_grouped_workspace_bytes.restype = sz
+        L.mmb200_grouped_scaled_mm.argtypes = [vp, i64, ci, vp, i64, i64, ci, vp, i64, ci, vp, vp, vp, ci, ci, ci, ci, ci, vp, ci,
+                                               vp, ci, vp, ci, vp, sz, vp]
+        L.mmb200_grouped_scaled_mm.restype = ci
+        L.mmb200_grouped_status.argtypes = [vp, vp]
+        L.mmb200_grouped_status.restype = ci
+        L.mmb200_quantize_int8.argtypes = [vp, i64, ci, vp, i64, vp, i64, ci, vp]
+        L.mmb200_quantize_int8.restype = ci
+        L.mmb200_int8_workspace_bytes.argtypes = [vp, i64, vp, i64, i64, ci, ci, ci, ci]
+        L.mmb200_int8_workspace_bytes.restype = sz
+        L.mmb200_int8_scaled_mm.argtypes = [vp, i64, vp, i64, i64, vp, i64, ci, ci, ci, ci, ci, vp, vp, ci, vp, i64, ci, vp, ci,
+                                            i64, ci, vp, sz, vp]
+        L.mmb200_int8_scaled_mm.restype = ci
+        L.mmb200_int8_status.argtypes = [vp]
+        L.mmb200_int8_status.restype = ci
         L.mmb200_launch_count.argtypes = []
         L.mmb200_launch_count.restype = i64
         got = L.mmb200_abi_version()

@@ -16,11 +16,13 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libmmaemu_b200.so"
-SOURCES = ("api.cu", "kernel_integer.cu", "kernel_fast.cu", "kernel_umma.cu", "static_scratch.cu")
+SOURCES = ("api.cu", "kernel_integer.cu", "kernel_fast.cu", "kernel_umma.cu", "kernel_int8.cu", "kernel_quantise.cu",
+           "static_scratch.cu")
 # translation units: (source, extra defines). kernel_fast.cu is compiled once per FP8 format pair and kind of kernel
 # (tensor cores: parts 0..3, CUDA cores: 4..7), in parallel.
 UNITS = (("api.cu", ()), ("kernel_integer.cu", ()), ("static_scratch.cu", ()), ("kernel_umma.cu", ()),
-         *(("kernel_fast.cu", (f"-DMMB_PART={part}",)) for part in range(8)))
+         *(("kernel_fast.cu", (f"-DMMB_PART={part}",)) for part in range(8)),
+         ("kernel_int8.cu", ()), ("kernel_quantise.cu", ()))
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "--fmad=false", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 OBJ = PKG / "csrc" / "_obj"
@@ -37,7 +39,7 @@ def stale() -> bool:
     if not LIB.exists():
         return True
     t = LIB.stat().st_mtime
-    deps = [CSRC / s for s in SOURCES] + list(CSRC.glob("*.cuh")) + [PKG.parent / "include" / "mmaemu_b200.h"]
+    deps = [CSRC / s for s in SOURCES] + [*CSRC.glob("*.cuh"), *CSRC.glob("*.h")] + [PKG.parent / "include" / "mmaemu_b200.h"]
     return any(d.stat().st_mtime > t for d in deps)
 
 
@@ -50,7 +52,7 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
     nvcc = nvcc_path()
     # a unit is compiled again when its object is older than its source, a shared header or this file
-    shared = [*CSRC.glob("*.cuh"), PKG.parent / "include" / "mmaemu_b200.h", Path(__file__)]
+    shared = [*CSRC.glob("*.cuh"), *CSRC.glob("*.h"), PKG.parent / "include" / "mmaemu_b200.h", Path(__file__)]
     newest_shared = max(d.stat().st_mtime for d in shared)
     jobs = []
     for i, (src, defines) in enumerate(UNITS):

@@ -6,6 +6,7 @@
 #include <cstring>
 
 #include "common.cuh"
+#include "int8.h"
 
 namespace {
 
@@ -45,7 +46,7 @@ int run(const void* A, int64_t lda, int fmt_a, const void* B, int64_t ldb, int f
         const float* sr, int epilogue, int patch, int kernel, void* stream, void* workspace = nullptr,
         size_t workspace_bytes = 0, const void* a_hp = nullptr, int64_t ld_hp = 0, int hp_dtype = 0,
         const float* quant_scale = nullptr, void* const* peer_D = nullptr, int n_peers = 0,
-        unsigned char* shared_b = nullptr, bool alu = mmb::tensor_cores_off()) {
+        unsigned char* shared_b = nullptr, bool alu = mmb::tensor_cores_off(), int* status_word = nullptr) {
   if (n_peers < 0 || n_peers > MMB200_MAX_PEERS || (n_peers > 0 && !peer_D)) return MMB200_ERR_BAD_ARG;
   for (int q = 0; q < n_peers; ++q)
     if (!peer_D[q]) return MMB200_ERR_BAD_ARG;
@@ -91,6 +92,7 @@ int run(const void* A, int64_t lda, int fmt_a, const void* B, int64_t ldb, int f
   for (int q = 0; q < n_peers; ++q) p.peer_D[q] = peer_D[q];
   p.shared_b = shared_b;
   p.no_tensor_epass = alu ? 1 : 0;
+  p.status_word = status_word;
 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t err;
@@ -513,6 +515,153 @@ int mmb200_scaled_mm_host(const void* A, int64_t lda, int fmt_a, const void* B, 
   for (int i = 0; i < n_slabs; ++i)
     if (words[i] != 0) return MMB200_ERR_TIMEOUT;   // slabs are copied back as they finish: D is unspecified then
   return MMB200_OK;
+}
+
+// Scratch memory of a grouped call: a status word for all its launches, then the scratch memory of one group after the other.
+constexpr size_t GROUPED_HEADER = 256;
+
+size_t mmb200_grouped_workspace_bytes(const int* m_splits, const int* splits, int E, int N, int K) {
+  if (!m_splits || E <= 0 || E > MMB200_MAX_GROUPS || N <= 0 || K <= 0) return 0;
+  size_t most = 0;
+  for (int e = 0; e < E; ++e) {
+    if (m_splits[e] <= 0) continue;
+    const size_t n = mmb::staged_workspace_bytes(m_splits[e], N, K, splits ? splits[e] : 1, true, false, mmb::tensor_cores_off());
+    if (n > most) most = n;
+  }
+  return most ? GROUPED_HEADER + most : 0;
+}
+
+int mmb200_grouped_status(const void* workspace, void* stream) {
+  if (!workspace) return MMB200_OK;                   // nothing waits
+  int word = 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t err = cudaMemcpyAsync(&word, workspace, sizeof(int), cudaMemcpyDeviceToHost, st);
+  if (err == cudaSuccess) err = cudaStreamSynchronize(st);
+  if (err != cudaSuccess) return cuda_fail(err);
+  return word ? MMB200_ERR_TIMEOUT : MMB200_OK;
+}
+
+int mmb200_grouped_scaled_mm(const void* A, int64_t lda, int fmt_a, const void* B, int64_t ldb, int64_t group_stride_b, int fmt_b,
+                             void* D, int64_t ldd, int out_dtype, const int* m_splits, const int* splits, const int* schemes,
+                             int E, int N, int K, int nfma, int fast, const float* scale_a, int sa_stride, const float* scale_b,
+                             int sb_stride, const float* scale_result, int kernel, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  if (E < 0 || N < 0 || K < 0 || (E > 0 && !m_splits) || !splits != !schemes) return MMB200_ERR_BAD_ARG;
+  if (E > MMB200_MAX_GROUPS) return MMB200_ERR_TOO_LARGE;
+  if (!scale_a || !scale_b || sa_stride < 0 || sb_stride < 0 || group_stride_b < 0) return MMB200_ERR_BAD_ARG;
+  if (out_dtype < MMB200_OUT_F32 || out_dtype > MMB200_OUT_E5M2) return MMB200_ERR_BAD_ARG;
+  long long rows = 0;
+  for (int e = 0; e < E; ++e) {
+    if (m_splits[e] < 0) return MMB200_ERR_BAD_ARG;
+    rows += m_splits[e];
+  }
+  if (rows > 0x7FFFFFFFLL) return MMB200_ERR_TOO_LARGE;
+  const size_t es = out_size(out_dtype);
+  const uint8_t* a = static_cast<const uint8_t*>(A);
+  uint8_t* d = static_cast<uint8_t*>(D);
+  int* word = nullptr;
+  if (workspace && workspace_bytes > GROUPED_HEADER && rows > 0 && N > 0) {
+    const int rc = current_device_ok();
+    if (rc != MMB200_OK) return rc;
+    word = static_cast<int*>(workspace);
+    const cudaError_t err = cudaMemsetAsync(word, 0, sizeof(int), static_cast<cudaStream_t>(stream));
+    if (err != cudaSuccess) return cuda_fail(err);
+    workspace = static_cast<unsigned char*>(workspace) + GROUPED_HEADER;
+    workspace_bytes -= GROUPED_HEADER;
+  } else {
+    workspace = nullptr;
+    workspace_bytes = 0;
+  }
+  for (int e = 0; e < E; ++e) {
+    const int rc = run(a, lda, fmt_a, static_cast<const uint8_t*>(B) + (size_t)e * (size_t)group_stride_b, ldb, fmt_b, d, ldd,
+                       out_dtype, m_splits[e], N, K, nfma, fast, splits ? splits[e] : 1, splits ? schemes[e] : 0,
+                       scale_a + (size_t)e * sa_stride, scale_b + (size_t)e * sb_stride, scale_result, 1, 1, kernel, stream,
+                       workspace, workspace_bytes, nullptr, 0, 0, nullptr, nullptr, 0, nullptr, mmb::tensor_cores_off(), word);
+    if (rc != MMB200_OK) return rc;
+    a += (size_t)m_splits[e] * (size_t)lda;
+    d += (size_t)m_splits[e] * (size_t)ldd * es;
+  }
+  return MMB200_OK;
+}
+
+int mmb200_quantize_int8(const void* X, int64_t ldx, int x_dtype, int8_t* codes, int64_t ldc, float* scale, int64_t rows, int K,
+                         void* stream) {
+  if (x_dtype < MMB200_HP_F32 || x_dtype > MMB200_HP_F16 || rows < 0 || K < 0) return MMB200_ERR_BAD_ARG;
+  if (rows == 0) return MMB200_OK;
+  if (!scale || (K > 0 && (!X || !codes))) return MMB200_ERR_BAD_ARG;
+  if (rows > 1 && (ldx < K || ldc < K)) return MMB200_ERR_BAD_ARG;
+  if (rows > 0x7FFFFFFFLL || K > (1 << 30)) return MMB200_ERR_TOO_LARGE;
+  const int size = x_dtype == MMB200_HP_F32 ? 4 : 2, per8 = x_dtype == MMB200_HP_F32 ? 4 : 8;
+  if (reinterpret_cast<uintptr_t>(X) % size || reinterpret_cast<uintptr_t>(scale) % 4) return MMB200_ERR_BAD_ARG;
+  const int rc = current_device_ok();
+  if (rc != MMB200_OK) return rc;
+  mmb::QuantiseParams p;
+  p.x = X; p.codes = codes; p.scale = scale;
+  p.ldx = ldx; p.ldc = ldc; p.rows = rows; p.K = K;
+  p.vec_in = !(reinterpret_cast<uintptr_t>(X) & 15) && (rows == 1 || (ldx * size) % 16 == 0);
+  p.vec_out = reinterpret_cast<uintptr_t>(codes) % per8 == 0 && (rows == 1 || ldc % per8 == 0);
+  const cudaError_t err = mmb::launch_quantise(p, x_dtype, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err);
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return MMB200_OK;
+}
+
+size_t mmb200_int8_workspace_bytes(const int8_t* A, int64_t lda, const int8_t* W, int64_t ldw, int64_t group_stride_w, int T, int N,
+                                   int K, int E) {
+  if (T <= 0 || N <= 0 || K <= 0 || E <= 0) return 0;
+  mmb::Int8Params p;
+  std::memset(&p, 0, sizeof(p));
+  p.a = A; p.w = W; p.lda = lda; p.ldw = ldw; p.gsw = group_stride_w; p.T = T; p.N = N; p.K = K; p.E = E;
+  return mmb::int8_workspace_bytes(p);
+}
+
+int mmb200_int8_scaled_mm(const int8_t* A, int64_t lda, const int8_t* W, int64_t ldw, int64_t group_stride_w, void* D, int64_t ldd,
+                          int out_dtype, int T, int N, int K, int E, const int* offs, const float* scale_a, int sa_stride,
+                          const float* scale_b, int64_t sb_group_stride, int sb_stride, const void* bias, int bias_dtype,
+                          int64_t bias_group_stride, int zero_rest, void* workspace, size_t workspace_bytes, void* stream) {
+  if (T < 0 || N < 0 || K < 0 || E < 0 || (!offs && E != 1)) return MMB200_ERR_BAD_ARG;
+  if (out_dtype < MMB200_OUT_F32 || out_dtype > MMB200_OUT_F16) return MMB200_ERR_BAD_ARG;
+  if (bias && (bias_dtype < MMB200_HP_F32 || bias_dtype > MMB200_HP_F16)) return MMB200_ERR_BAD_ARG;
+  if (!scale_a || !scale_b || sa_stride < 0 || sb_stride < 0 || sb_group_stride < 0 || bias_group_stride < 0 || group_stride_w < 0)
+    return MMB200_ERR_BAD_ARG;
+  if (K > MMB200_INT8_MAX_K || T > MMB200_INT8_MAX_ROWS || E > MMB200_MAX_GROUPS) return MMB200_ERR_TOO_LARGE;
+  if (T == 0 || N == 0) return MMB200_OK;
+  if (!D || (T > 1 && ldd < N)) return MMB200_ERR_BAD_ARG;
+  if (K > 0 && E > 0 && (!A || !W || (T > 1 && lda < K) || (N > 1 && ldw < K))) return MMB200_ERR_BAD_ARG;
+  const uintptr_t es = out_dtype == MMB200_OUT_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(D) % es) return MMB200_ERR_BAD_ARG;
+  const int rc = current_device_ok();
+  if (rc != MMB200_OK) return rc;
+  mmb::Int8Params p;
+  std::memset(&p, 0, sizeof(p));
+  p.a = A; p.w = W; p.d = D;
+  p.scale_a = scale_a; p.scale_b = scale_b; p.bias = bias; p.offs = offs;
+  p.lda = lda; p.ldw = ldw; p.gsw = group_stride_w; p.ldd = ldd; p.sb_group = sb_group_stride; p.bias_group = bias_group_stride;
+  p.T = T; p.N = N; p.K = K; p.E = E;
+  p.sa_stride = sa_stride; p.sb_stride = sb_stride;
+  p.bias_dtype = bias_dtype; p.out_dtype = out_dtype;
+  p.zero_rest = zero_rest;
+  const size_t need = E > 0 ? mmb::int8_workspace_bytes(p) : 0;
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) return MMB200_ERR_BAD_ARG;
+  int launches = 0;
+  const cudaError_t err = mmb::launch_int8(p, workspace, static_cast<cudaStream_t>(stream), &launches);
+  g_launches.fetch_add(launches, std::memory_order_relaxed);
+  if (err != cudaSuccess) return cuda_fail(err);
+  return MMB200_OK;
+}
+
+int mmb200_int8_status(void* stream) {
+  const int rc = current_device_ok();
+  if (rc != MMB200_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int* word = nullptr;
+  int seen = 0;
+  cudaError_t err = mmb::int8_status_word(&word);
+  if (err == cudaSuccess) err = cudaMemcpyAsync(&seen, word, sizeof(int), cudaMemcpyDeviceToHost, st);
+  if (err == cudaSuccess) err = cudaMemsetAsync(word, 0, sizeof(int), st);
+  if (err == cudaSuccess) err = cudaStreamSynchronize(st);
+  if (err != cudaSuccess) return cuda_fail(err);
+  return seen ? MMB200_ERR_TIMEOUT : MMB200_OK;
 }
 
 int mmb200_kernel_for(const void* A, int64_t lda, const void* B, int64_t ldb, int K, int nfma, int S) {

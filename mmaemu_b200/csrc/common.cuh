@@ -41,6 +41,7 @@ struct Params {
   int* ws_flag_a;
   int* ws_flag_b;
   int* status;
+  int* status_word;      // caller's status word instead of the one in the scratch memory (a word for several launches), or null
   int k_tiles;
   // B decoded by an earlier launch (the host-buffer entry point decodes B once and runs the rows of A slab by slab):
   // shared_b holds B's tile images followed by its column flags (staged_shared_b_bytes); the launch then neither
@@ -329,6 +330,7 @@ cudaError_t launch_staged(const Params& p, int nfma, void* workspace, size_t wor
 size_t staged_status_offset(int M, int N);
 // Test hooks of the bounded waits (process-wide; wait_polls <= 0 and announce_extra <= 0 restore the defaults).
 void staged_test_hooks(int wait_polls, int announce_extra);
+void staged_wait_limits(int* wait_polls, int* announce_extra);      // what they are set to
 // Text of the last CUDA runtime error seen by this thread inside the library; returns MMB200_ERR_LAUNCH.
 int record_cuda_error(cudaError_t err);
 

@@ -1342,6 +1342,10 @@ void staged_test_hooks(int wait_polls, int announce_extra) {
   g_wait_polls.store(wait_polls > 0 ? wait_polls : WAIT_POLLS);
   g_announce_extra.store(announce_extra > 0 ? announce_extra : 0);
 }
+void staged_wait_limits(int* wait_polls, int* announce_extra) {
+  *wait_polls = g_wait_polls.load();
+  *announce_extra = g_announce_extra.load();
+}
 
 cudaError_t launch_staged(const Params& p_in, int nfma, void* workspace, size_t workspace_bytes, cudaStream_t stream,
                           int* launches) {
@@ -1454,10 +1458,9 @@ cudaError_t launch_staged(const Params& p_in, int nfma, void* workspace, size_t 
   }
   p.only_b = 0;
   p.byte_loads = vector_loads(p) ? 0 : 1;
-  p.status = reinterpret_cast<int*>(base + w.status);
+  p.status = p.status_word ? p.status_word : reinterpret_cast<int*>(base + w.status);
   p.plan_group = plan.group;
-  p.wait_polls = g_wait_polls.load();
-  p.test_announce_extra = g_announce_extra.load();
+  staged_wait_limits(&p.wait_polls, &p.test_announce_extra);
   cudaError_t err = cudaMemsetAsync(base + w.flag_a, 0, w.a - w.flag_a, stream);     // row flags and status word
   if (err != cudaSuccess) return err;
   if (p.S > 1 || p.slices > 1) {

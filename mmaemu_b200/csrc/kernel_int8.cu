@@ -1,0 +1,498 @@
+// Products of int8 matrices with a scale for each row and column: y = out(fma(RN32(acc), RN32(sa sb), bias)), acc the exact
+// int32 sum over k (K <= 131071, so |acc| <= 2^14 K < 2^31). Dense, or for ragged groups of rows with a weight matrix each.
+//
+// tcgen05.mma kind::i8 (int8 x int8 into int32 in TMEM). The weights' output channels are the 128 lanes of the accumulator
+// and the rows (tokens) its columns, so few rows make a narrow tile instead of an empty one, the channel's scale and bias are
+// one register per thread, and the stores of a warp cover 32 consecutive outputs of a row.
+//
+// int8_tile_kernel: one tile of 128 channels x BT rows per cluster; the CTAs of a cluster each take a part of K and add their
+// int32 sums through distributed shared memory. Integer sums are exact in any order, so the split changes no bit.
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include <atomic>
+#include <cstring>
+
+#include "int8.h"
+#include "staging.cuh"
+
+namespace mmb {
+namespace {
+
+__device__ int g_int8_status;
+
+constexpr int CH = 128;                    // output channels of a tile
+constexpr int KB = 128;                    // bytes of K per stage: one 128-byte swizzle atom
+constexpr int TILE_THREADS = 192;          // warp 0: copies, warp 1: MMAs, warps 2 to 5: output
+
+// ---- device helpers
+__device__ __forceinline__ uint64_t desc_sw128(const void* ptr) {      // K-major, 128-byte swizzle, 8-row groups 1024 bytes apart
+  return ((uint64_t)(smem_addr(ptr) >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void commit(unsigned long long* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, unsigned long long* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ int remote_int(uint32_t addr, int rank) {
+  uint32_t there;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(there) : "memory");
+  return v;
+}
+template <int N>
+__device__ __forceinline__ void tmem_load(int (&r)[N], uint32_t addr);
+template <>
+__device__ __forceinline__ void tmem_load<16>(int (&r)[16], uint32_t addr) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+               "[%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int q = 0; q < 16; ++q) asm volatile("" : "+r"(r[q])::"memory");
+}
+
+// ---- the output of one thread: channel n of group g
+template <int OUT> struct OutType;
+template <> struct OutType<MMB200_OUT_F32> { using type = uint32_t; };
+template <> struct OutType<MMB200_OUT_BF16> { using type = uint16_t; };
+template <> struct OutType<MMB200_OUT_F16> { using type = uint16_t; };
+
+__device__ __forceinline__ float bias_at(const Int8Params& p, long long i) {
+  if (!p.bias) return 0.0f;
+  if (p.bias_dtype == MMB200_HP_F32) return __ldg(static_cast<const float*>(p.bias) + i);
+  if (p.bias_dtype == MMB200_HP_F16) return __half2float(__ldg(static_cast<const __half*>(p.bias) + i));
+  return __uint_as_float((uint32_t)__ldg(static_cast<const uint16_t*>(p.bias) + i) << 16);
+}
+template <int OUT>
+__device__ __forceinline__ typename OutType<OUT>::type out_bits(float y) {
+  if constexpr (OUT == MMB200_OUT_BF16) return f32_to_bf16_bits(y);
+  else if constexpr (OUT == MMB200_OUT_F16) return f32_to_f16_bits(y);
+  else {
+    const uint32_t u = __float_as_uint(y);
+    return (u & 0x7FFFFFFFu) > 0x7F800000u ? CANON_NAN32 : u;
+  }
+}
+
+// ---- groups. Ends are taken as a running maximum, clamped to [0, T], so that no content of offs leads out of the operands.
+struct Group { int g, start, end, tile; };       // g < 0: no such tile
+// The group of tile `slot` of BT rows, found by one warp (every lane returns it).
+template <int BT>
+__device__ __forceinline__ Group find_group(const Int8Params& p, int slot) {
+  if (!p.offs) return Group{0, 0, p.T, slot};
+  const int lane = threadIdx.x % 32;
+  int tiles = 0, last = 0;
+  for (int base = 0; base < p.E; base += 32) {
+    int end = base + lane < p.E ? min(max(__ldg(p.offs + base + lane), 0), p.T) : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int other = __shfl_up_sync(0xFFFFFFFFu, end, d);
+      if (lane >= d) end = max(end, other);
+    }
+    end = max(end, last);
+    int start = __shfl_up_sync(0xFFFFFFFFu, end, 1);
+    if (lane == 0) start = last;
+    int upto = (end - start + BT - 1) / BT;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int other = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+      if (lane >= d) upto += other;
+    }
+    upto += tiles;
+    const unsigned after = __ballot_sync(0xFFFFFFFFu, upto > slot);
+    if (after) {
+      const int l = __ffs(after) - 1;
+      Group r;
+      r.g = base + l;
+      r.start = __shfl_sync(0xFFFFFFFFu, start, l);
+      r.end = __shfl_sync(0xFFFFFFFFu, end, l);
+      const int before = __shfl_sync(0xFFFFFFFFu, upto - (end - start + BT - 1) / BT, l);
+      r.tile = slot - before;
+      return r;
+    }
+    tiles = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    last = __shfl_sync(0xFFFFFFFFu, end, 31);
+  }
+  return Group{-1, last, p.T, 0};                 // start: the first row behind the last group
+}
+
+template <int BT>
+constexpr int tile_stages() { return BT <= 16 ? 6 : (BT <= 32 ? 5 : 4); }
+template <int BT>
+struct SmemTile {
+  static constexpr int STAGES = tile_stages<BT>();
+  struct Stage { unsigned char w[CH * KB], a[BT * KB]; } stage[STAGES];
+  unsigned long long full[STAGES], empty[STAGES], done;
+  uint32_t tmem;
+  Group group;
+};
+
+template <int BT, int OUT>
+__global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                                 const __grid_constant__ CUtensorMap map_a,
+                                                                 const __grid_constant__ Int8Params p) {
+  using Smem = SmemTile<BT>;
+  constexpr int STAGES = Smem::STAGES, COLS = BT < 32 ? 32 : BT;
+  static_assert(STAGES * sizeof(typename Smem::Stage) >= (size_t)BT * CH * 4, "partial sums reuse the stages");
+  extern __shared__ unsigned char smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u));
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  int rank, parts;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
+  const int n0 = (int)(blockIdx.x / (unsigned)parts) * CH;
+  const int kb0 = (int)((long long)p.k_blocks * rank / parts), nk = (int)((long long)p.k_blocks * (rank + 1) / parts) - kb0;
+  if (threadIdx.x == 0) {
+    for (int q = 0; q < STAGES; ++q) { mbar_init(&sm.full[q], 1); mbar_init(&sm.empty[q], 1); }
+    mbar_init(&sm.done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "n"(COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (warp == 2) {
+    const Group found = find_group<BT>(p, (int)blockIdx.y);
+    if (lane == 0) sm.group = found;
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sm.tmem;
+  const Group g = sm.group;
+  const int row0 = g.start + g.tile * BT;
+  const bool work = g.g >= 0 && row0 < g.end;     // the same for every CTA of the cluster
+  bool ok = true;
+  if (work && nk > 0) {
+    if (warp == 0) {
+      if (lane == 0) {
+        int issued = 0;
+        for (int t = 0; t < nk; ++t) {
+          const int s = t % STAGES;
+          if (t >= STAGES && !mbar_wait(&sm.empty[s], ((t / STAGES) - 1) & 1, p.wait_polls)) { ok = false; break; }
+          mbar_expect_tx(&sm.full[s], (uint32_t)sizeof(typename Smem::Stage) + (uint32_t)p.announce_extra);
+          tma_3d(sm.stage[s].w, &map_w, (kb0 + t) * KB, n0, g.g, &sm.full[s]);
+          tma_2d(sm.stage[s].a, &map_a, (kb0 + t) * KB, row0, &sm.full[s]);
+          issued = t + 1;
+        }
+        // the CTA must not end while a copy may be in flight: wait for the last copy into every stage (bounded)
+        for (int t = issued > STAGES ? issued - STAGES : 0; t < issued; ++t)
+          if (!mbar_wait(&sm.full[t % STAGES], (t / STAGES) & 1, p.wait_polls)) ok = false;
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      if (lane == 0) {
+        // int32 accumulator, signed 8-bit operands, both K-major
+        constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BT >> 3) << 17) | ((uint32_t)(CH >> 4) << 24);
+        for (int t = 0; t < nk; ++t) {
+          const int s = t % STAGES;
+          if (!mbar_wait(&sm.full[s], (t / STAGES) & 1, p.wait_polls)) { ok = false; break; }
+          fence_after();
+          const uint64_t dw = desc_sw128(sm.stage[s].w), da = desc_sw128(sm.stage[s].a);
+#pragma unroll
+          for (int k = 0; k < KB / 32; ++k)         // 32 k per instruction: 32 bytes further inside the swizzle atom
+            mma_i8(tmem, dw + 2 * k, da + 2 * k, IDESC, t > 0 || k > 0 ? 1u : 0u);
+          commit(&sm.empty[s]);
+        }
+        commit(&sm.done);
+      }
+      __syncwarp();
+    }
+    // everyone: the products of this CTA are complete (a failed role still commits, so this ends)
+    if (!mbar_wait(&sm.done, 0, p.wait_polls)) ok = false;
+    fence_after();
+  }
+  if (!ok) atomicExch(p.status, 1);
+  const bool bad = __syncthreads_or(ok ? 0 : 1) != 0;
+  const int lane_ch = 32 * (warp % 4) + lane, n = n0 + lane_ch;
+  const uint32_t mine = tmem + ((uint32_t)(32 * (warp % 4)) << 16);
+  int* part = reinterpret_cast<int*>(&sm.stage[0]);                 // [column][channel]
+  if (parts > 1) {
+    if (warp >= 2 && work) {
+#pragma unroll 1
+      for (int c = 0; c < BT; c += 16) {
+        int r[16];
+        if (nk > 0) {
+          tmem_load(r, mine + c);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 16; ++q) r[q] = 0;
+        }
+#pragma unroll
+        for (int q = 0; q < 16; ++q) part[(c + q) * CH + lane_ch] = r[q];
+      }
+    }
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (work && warp >= 2 && !bad && n < p.N) {
+    using O = typename OutType<OUT>::type;
+    const float sb = __ldg(p.scale_b + (long long)g.g * p.sb_group + (long long)n * p.sb_stride);
+    const float bias = bias_at(p, (long long)g.g * p.bias_group + n);
+    O* out = static_cast<O*>(p.d) + n;
+    auto write = [&](int row, int acc) {
+      const float alpha = __fmul_rn(__ldg(p.scale_a + (long long)row * p.sa_stride), sb);
+      out[(long long)row * p.ldd] = out_bits<OUT>(__fmaf_rn(__int2float_rn(acc), alpha, bias));
+    };
+    if (parts > 1) {
+      const int c0 = BT * rank / parts, c1 = BT * (rank + 1) / parts;
+      for (int c = c0; c < c1 && row0 + c < g.end; ++c) {
+        int acc = 0;
+        for (int q = 0; q < parts; ++q) acc += remote_int(smem_addr(part + c * CH + lane_ch), q);
+        write(row0 + c, acc);
+      }
+    }
+  }
+  if (work && warp >= 2 && !bad && parts == 1) {    // TMEM loads take whole warps
+    using O = typename OutType<OUT>::type;
+    const bool real = n < p.N;
+    const float sb = real ? __ldg(p.scale_b + (long long)g.g * p.sb_group + (long long)n * p.sb_stride) : 0.0f;
+    const float bias = real ? bias_at(p, (long long)g.g * p.bias_group + n) : 0.0f;
+    O* out = static_cast<O*>(p.d) + n;
+#pragma unroll 1
+    for (int c = 0; c < BT && row0 + c < g.end; c += 16) {
+      int r[16];
+      if (nk > 0) {
+        tmem_load(r, mine + c);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) r[q] = 0;
+      }
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const int row = row0 + c + q;
+        if (real && row < g.end) {
+          const float alpha = __fmul_rn(__ldg(p.scale_a + (long long)row * p.sa_stride), sb);
+          out[(long long)row * p.ldd] = out_bits<OUT>(__fmaf_rn(__int2float_rn(r[q]), alpha, bias));
+        }
+      }
+    }
+  }
+  if (parts > 1) {                                  // nobody leaves while its sums may be read
+    cluster_arrive();
+    cluster_wait();
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLS));
+  }
+}
+
+// Rows behind the last group: zero.
+__global__ void __launch_bounds__(256) zero_rest_kernel(const __grid_constant__ Int8Params p) {
+  __shared__ int first;
+  if (threadIdx.x < 32) {
+    int last = 0;
+    for (int e = threadIdx.x; e < p.E; e += 32) last = max(last, min(max(__ldg(p.offs + e), 0), p.T));
+    last = __reduce_max_sync(0xFFFFFFFFu, last);
+    if (threadIdx.x == 0) first = last;
+  }
+  __syncthreads();
+  const int es = p.out_dtype == MMB200_OUT_F32 ? 4 : 2;
+  for (long long row = (long long)first + blockIdx.x; row < p.T; row += gridDim.x) {
+    unsigned char* d = static_cast<unsigned char*>(p.d) + row * p.ldd * es;
+    for (int n = threadIdx.x; n < p.N; n += 256) {
+      if (es == 4) reinterpret_cast<uint32_t*>(d)[n] = 0;
+      else reinterpret_cast<uint16_t*>(d)[n] = 0;
+    }
+  }
+}
+
+// Rows of any alignment -> rows of `pitch` bytes (a multiple of 16) that TMA can read. The bytes behind K are not read.
+__global__ void __launch_bounds__(256) repack_kernel(const int8_t* src, long long ld, long long group_stride, long long rows_per_group,
+                                                     long long rows, int K, int8_t* dst, long long pitch) {
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const int8_t* s = src + row / rows_per_group * group_stride + row % rows_per_group * ld;
+    int8_t* d = dst + row * pitch;
+    for (int k = threadIdx.x * 4; k < K; k += 1024) {
+      uint32_t v = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (k + q < K) v |= (uint32_t)(uint8_t)__ldg(s + k + q) << (8 * q);
+      *reinterpret_cast<uint32_t*>(d + k) = v;
+    }
+  }
+}
+
+// ---- host
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+  static std::atomic<EncodeFn> cached{nullptr};
+  EncodeFn fn = cached.load(std::memory_order_acquire);
+  if (fn) return fn;
+  void* entry = nullptr;
+  cudaDriverEntryPointQueryResult found;
+  if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+      found != cudaDriverEntryPointSuccess || !entry)
+    return nullptr;
+  fn = reinterpret_cast<EncodeFn>(entry);
+  cached.store(fn, std::memory_order_release);
+  return fn;
+}
+// A map of bytes [groups][rows][K] with boxes of box_rows rows and 128 bytes, 128-byte swizzle, zeros outside.
+cudaError_t byte_map(CUtensorMap* map, const void* base, int K, long long rows, long long ld, int groups, long long group_stride,
+                     int box_rows, bool three) {
+  const EncodeFn fn = encoder();
+  if (!fn) return cudaErrorNotSupported;
+  const cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)groups};
+  const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)group_stride};
+  const cuuint32_t box[3] = {KB, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, three ? 3 : 2, const_cast<void*>(base), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+// TMA reads rows in place when every row starts on 16 bytes and the strides are below 2^40.
+bool in_place(const void* base, long long ld, long long rows, long long group_stride, int groups) {
+  if (reinterpret_cast<uintptr_t>(base) & 15) return false;
+  if (rows > 1 && ((ld & 15) || ld >= (1ll << 40))) return false;
+  return groups <= 1 || (group_stride > 0 && !(group_stride & 15) && group_stride < (1ll << 40));
+}
+long long pitch_of(int K) { return ((long long)K + 127) / 128 * 128; }
+
+int sms() {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+  cached[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+struct Maps { CUtensorMap w, a; };
+
+template <int BT, int OUT>
+cudaError_t launch_tile(const Int8Params& p, const Maps& m, int parts, unsigned tiles_t, cudaStream_t st) {
+  auto kern = int8_tile_kernel<BT, OUT>;
+  constexpr size_t SMEM = sizeof(SmemTile<BT>) + 1024;
+  static_assert(SMEM <= 232448, "shared memory of a CTA");
+  cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.tiles_n * parts), tiles_t);
+  cfg.blockDim = dim3(TILE_THREADS);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, m.w, m.a, p);
+}
+template <int BT>
+cudaError_t launch_out(const Int8Params& p, const Maps& m, int parts, unsigned tiles_t, cudaStream_t st) {
+  switch (p.out_dtype) {
+    case MMB200_OUT_F32: return launch_tile<BT, MMB200_OUT_F32>(p, m, parts, tiles_t, st);
+    case MMB200_OUT_BF16: return launch_tile<BT, MMB200_OUT_BF16>(p, m, parts, tiles_t, st);
+    default: return launch_tile<BT, MMB200_OUT_F16>(p, m, parts, tiles_t, st);
+  }
+}
+
+}  // namespace
+
+cudaError_t int8_status_word(int** word) { return cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_int8_status); }
+
+size_t int8_workspace_bytes(const Int8Params& p) {
+  size_t n = 0;
+  if (p.K <= 0) return 0;
+  if (!in_place(p.a, p.lda, p.T, 0, 1)) n += (size_t)p.T * pitch_of(p.K);
+  if (!in_place(p.w, p.ldw, p.N, p.gsw, p.E)) n += (size_t)p.E * p.N * pitch_of(p.K);
+  return n;
+}
+
+namespace {
+cudaError_t launch_zero_rest(const Int8Params& p, cudaStream_t st, int* launches) {
+  if (!p.offs || !p.zero_rest) return cudaSuccess;
+  zero_rest_kernel<<<(unsigned)sms(), 256, 0, st>>>(p);
+  const cudaError_t err = cudaGetLastError();
+  if (err == cudaSuccess) *launches += 1;
+  return err;
+}
+}  // namespace
+
+cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st, int* launches) {
+  Int8Params p = p_in;
+  if (p.E == 0) return launch_zero_rest(p, st, launches);
+  staged_wait_limits(&p.wait_polls, &p.announce_extra);
+  cudaError_t err = int8_status_word(&p.status);
+  if (err != cudaSuccess) return err;
+  int8_t* ws = static_cast<int8_t*>(workspace);
+  if (p.K > 0) {
+    const long long pitch = pitch_of(p.K);
+    const unsigned most = (unsigned)sms() * 16;
+    if (!in_place(p.a, p.lda, p.T, 0, 1)) {
+      repack_kernel<<<(unsigned)(p.T < (int)most ? p.T : (int)most), 256, 0, st>>>(p.a, p.lda, 0, p.T, p.T, p.K, ws, pitch);
+      if ((err = cudaGetLastError()) != cudaSuccess) return err;
+      *launches += 1;
+      p.a = ws;
+      p.lda = pitch;
+      ws += (size_t)p.T * pitch;
+    }
+    if (!in_place(p.w, p.ldw, p.N, p.gsw, p.E)) {
+      const long long rows = (long long)p.E * p.N;
+      repack_kernel<<<(unsigned)(rows < (long long)most ? rows : (long long)most), 256, 0, st>>>(p.w, p.ldw, p.gsw, p.N, rows, p.K, ws, pitch);
+      if ((err = cudaGetLastError()) != cudaSuccess) return err;
+      *launches += 1;
+      p.w = ws;
+      p.ldw = pitch;
+      p.gsw = pitch * p.N;
+    }
+  }
+  p.k_blocks = (p.K + KB - 1) / KB;
+  p.tiles_n = (p.N + CH - 1) / CH;
+  // rows of a tile: a power of two that holds the rows of a group, at most 256
+  const long long per_group = ((long long)p.T + p.E - 1) / p.E;
+  const int bt = per_group <= 16 ? 16 : per_group <= 32 ? 32 : per_group <= 64 ? 64 : per_group <= 128 ? 128 : 256;
+  const long long tiles_t = p.offs ? (long long)p.T / bt + (p.E < p.T ? p.E : p.T) : ((long long)p.T + bt - 1) / bt;
+  if (tiles_t > 65535) return cudaErrorInvalidValue;
+  Maps m;
+  std::memset(&m, 0, sizeof(m));
+  if (p.K > 0) {
+    // (a single row's stride is never used, but the map wants a multiple of 16)
+    const long long ldw = p.N > 1 ? p.ldw : pitch_of(p.K), lda = p.T > 1 ? p.lda : pitch_of(p.K);
+    err = byte_map(&m.w, p.w, p.K, p.N, ldw, p.E, p.E > 1 ? p.gsw : pitch_of(p.K), CH, true);
+    if (err == cudaSuccess) err = byte_map(&m.a, p.a, p.K, p.T, lda, 1, 0, bt, false);
+    if (err != cudaSuccess) return err;
+  }
+  int parts = 1;
+  const long long ctas = (long long)p.tiles_n * tiles_t;
+  while (parts < 8 && bt <= 64 && ctas * parts * 2 <= 2ll * sms() && p.k_blocks >= 4 * parts) parts *= 2;
+  switch (bt) {
+    case 16: err = launch_out<16>(p, m, parts, (unsigned)tiles_t, st); break;
+    case 32: err = launch_out<32>(p, m, parts, (unsigned)tiles_t, st); break;
+    case 64: err = launch_out<64>(p, m, parts, (unsigned)tiles_t, st); break;
+    case 128: err = launch_out<128>(p, m, parts, (unsigned)tiles_t, st); break;
+    default: err = launch_out<256>(p, m, parts, (unsigned)tiles_t, st); break;
+  }
+  if (err != cudaSuccess) return err;
+  *launches += 1;
+  return launch_zero_rest(p, st, launches);
+}
+
+}  // namespace mmb

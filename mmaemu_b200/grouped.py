@@ -1,0 +1,140 @@
+"""grouped_scaled_mm: the emulated FP8 GEMM for ragged groups of rows with weights of their own, in one call.
+
+A mixture-of-experts layer sorts its rows by expert and multiplies every expert's rows with that expert's weights; on the
+emulated platform that is one torch._scaled_mm (Transformer Engine: one cuBLASLt GEMM) per expert. The result here has the
+bits of that loop over `scaled_mm`. The split-K decision of the emulated cuBLASLt depends on a group's number of rows, so
+the group sizes are host integers, as Transformer Engine's grouped linear layers take them (m_splits). The reference has no
+grouped call; its checks and raises (astding/mmaemu, mmaemu/api.py:280-326) apply to every group.
+"""
+from __future__ import annotations
+
+import ctypes
+import os
+
+import torch
+
+from . import _lib
+from .api import (_check_argument_types, _check_like_cublas, _check_like_torch, _check_scope, _emit_maturity, _kernel_choice,
+                  _kernel_code, _misaligned, _on_device, _require_device, _scalar_ptr, _stream_ptr)
+from .errors import ReferenceRejectsError
+from .formats import OUT_DTYPE_NAMES, fmt_of
+from .numerics import check_plan, get_preset
+from .platforms import get_profile
+from .splitk import resolve_splitk
+
+__all__ = ["grouped_scaled_mm"]
+
+MAX_GROUPS = 4096
+
+
+def _sizes(m_splits, E: int, T: int) -> list:
+    if isinstance(m_splits, torch.Tensor):
+        if m_splits.device.type != "cpu":
+            raise TypeError("grouped_scaled_mm(): m_splits is read on the host (the split-K decision depends on it); got a tensor "
+                            f"on {m_splits.device}")
+        if m_splits.is_floating_point() or m_splits.is_complex() or m_splits.dtype == torch.bool:
+            raise TypeError(f"grouped_scaled_mm(): m_splits must hold integers, got {m_splits.dtype}")
+        m_splits = m_splits.tolist()
+    if not isinstance(m_splits, (list, tuple)) or any(isinstance(m, bool) or not isinstance(m, int) for m in m_splits):
+        raise TypeError("grouped_scaled_mm(): m_splits must be a list of ints (or a CPU tensor of integers)")
+    if len(m_splits) != E:
+        raise ValueError(f"grouped_scaled_mm(): mat2 has {E} matrices, m_splits {len(m_splits)} entries")
+    if any(m < 0 for m in m_splits) or sum(m_splits) != T:
+        raise ValueError(f"grouped_scaled_mm(): m_splits must be non-negative and add up to the {T} rows of input, got a sum of "
+                         f"{sum(m_splits)}")
+    return list(m_splits)
+
+
+def _group_scale(name: str, t: torch.Tensor, E: int) -> int:
+    """Stride of a scale over the groups: 0 for one element, else of an [E] tensor."""
+    if t.numel() == 1:
+        return 0
+    if tuple(t.shape) != (E,):
+        raise ValueError(f"grouped_scaled_mm(): {name} must have one element or shape {(E,)}, got {tuple(t.shape)}")
+    return t.stride(0)
+
+
+def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None, out_dtype=None, use_fast_accum=False, *,
+                      out=None, profile=None, splitk="auto", backend="auto"):
+    """scaled_mm of every group of rows, bit for bit: the first m_splits[0] rows of input [T, K] with mat2[0], the next
+    m_splits[1] rows with mat2[1], and so on.
+
+    mat2: [E, K, N] FP8, every matrix column-major (w.transpose(1, 2) of [E, N, K] weights). m_splits: E host integers that
+    add up to T; groups may be empty. scale_a, scale_b: fp32, one element or one per group ([E]). out: a row-major [T, N]
+    tensor of the output dtype to write into. profile, splitk, use_fast_accum, scale_result, out_dtype, backend and every
+    raise: scaled_mm's; splitk="auto" decides for every group by its own number of rows. E <= 4096. Returns [T, N]."""
+    fast = use_fast_accum
+    _check_argument_types(input, mat2, scale_a, scale_b, None, scale_result, out_dtype, fast, out)
+    if mat2.dim() != 3:
+        raise ValueError(f"grouped_scaled_mm(): mat2 must be [E, K, N], got {tuple(mat2.shape)}")
+    if input.dim() != 2:
+        raise ReferenceRejectsError("mat1 must be a matrix")
+    E, N, (T, K) = mat2.shape[0], mat2.shape[2], input.shape
+    if E < 1 or E > MAX_GROUPS:
+        raise ValueError(f"grouped_scaled_mm(): between 1 and {MAX_GROUPS} groups, got {E}")
+    sizes = _sizes(m_splits, E, T)
+    sa, sb = _group_scale("scale_a", scale_a, E), _group_scale("scale_b", scale_b, E)
+    scaling, od = _check_like_torch(input, mat2[0], scale_a.reshape(-1)[:1], scale_b.reshape(-1)[:1], None, scale_result, out_dtype,
+                                    out)
+    prof = get_profile(profile)
+    preset = get_preset(prof.preset)
+    if out is not None and (tuple(out.shape) != (T, N) or (N > 1 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N)):
+        raise ValueError(f"grouped_scaled_mm(): out must be a row-major tensor of shape {(T, N)}, got shape {tuple(out.shape)} with "
+                         f"strides {tuple(out.stride())}")
+    if T == 0 or N == 0 or K == 0:
+        return torch.zeros((T, N), dtype=od, device=input.device) if out is None else out.zero_()
+    mat1 = _check_like_cublas(input, mat2[0], scaling, od)
+    if E > 1 and _misaligned(mat2[1]):
+        raise ReferenceRejectsError("CUBLAS_STATUS_NOT_SUPPORTED when calling cublasLtMatmul (operand pointer not 16-byte aligned)")
+    fa, fb = fmt_of(mat1.dtype), fmt_of(mat2.dtype)
+    rule = prof.rejection(fa, fb, od)
+    if rule is not None:
+        raise ReferenceRejectsError(f"{rule.message} [profile {prof.name}]")
+    _check_scope(scaling, None, (mat1, mat2, scale_a, scale_b, scale_result))
+    _emit_maturity(prof, preset)
+    layout_std = mat1.is_contiguous() and mat2[0].t().is_contiguous()
+    plans = {}                                           # rows of a group -> (splits, scheme)
+    for m in sizes:
+        if m and m not in plans:
+            d = resolve_splitk(m, N, K, a_dtype=mat1.dtype, b_dtype=mat2.dtype, out_dtype=od, use_fast_accum=fast, profile=prof,
+                               splitk=splitk, layout_std=layout_std, dry=False)
+            plans[m] = (d.S, check_plan(preset, K, d.S, d.scheme, fast))
+    kernel = _kernel_choice(backend)
+    dev = mat1.device
+    _require_device(dev)
+    a, w = mat1.detach(), mat2.detach()
+    lda = a.stride(0) if T > 1 else K
+    ldb = w.stride(2) if N > 1 else K
+    y = torch.empty((T, N), dtype=od, device=dev) if out is None else out
+    ints = ctypes.c_int * E
+    rows, splits, schemes = ints(*sizes), None, None
+    if any(S > 1 for S, _ in plans.values()):
+        splits = ints(*[plans[m][0] if m else 1 for m in sizes])
+        schemes = ints(*[_lib.SCHEME_CODES[plans[m][1]] if m else 0 for m in sizes])
+    keep_r, pr = (None, None) if scale_result is None else _scalar_ptr(scale_result, dev)
+    L = _lib.load()
+    with _on_device(dev):
+        ws, ws_ptr, n = None, None, 0
+        if kernel not in ("integer", "direct") and not preset.late_c and os.environ.get("MMAEMU_B200_WORKSPACE", "1") != "0":
+            n = int(L.mmb200_grouped_workspace_bytes(rows, splits, E, N, K))
+            if n:
+                try:
+                    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+                    ws_ptr = ws.data_ptr()
+                except torch.OutOfMemoryError:
+                    if kernel != "auto":
+                        raise                            # a request for the fast kernels by name
+                    n = 0
+        rc = L.mmb200_grouped_scaled_mm(a.data_ptr(), lda, _lib.FMT_CODES[fa], w.data_ptr(), ldb, w.stride(0) if E > 1 else 0,
+                                        _lib.FMT_CODES[fb], y.data_ptr(), y.stride(0) if T > 1 else N,
+                                        _lib.OUT_CODES[OUT_DTYPE_NAMES[od]], rows, splits, schemes, E, N, K, preset.code, int(fast),
+                                        scale_a.data_ptr(), sa, scale_b.data_ptr(), sb, pr, _kernel_code(kernel), ws_ptr, n,
+                                        _stream_ptr(dev))
+        _lib.check("mmb200_grouped_scaled_mm", rc)
+        if ws is not None and os.environ.get("MMAEMU_B200_CHECK_STATUS", "0") == "1":
+            _lib.check("mmb200_grouped_status", L.mmb200_grouped_status(ws_ptr, _stream_ptr(dev)))
+    del keep_r, ws
+    return y
+
+
+grouped_scaled_mm = torch.compiler.disable(grouped_scaled_mm)

@@ -1,0 +1,274 @@
+"""int8 products next to the emulated FP8 GEMM: quantize_int8, int8_scaled_mm, int8_grouped_scaled_mm.
+
+    xq, sx = quantize_int8(x)                        # codes [.., K] int8, one fp32 scale per row [.., 1]
+    wq, sw = quantize_int8(w)                        # w: [N, K], one scale per output channel
+    y = int8_scaled_mm(xq, wq.t(), sx, sw.t(), bias, torch.bfloat16)
+
+Integer tensor-core sums are exact on every GPU, so no profile takes part: the result is
+
+    y = out_dtype(RN32(RN32(sum_k a[m, k] b[k, n]) * RN32(scale_a[m] * scale_b[n]) + bias[n]))
+
+with one rounding for the product and the bias together (+0 without one, so a zero result is +0): the epilogue of
+`scaled_mm` with a scale for each row and column.
+The reference has no int8 path. Errors are TypeError for argument types, ValueError for shapes, layouts and devices,
+UnsupportedFeatureError for inputs that require grad, BackendUnavailableError without an sm_100 device. Calls run on the
+current stream of the operands' device, do not synchronise and can be captured into CUDA graphs.
+"""
+from __future__ import annotations
+
+import ctypes
+import os
+
+import torch
+
+from . import _lib
+from .api import _on_device, _require_device
+from .errors import UnsupportedFeatureError
+
+__all__ = ["quantize_int8", "int8_scaled_mm", "int8_grouped_scaled_mm"]
+
+MAX_K = 131071                     # 2^14 * K < 2^31: the int32 sums cannot overflow
+MAX_ROWS = 1 << 23
+MAX_GROUPS = 4096
+_REAL_CODES = {torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}           # MMB200_HP_*
+_OUT_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # MMB200_OUT_*
+_supported: set = set()            # indices of devices that have been checked
+
+
+def _device(t: torch.Tensor) -> torch.device:
+    dev = t.device
+    if dev.type != "cuda" or dev.index not in _supported:
+        _require_device(dev)
+        _supported.add(dev.index)
+    return dev
+
+
+def _tensor(who: str, name: str, t) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{who}(): argument '{name}' must be Tensor, not {type(t).__name__}")
+
+
+def _no_grad(who: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise UnsupportedFeatureError(f"{who}(): inference only: an input requires grad while grad mode is enabled")
+
+
+def _stream(dev: torch.device) -> ctypes.c_void_p:
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(dev.index))
+
+
+def quantize_int8(x):
+    """Symmetric int8 quantisation of every row (last dimension) of x, fp32, bf16 or fp16: (codes, scale).
+
+    scale = amax / 127 (fp32, shape [..., 1]) and codes = the integer nearest to x * 127 / amax, ties to even, decided
+    exactly (int8, the shape of x, contiguous; between -127 and 127). A row of zeros has scale 0; a row with a NaN or an
+    infinity has scale NaN and codes 0, which makes every product with it NaN. Rows quantised this way are the operands of
+    int8_scaled_mm: activations [M, K] give scale_a [M, 1], weights [N, K] give scale_b.t() [1, N]."""
+    _tensor("quantize_int8", "x", x)
+    code = _REAL_CODES.get(x.dtype)
+    if code is None:
+        raise TypeError(f"quantize_int8(): x must be float32, bfloat16 or float16, got {x.dtype}")
+    if x.dim() == 0:
+        raise ValueError("quantize_int8(): x must have at least one dimension")
+    _no_grad("quantize_int8", x)
+    dev = _device(x)
+    K = x.shape[-1]
+    if x.dim() != 2 or (x.stride(1) != 1 and K > 1) or (x.stride(0) < K and x.shape[0] > 1):
+        rows = x.detach().reshape(-1, K) if K else x.detach().reshape(x.shape[:-1].numel(), 0)
+        if (rows.stride(1) != 1 and K > 1) or (rows.stride(0) < K and rows.shape[0] > 1):
+            rows = rows.contiguous()
+    else:
+        rows = x
+    codes = torch.empty(x.shape, dtype=torch.int8, device=dev)
+    scale = torch.empty(x.shape[:-1] + (1,), dtype=torch.float32, device=dev)
+    n = rows.shape[0]
+    if n == 0:
+        return codes, scale
+    L = _lib.load()
+    with _on_device(dev):
+        rc = L.mmb200_quantize_int8(rows.data_ptr(), rows.stride(0) if n > 1 else K, code, codes.data_ptr(), K,
+                                    scale.data_ptr(), n, K, _stream(dev))
+    if rc:
+        _lib.check("mmb200_quantize_int8", rc)
+    return codes, scale
+
+
+def _matrix(who: str, t: torch.Tensor, rows: int, K: int):
+    """(tensor, row stride) of a [rows, K] int8 operand whose rows the kernels can read: unit stride along K, no overlap."""
+    t = t.detach()
+    if (K > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < K):
+        t = t.contiguous()
+    return t, (t.stride(0) if rows > 1 else K)
+
+
+def _scale_a(who, scale_a, rows):
+    if scale_a.dtype != torch.float32:
+        raise ValueError(f"{who}(): scale_a must be float32, got {scale_a.dtype}")
+    if scale_a.numel() == 1:
+        return 0
+    if tuple(scale_a.shape) != (rows, 1):
+        raise ValueError(f"{who}(): scale_a must have one element or shape {(rows, 1)}, got {tuple(scale_a.shape)}")
+    return scale_a.stride(0)
+
+
+def _output(who, out, out_dtype, rows, N):
+    """(dtype, its code) of the output; out checked."""
+    if out_dtype is not None and not isinstance(out_dtype, torch.dtype):
+        raise TypeError(f"{who}(): argument 'out_dtype' must be torch.dtype, not {type(out_dtype).__name__}")
+    if out is not None and out_dtype is not None and out_dtype != out.dtype:
+        raise ValueError(f"{who}(): out_dtype must match the dtype of out ({out_dtype}, {out.dtype})")
+    dtype = out.dtype if out is not None else torch.bfloat16 if out_dtype is None else out_dtype
+    code = _OUT_CODES.get(dtype)
+    if code is None:
+        raise ValueError(f"{who}(): the output is float32, bfloat16 or float16, got {dtype}")
+    if out is not None and (tuple(out.shape) != (rows, N) or (N > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < N)):
+        raise ValueError(f"{who}(): out must be a row-major tensor of shape {(rows, N)}, got shape {tuple(out.shape)} with strides "
+                         f"{tuple(out.stride())}")
+    return dtype, code
+
+
+def _bias(who, bias, shape):
+    """(tensor or None, pointer or None, code of the dtype)"""
+    if bias is None:
+        return None, None, 0
+    code = _REAL_CODES.get(bias.dtype)
+    if code is None:
+        raise ValueError(f"{who}(): bias must be float32, bfloat16 or float16, got {bias.dtype}")
+    if tuple(bias.shape) != shape:
+        raise ValueError(f"{who}(): bias must have shape {shape}, got {tuple(bias.shape)}")
+    bias = bias.detach().contiguous()
+    return bias, bias.data_ptr(), code
+
+
+def _check_operands(who, input, mat2, scale_a, scale_b, bias, out, others=()):
+    _tensor(who, "input", input)
+    _tensor(who, "mat2", mat2)
+    _tensor(who, "scale_a", scale_a)
+    _tensor(who, "scale_b", scale_b)
+    if bias is not None:
+        _tensor(who, "bias", bias)
+    if out is not None:
+        _tensor(who, "out", out)
+    if input.dtype != torch.int8 or mat2.dtype != torch.int8:
+        raise TypeError(f"{who}(): input and mat2 must be int8, got {input.dtype} and {mat2.dtype}")
+    dev = input.device
+    for t in (mat2, scale_a, scale_b, bias, out, *others):
+        if isinstance(t, torch.Tensor) and t.device != dev:
+            raise ValueError(f"{who}(): expected all tensors on one device, found {dev} and {t.device}")
+    _no_grad(who, scale_a, scale_b, bias, out)
+
+
+def _run(who, dev, a, lda, w, ldw, gsw, y, ldd, code, T, N, K, E, offs, scale_a, sa, scale_b, sb_group, sb, bias, bias_code,
+         bias_group, zero_rest):
+    L = _lib.load()
+    ap, wp = a.data_ptr(), w.data_ptr()
+    with _on_device(dev):
+        ws, ws_ptr, n = None, None, 0
+        if (ap | wp | lda | ldw | gsw) & 15 or (E > 1 and not gsw):     # rows that TMA cannot read in place: room for copies
+            n = int(L.mmb200_int8_workspace_bytes(ap, lda, wp, ldw, gsw, T, N, K, E))
+            if n:
+                ws = torch.empty(n, dtype=torch.uint8, device=dev)
+                ws_ptr = ws.data_ptr()
+        stream = _stream(dev)
+        rc = L.mmb200_int8_scaled_mm(ap, lda, wp, ldw, gsw, y.data_ptr(), ldd, code, T, N, K, E, offs, scale_a.data_ptr(), sa,
+                                     scale_b.data_ptr(), sb_group, sb, bias, bias_code, bias_group, zero_rest, ws_ptr, n, stream)
+        if rc:
+            _lib.check("mmb200_int8_scaled_mm", rc)
+        if os.environ.get("MMAEMU_B200_CHECK_STATUS") == "1":
+            _lib.check("mmb200_int8_status", L.mmb200_int8_status(stream))
+    return y
+
+
+def int8_scaled_mm(input, mat2, scale_a, scale_b, bias=None, out_dtype=None, *, out=None):
+    """input [M, K] int8 times mat2 [K, N] int8 (column-major: w.t() of a row-major [N, K] weight) with exact int32 sums,
+    scaled: out_dtype(sum * (scale_a * scale_b) + bias), the arithmetic of the module docstring.
+
+    scale_a: one element or [M, 1], scale_b: one element or [1, N], fp32. bias: [N] fp32, bf16 or fp16. out_dtype: bfloat16
+    (default), float16 or float32. out: a row-major [M, N] tensor of the output dtype (any row stride) to write into.
+    K <= 131071, M <= 2^23. Rows of any alignment and stride are served; those that do not start on 16 bytes are copied
+    first."""
+    who = "int8_scaled_mm"
+    _check_operands(who, input, mat2, scale_a, scale_b, bias, out)
+    if input.dim() != 2 or mat2.dim() != 2 or input.shape[1] != mat2.shape[0]:
+        raise ValueError(f"{who}(): expected input [M, K] and mat2 [K, N], got {tuple(input.shape)} and {tuple(mat2.shape)}")
+    (M, K), N = input.shape, mat2.shape[1]
+    if K > MAX_K or M > MAX_ROWS:
+        raise ValueError(f"{who}(): K is at most {MAX_K} (int32 sums) and M at most {MAX_ROWS}, got K = {K}, M = {M}")
+    if K > 1 and N > 0 and mat2.stride(0) != 1:
+        raise ValueError(f"{who}(): mat2 must be column-major (the transpose of a row-major [N, K] weight), got strides "
+                         f"{tuple(mat2.stride())}")
+    sa = _scale_a(who, scale_a, M)
+    if scale_b.dtype != torch.float32:
+        raise ValueError(f"{who}(): scale_b must be float32, got {scale_b.dtype}")
+    if scale_b.numel() == 1:
+        sb = 0
+    elif tuple(scale_b.shape) == (1, N):
+        sb = scale_b.stride(1)
+    else:
+        raise ValueError(f"{who}(): scale_b must have one element or shape {(1, N)}, got {tuple(scale_b.shape)}")
+    bias, bias_ptr, bias_code = _bias(who, bias, (N,))
+    dtype, code = _output(who, out, out_dtype, M, N)
+    dev = _device(input)
+    y = torch.empty((M, N), dtype=dtype, device=dev) if out is None else out
+    ldd = y.stride(0) if M > 1 else N
+    if M == 0 or N == 0:
+        return y
+    a, lda = _matrix(who, input, M, K)
+    w, ldw = _matrix(who, mat2.t(), N, K)
+    return _run(who, dev, a, lda, w, ldw, 0, y, ldd, code, M, N, K, 1, None, scale_a, sa, scale_b, 0, sb, bias_ptr, bias_code, 0, 0)
+
+
+def int8_grouped_scaled_mm(input, mat2, offs, scale_a, scale_b, bias=None, out_dtype=None, *, out=None):
+    """int8_scaled_mm for ragged groups of rows with weights of their own (rows sorted by expert): the rows
+    offs[e - 1] .. offs[e] - 1 of input [T, K] are multiplied with mat2[e].
+
+    mat2: [E, K, N] int8, every matrix column-major (w.transpose(1, 2) of [E, N, K] weights). offs: int32 [E] on the device,
+    the end of every group's rows; it is read by the kernels, never by the host, so routing decided on the GPU needs no
+    synchronisation. Groups may be empty. Ends are taken as a running maximum and clamped to [0, T]. scale_a: one element or
+    [T, 1]; scale_b: one element or [E, 1, N]; bias: [E, N]. Rows behind the last group (a padded batch) are zero in a new
+    output and keep their contents in `out`. Everything else as int8_scaled_mm; E <= 4096."""
+    who = "int8_grouped_scaled_mm"
+    _tensor(who, "offs", offs)
+    _check_operands(who, input, mat2, scale_a, scale_b, bias, out, (offs,))
+    if input.dim() != 2 or mat2.dim() != 3 or input.shape[1] != mat2.shape[1]:
+        raise ValueError(f"{who}(): expected input [T, K] and mat2 [E, K, N], got {tuple(input.shape)} and {tuple(mat2.shape)}")
+    (T, K), E, N = input.shape, mat2.shape[0], mat2.shape[2]
+    if K > MAX_K or T > MAX_ROWS or E > MAX_GROUPS:
+        raise ValueError(f"{who}(): K is at most {MAX_K} (int32 sums), T at most {MAX_ROWS} and E at most {MAX_GROUPS}, got K = {K}, "
+                         f"T = {T}, E = {E}")
+    if offs.dtype != torch.int32 or tuple(offs.shape) != (E,):
+        raise ValueError(f"{who}(): offs must be int32 of shape {(E,)}, got {offs.dtype} of shape {tuple(offs.shape)}")
+    if K > 1 and N > 0 and E > 0 and mat2.stride(1) != 1:
+        raise ValueError(f"{who}(): every matrix of mat2 must be column-major (the transpose of row-major [E, N, K] weights), got "
+                         f"strides {tuple(mat2.stride())}")
+    sa = _scale_a(who, scale_a, T)
+    if scale_b.dtype != torch.float32:
+        raise ValueError(f"{who}(): scale_b must be float32, got {scale_b.dtype}")
+    if scale_b.numel() == 1:
+        sb_group = sb = 0
+    elif tuple(scale_b.shape) == (E, 1, N):
+        sb_group, sb = scale_b.stride(0), scale_b.stride(2)
+    else:
+        raise ValueError(f"{who}(): scale_b must have one element or shape {(E, 1, N)}, got {tuple(scale_b.shape)}")
+    bias, bias_ptr, bias_code = _bias(who, bias, (E, N))
+    dtype, code = _output(who, out, out_dtype, T, N)
+    dev = _device(input)
+    y = torch.empty((T, N), dtype=dtype, device=dev) if out is None else out
+    ldd = y.stride(0) if T > 1 else N
+    if T == 0 or N == 0:
+        return y
+    if E == 0:
+        return y.zero_() if out is None else y
+    a, lda = _matrix(who, input, T, K)
+    w = mat2.detach()
+    if N > 1 and w.stride(2) < K:
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    offs = offs.contiguous()
+    return _run(who, dev, a, lda, w, w.stride(2) if N > 1 else K, w.stride(0) if E > 1 else 0, y, ldd, code, T, N, K, E,
+                offs.data_ptr(), scale_a, sa, scale_b, sb_group, sb, bias_ptr, bias_code, N, int(out is None))
+
+
+# torch.compile must not trace into these entry points (they call a foreign library through ctypes)
+quantize_int8 = torch.compiler.disable(quantize_int8)
+int8_scaled_mm = torch.compiler.disable(int8_scaled_mm)
+int8_grouped_scaled_mm = torch.compiler.disable(int8_grouped_scaled_mm)
