@@ -7,6 +7,10 @@
 //
 // int8_tile_kernel: one tile of 128 channels x BT rows per cluster; the CTAs of a cluster each take a part of K and add their
 // int32 sums through distributed shared memory. Integer sums are exact in any order, so the split changes no bit.
+//
+// int8_pair_kernel: many rows. Two CTAs on neighbouring SMs (cta_group::2) work on a tile of 256 channels x 256 rows, each
+// holding half of both operands, so a byte of shared memory feeds twice the products; persistent, and TMEM holds two
+// accumulators, so the output of a tile leaves while the next one is multiplied.
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -298,6 +302,182 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
   }
 }
 
+// ---- pairs of CTAs
+constexpr int PAIR_STAGES = 6, PAIR_T = 256;
+constexpr int PAIR_BAND = 8;               // tiles of rows that share a pass over the channels (16 MB of rows at K = 8192 stay in L2)
+struct SmemPair {
+  struct Stage { unsigned char w[CH * KB], a[CH * KB]; } stage[PAIR_STAGES];
+  unsigned long long full[PAIR_STAGES];    // leader: both CTAs' copies of the stage have landed
+  unsigned long long empty[PAIR_STAGES];   // the MMAs that read the stage are done
+  unsigned long long acc_full[2];          // the accumulator is complete
+  unsigned long long acc_empty[2];         // leader: all eight output warps have read it
+  unsigned long long drain;
+  uint32_t tmem;
+};
+__device__ __forceinline__ uint32_t leader_addr(const void* ptr) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(ptr)));
+  return a;
+}
+__device__ __forceinline__ void tma_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_3d_pair(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void commit_pair(unsigned long long* bar) {       // arrives at the barrier of both CTAs
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(smem_addr(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// The tiles of a launch in order: group by group, inside a group bands of PAIR_BAND tiles of rows, inside a band channel tile
+// by channel tile. A worker walks an increasing sequence of indices; every role of a CTA has a walker of its own.
+struct Walker {
+  int g = -1, start = 0, end = 0, tiles_t = 0;
+  long long base = 0, count = 0;           // tiles before the group, tiles of the group
+  __device__ __forceinline__ bool find(const Int8Params& p, int tiles_n, long long t, int& row0, int& n_tile) {
+    while (t >= base + count) {
+      base += count;
+      if (++g >= p.E) return false;
+      start = end;
+      end = p.offs ? max(end, min(max(__ldg(p.offs + g), 0), p.T)) : p.T;
+      tiles_t = (end - start + PAIR_T - 1) / PAIR_T;
+      count = (long long)tiles_t * tiles_n;
+    }
+    const long long i = t - base, per_band = (long long)PAIR_BAND * tiles_n;
+    const int band = (int)(i / per_band), j = (int)(i - band * per_band), width = min(PAIR_BAND, tiles_t - band * PAIR_BAND);
+    n_tile = j / width;
+    row0 = start + (band * PAIR_BAND + j % width) * PAIR_T;
+    return true;
+  }
+};
+
+template <int OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1)
+    int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
+                     const __grid_constant__ Int8Params p) {
+  extern __shared__ unsigned char smem_raw[];
+  SmemPair& sm = *reinterpret_cast<SmemPair*>(smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u));
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  int rank;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int tiles_n = (p.N + 2 * CH - 1) / (2 * CH), nk = p.k_blocks;
+  const long long first = blockIdx.x / 2, step = gridDim.x / 2;
+  if (threadIdx.x == 0) {
+    for (int q = 0; q < PAIR_STAGES; ++q) { mbar_init(&sm.full[q], 1); mbar_init(&sm.empty[q], 1); }
+    for (int q = 0; q < 2; ++q) { mbar_init(&sm.acc_full[q], 1); mbar_init(&sm.acc_empty[q], 8); }
+    mbar_init(&sm.drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sm.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  cluster_arrive();                                 // the other CTA's barriers and TMEM are ready too
+  cluster_wait();
+  fence_after();
+  const uint32_t tmem = sm.tmem;
+  bool ok = true;
+  Walker walk;
+  int row0, n_tile;
+  if (warp == 0) {
+    if (lane == 0) {
+      unsigned it = 0;
+      for (long long t = first; ok && walk.find(p, tiles_n, t, row0, n_tile); t += step) {
+        for (int kb = 0; kb < nk; ++kb, ++it) {
+          const unsigned s = it % PAIR_STAGES, round = it / PAIR_STAGES;
+          if (round && !mbar_wait(&sm.empty[s], (round - 1) & 1, p.wait_polls)) { ok = false; break; }
+          if (rank == 0) mbar_expect_tx(&sm.full[s], 2 * (uint32_t)sizeof(SmemPair::Stage) + (uint32_t)p.announce_extra);
+          const uint32_t bar = leader_addr(&sm.full[s]);
+          tma_3d_pair(sm.stage[s].w, &map_w, kb * KB, (2 * n_tile + rank) * CH, walk.g, bar);
+          tma_2d_pair(sm.stage[s].a, &map_a, kb * KB, row0 + CH * rank, bar);
+        }
+      }
+      // no CTA of the pair ends while a copy may be in flight: the leader waits for the last copies into every stage (bounded)
+      if (rank == 0)
+        for (unsigned q = it > PAIR_STAGES ? it - PAIR_STAGES : 0; q < it; ++q)
+          if (!mbar_wait(&sm.full[q % PAIR_STAGES], (q / PAIR_STAGES) & 1, p.wait_polls)) ok = false;
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(PAIR_T >> 3) << 17) | ((uint32_t)(2 * CH >> 4) << 24);
+      unsigned it = 0, i = 0;
+      for (long long t = first; ok && walk.find(p, tiles_n, t, row0, n_tile); t += step, ++i) {
+        const uint32_t acc = tmem + (i & 1) * PAIR_T;
+        if (i >= 2 && !mbar_wait(&sm.acc_empty[i & 1], ((i >> 1) - 1) & 1, p.wait_polls)) { ok = false; break; }
+        fence_after();
+        for (int kb = 0; kb < nk; ++kb, ++it) {
+          const unsigned s = it % PAIR_STAGES;
+          if (!mbar_wait(&sm.full[s], (it / PAIR_STAGES) & 1, p.wait_polls)) { ok = false; break; }
+          fence_after();
+          const uint64_t dw = desc_sw128(sm.stage[s].w), da = desc_sw128(sm.stage[s].a);
+#pragma unroll
+          for (int k = 0; k < KB / 32; ++k) mma_i8_pair(acc, dw + 2 * k, da + 2 * k, IDESC, kb > 0 || k > 0 ? 1u : 0u);
+          commit_pair(&sm.empty[s]);
+        }
+        if (ok) commit_pair(&sm.acc_full[i & 1]);
+      }
+      // nothing in flight when the TMEM is given back
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(&sm.drain)) : "memory");
+      if (!mbar_wait(&sm.drain, 0, WAIT_POLLS)) ok = false;
+    }
+    __syncwarp();
+  } else {
+    using O = typename OutType<OUT>::type;
+    const uint32_t mine = tmem + ((uint32_t)(32 * (warp % 4)) << 16);
+    unsigned i = 0;
+    for (long long t = first; walk.find(p, tiles_n, t, row0, n_tile); t += step, ++i) {
+      const int n = (2 * n_tile + rank) * CH + 32 * (warp % 4) + lane;
+      const bool real = n < p.N;
+      const float sb = real ? __ldg(p.scale_b + (long long)walk.g * p.sb_group + (long long)n * p.sb_stride) : 0.0f;
+      const float bias = real ? bias_at(p, (long long)walk.g * p.bias_group + n) : 0.0f;
+      O* out = static_cast<O*>(p.d) + n;
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.acc_full[i & 1], (i >> 1) & 1, p.wait_polls));
+      if (!ok) break;
+      fence_after();
+      const int rows = min(walk.end - row0, PAIR_T);
+#pragma unroll 1
+      for (int c = 0; c < rows; c += 16) {
+        int r[16];
+        tmem_load(r, mine + (i & 1) * PAIR_T + c);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const long long row = row0 + c + q;
+          if (real && c + q < rows) {
+            const float alpha = __fmul_rn(__ldg(p.scale_a + row * p.sa_stride), sb);
+            out[row * p.ldd] = out_bits<OUT>(__fmaf_rn(__int2float_rn(r[q]), alpha, bias));
+          }
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_remote(leader_addr(&sm.acc_empty[i & 1]));
+    }
+  }
+  if (!ok) atomicExch(p.status, 1);
+  fence_before();
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
 // Rows behind the last group: zero.
 __global__ void __launch_bounds__(256) zero_rest_kernel(const __grid_constant__ Int8Params p) {
   __shared__ int first;
@@ -405,6 +585,17 @@ cudaError_t launch_tile(const Int8Params& p, const Maps& m, int parts, unsigned 
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, m.w, m.a, p);
 }
+template <int OUT>
+cudaError_t launch_pair(const Int8Params& p, const Maps& m, long long tiles, cudaStream_t st) {
+  auto kern = int8_pair_kernel<OUT>;
+  constexpr size_t SMEM = sizeof(SmemPair) + 1024;
+  static_assert(SMEM <= 232448, "shared memory of a CTA");
+  const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+  if (err != cudaSuccess) return err;
+  const long long pairs = sms() / 2;
+  kern<<<(unsigned)(2 * (tiles < pairs ? tiles : pairs)), TILE_THREADS, SMEM, st>>>(m.w, m.a, p);
+  return cudaGetLastError();
+}
 template <int BT>
 cudaError_t launch_out(const Int8Params& p, const Maps& m, int parts, unsigned tiles_t, cudaStream_t st) {
   switch (p.out_dtype) {
@@ -468,6 +659,7 @@ cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st
   p.tiles_n = (p.N + CH - 1) / CH;
   // rows of a tile: a power of two that holds the rows of a group, at most 256
   const long long per_group = ((long long)p.T + p.E - 1) / p.E;
+  const bool pair = per_group >= 192 && p.K > 0;
   const int bt = per_group <= 16 ? 16 : per_group <= 32 ? 32 : per_group <= 64 ? 64 : per_group <= 128 ? 128 : 256;
   const long long tiles_t = p.offs ? (long long)p.T / bt + (p.E < p.T ? p.E : p.T) : ((long long)p.T + bt - 1) / bt;
   if (tiles_t > 65535) return cudaErrorInvalidValue;
@@ -477,8 +669,16 @@ cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st
     // (a single row's stride is never used, but the map wants a multiple of 16)
     const long long ldw = p.N > 1 ? p.ldw : pitch_of(p.K), lda = p.T > 1 ? p.lda : pitch_of(p.K);
     err = byte_map(&m.w, p.w, p.K, p.N, ldw, p.E, p.E > 1 ? p.gsw : pitch_of(p.K), CH, true);
-    if (err == cudaSuccess) err = byte_map(&m.a, p.a, p.K, p.T, lda, 1, 0, bt, false);
+    if (err == cudaSuccess) err = byte_map(&m.a, p.a, p.K, p.T, lda, 1, 0, pair ? CH : bt, false);
     if (err != cudaSuccess) return err;
+  }
+  if (pair) {
+    const long long tiles = tiles_t * ((p.N + 2 * CH - 1) / (2 * CH));      // at most
+    err = p.out_dtype == MMB200_OUT_F32 ? launch_pair<MMB200_OUT_F32>(p, m, tiles, st)
+          : p.out_dtype == MMB200_OUT_BF16 ? launch_pair<MMB200_OUT_BF16>(p, m, tiles, st) : launch_pair<MMB200_OUT_F16>(p, m, tiles, st);
+    if (err != cudaSuccess) return err;
+    *launches += 1;
+    return launch_zero_rest(p, st, launches);
   }
   int parts = 1;
   const long long ctas = (long long)p.tiles_n * tiles_t;
