@@ -61,17 +61,19 @@ __device__ __forceinline__ int remote_int(uint32_t addr, int rank) {
   return v;
 }
 template <int N>
-__device__ __forceinline__ void tmem_load(int (&r)[N], uint32_t addr);
-template <>
-__device__ __forceinline__ void tmem_load<16>(int (&r)[16], uint32_t addr) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-               "[%16];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-               : "r"(addr) : "memory");
+__device__ __forceinline__ void tmem_load(int (&r)[N], uint32_t addr) {
+  static_assert(N == 16 || N == 32, "columns of a load");
+#pragma unroll
+  for (int h = 0; h < N; h += 16)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+                 "[%16];"
+                 : "=r"(r[h]), "=r"(r[h + 1]), "=r"(r[h + 2]), "=r"(r[h + 3]), "=r"(r[h + 4]), "=r"(r[h + 5]), "=r"(r[h + 6]),
+                   "=r"(r[h + 7]), "=r"(r[h + 8]), "=r"(r[h + 9]), "=r"(r[h + 10]), "=r"(r[h + 11]), "=r"(r[h + 12]),
+                   "=r"(r[h + 13]), "=r"(r[h + 14]), "=r"(r[h + 15])
+                 : "r"(addr + h) : "memory");
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int q = 0; q < 16; ++q) asm volatile("" : "+r"(r[q])::"memory");
+  for (int q = 0; q < N; ++q) asm volatile("" : "+r"(r[q])::"memory");
 }
 
 // ---- the output of one thread: channel n of group g
@@ -86,13 +88,48 @@ __device__ __forceinline__ float bias_at(const Int8Params& p, long long i) {
   if (p.bias_dtype == MMB200_HP_F16) return __half2float(__ldg(static_cast<const __half*>(p.bias) + i));
   return __uint_as_float((uint32_t)__ldg(static_cast<const uint16_t*>(p.bias) + i) << 16);
 }
+// (FMA and the conversions return the framework's NaN: 0x7FFFFFFF, 0x7FFF)
 template <int OUT>
 __device__ __forceinline__ typename OutType<OUT>::type out_bits(float y) {
-  if constexpr (OUT == MMB200_OUT_BF16) return f32_to_bf16_bits(y);
-  else if constexpr (OUT == MMB200_OUT_F16) return f32_to_f16_bits(y);
-  else {
-    const uint32_t u = __float_as_uint(y);
-    return (u & 0x7FFFFFFFu) > 0x7F800000u ? CANON_NAN32 : u;
+  if constexpr (OUT == MMB200_OUT_F32) return __float_as_uint(y);
+  uint16_t h;
+  if constexpr (OUT == MMB200_OUT_BF16) asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(h) : "f"(y));
+  else asm("cvt.rn.f16.f32 %0, %1;" : "=h"(h) : "f"(y));
+  return h;
+}
+// Scale of row `lane` of a chunk of CHUNK rows, `left` of which exist.
+template <int CHUNK>
+__device__ __forceinline__ float row_scales(const Int8Params& p, long long row, int left) {
+  const int lane = threadIdx.x % 32;
+  return lane < CHUNK && lane < left ? __ldg(p.scale_a + (row + lane) * p.sa_stride) : 0.0f;
+}
+// The output of a warp: its 32 channels (one per lane; `real`: inside N) of the rows [row0, row0 + rows), whose sums are the
+// columns of the accumulator at `acc`, or zero without products. The scale of a row is held by one lane and handed round;
+// `scale` comes in for the first chunk, so that its load runs before the accumulator is complete.
+template <int OUT, int BT>
+__device__ __forceinline__ void write_rows(const Int8Params& p, uint32_t acc, bool products, long long row0, int rows, int n, bool real, float sb,
+                                           float bias, float scale) {
+  constexpr int CHUNK = BT < 32 ? BT : 32;
+  typename OutType<OUT>::type* out = static_cast<typename OutType<OUT>::type*>(p.d) + row0 * p.ldd + n;
+#pragma unroll 1
+  for (int c = 0; c < rows; c += CHUNK) {
+    int r[CHUNK];
+    if (products) {
+      tmem_load<CHUNK>(r, acc + c);
+    } else {
+#pragma unroll
+      for (int q = 0; q < CHUNK; ++q) r[q] = 0;
+    }
+    const float s = scale;
+    scale = row_scales<CHUNK>(p, row0 + c + CHUNK, rows - c - CHUNK);
+    const int left = rows - c;
+#pragma unroll
+    for (int q = 0; q < CHUNK; ++q) {
+      const float alpha = __fmul_rn(__shfl_sync(0xFFFFFFFFu, s, q), sb);
+      const auto y = out_bits<OUT>(__fmaf_rn(__int2float_rn(r[q]), alpha, bias));
+      if (real && q < left) *out = y;
+      out += p.ldd;
+    }
   }
 }
 
@@ -247,46 +284,22 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
     cluster_arrive();
     cluster_wait();
   }
-  if (work && warp >= 2 && !bad && n < p.N) {
-    using O = typename OutType<OUT>::type;
-    const float sb = __ldg(p.scale_b + (long long)g.g * p.sb_group + (long long)n * p.sb_stride);
-    const float bias = bias_at(p, (long long)g.g * p.bias_group + n);
-    O* out = static_cast<O*>(p.d) + n;
-    auto write = [&](int row, int acc) {
-      const float alpha = __fmul_rn(__ldg(p.scale_a + (long long)row * p.sa_stride), sb);
-      out[(long long)row * p.ldd] = out_bits<OUT>(__fmaf_rn(__int2float_rn(acc), alpha, bias));
-    };
-    if (parts > 1) {
-      const int c0 = BT * rank / parts, c1 = BT * (rank + 1) / parts;
-      for (int c = c0; c < c1 && row0 + c < g.end; ++c) {
-        int acc = 0;
-        for (int q = 0; q < parts; ++q) acc += remote_int(smem_addr(part + c * CH + lane_ch), q);
-        write(row0 + c, acc);
-      }
-    }
-  }
-  if (work && warp >= 2 && !bad && parts == 1) {    // TMEM loads take whole warps
-    using O = typename OutType<OUT>::type;
+  if (work && warp >= 2 && !bad) {
     const bool real = n < p.N;
     const float sb = real ? __ldg(p.scale_b + (long long)g.g * p.sb_group + (long long)n * p.sb_stride) : 0.0f;
     const float bias = real ? bias_at(p, (long long)g.g * p.bias_group + n) : 0.0f;
-    O* out = static_cast<O*>(p.d) + n;
-#pragma unroll 1
-    for (int c = 0; c < BT && row0 + c < g.end; c += 16) {
-      int r[16];
-      if (nk > 0) {
-        tmem_load(r, mine + c);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 16; ++q) r[q] = 0;
-      }
-#pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const int row = row0 + c + q;
-        if (real && row < g.end) {
-          const float alpha = __fmul_rn(__ldg(p.scale_a + (long long)row * p.sa_stride), sb);
-          out[(long long)row * p.ldd] = out_bits<OUT>(__fmaf_rn(__int2float_rn(r[q]), alpha, bias));
-        }
+    const int rows = min(g.end - row0, BT);
+    if (parts == 1) {
+      write_rows<OUT, BT>(p, mine, nk > 0, row0, rows, n, real, sb, bias, row_scales<(BT < 32 ? BT : 32)>(p, row0, rows));
+    } else {
+      using O = typename OutType<OUT>::type;
+      const int c1 = min(BT * (rank + 1) / parts, rows);
+      for (int c = BT * rank / parts; c < c1; ++c) {
+        int acc = 0;
+        for (int q = 0; q < parts; ++q) acc += remote_int(smem_addr(part + c * CH + lane_ch), q);
+        const long long row = row0 + c;
+        const float alpha = __fmul_rn(__ldg(p.scale_a + row * p.sa_stride), sb);
+        if (real) static_cast<O*>(p.d)[row * p.ldd + n] = out_bits<OUT>(__fmaf_rn(__int2float_rn(acc), alpha, bias));
       }
     }
   }
@@ -436,32 +449,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1)
     }
     __syncwarp();
   } else {
-    using O = typename OutType<OUT>::type;
     const uint32_t mine = tmem + ((uint32_t)(32 * (warp % 4)) << 16);
     unsigned i = 0;
     for (long long t = first; walk.find(p, tiles_n, t, row0, n_tile); t += step, ++i) {
-      const int n = (2 * n_tile + rank) * CH + 32 * (warp % 4) + lane;
+      const int n = (2 * n_tile + rank) * CH + 32 * (warp % 4) + lane, rows = min(walk.end - row0, PAIR_T);
       const bool real = n < p.N;
       const float sb = real ? __ldg(p.scale_b + (long long)walk.g * p.sb_group + (long long)n * p.sb_stride) : 0.0f;
       const float bias = real ? bias_at(p, (long long)walk.g * p.bias_group + n) : 0.0f;
-      O* out = static_cast<O*>(p.d) + n;
+      const float scale = row_scales<32>(p, row0, rows);
       ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.acc_full[i & 1], (i >> 1) & 1, p.wait_polls));
       if (!ok) break;
       fence_after();
-      const int rows = min(walk.end - row0, PAIR_T);
-#pragma unroll 1
-      for (int c = 0; c < rows; c += 16) {
-        int r[16];
-        tmem_load(r, mine + (i & 1) * PAIR_T + c);
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const long long row = row0 + c + q;
-          if (real && c + q < rows) {
-            const float alpha = __fmul_rn(__ldg(p.scale_a + row * p.sa_stride), sb);
-            out[row * p.ldd] = out_bits<OUT>(__fmaf_rn(__int2float_rn(r[q]), alpha, bias));
-          }
-        }
-      }
+      write_rows<OUT, PAIR_T>(p, mine + (i & 1) * PAIR_T, true, row0, rows, n, real, sb, bias, scale);
       fence_before();
       __syncwarp();
       if (lane == 0) arrive_remote(leader_addr(&sm.acc_empty[i & 1]));
