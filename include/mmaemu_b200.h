@@ -274,7 +274,8 @@ int mmb200_int8_scaled_mm(const int8_t *A_dev, int64_t lda, const int8_t *W_dev,
                           int sb_stride, const void *bias_dev, int bias_dtype, int64_t bias_group_stride, int zero_rest,
                           void *workspace_dev, size_t workspace_bytes, void *stream);
 /* Synchronises `stream`, reads and clears the current device's status word of the int8 kernels: MMB200_ERR_TIMEOUT when a
- * bounded wait has run out since the word was last read (outputs of that call are unspecified), else MMB200_OK. */
+ * bounded wait has run out since the word was last read (outputs of that call are unspecified), else MMB200_OK. With
+ * MMAEMU_B200_CHECK_STATUS=1 in the environment mmb200_int8_scaled_mm ends with this call. */
 int mmb200_int8_status(void *stream);
 
 /* Issue-rate probe for roofline denominators: launches `ctas` blocks of 256 threads in which every thread executes

@@ -176,7 +176,11 @@ __device__ __forceinline__ Group find_group(const Int8Params& p, int slot) {
 }
 
 template <int BT>
-constexpr int tile_stages() { return BT <= 16 ? 6 : (BT <= 32 ? 5 : 4); }
+constexpr int tile_stages() { return
+#ifdef ST16
+ BT <= 16 ? ST16 :
+#endif
+ BT <= 16 ? 6 : (BT <= 32 ? 5 : 4); }
 template <int BT>
 struct SmemTile {
   static constexpr int STAGES = tile_stages<BT>();
@@ -317,13 +321,14 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
 
 // ---- pairs of CTAs
 constexpr int PAIR_STAGES = 6, PAIR_T = 256;
+constexpr int PAIR_THREADS = 320;        // warp 0: copies, warp 1: MMAs, warps 2 to 9: output (a quarter of the channels, half of the rows)
 constexpr int PAIR_BAND = 8;               // tiles of rows that share a pass over the channels (16 MB of rows at K = 8192 stay in L2)
 struct SmemPair {
   struct Stage { unsigned char w[CH * KB], a[CH * KB]; } stage[PAIR_STAGES];
   unsigned long long full[PAIR_STAGES];    // leader: both CTAs' copies of the stage have landed
   unsigned long long empty[PAIR_STAGES];   // the MMAs that read the stage are done
   unsigned long long acc_full[2];          // the accumulator is complete
-  unsigned long long acc_empty[2];         // leader: all eight output warps have read it
+  unsigned long long acc_empty[2];         // leader: all sixteen output warps have read it
   unsigned long long drain;
   uint32_t tmem;
 };
@@ -376,7 +381,7 @@ struct Walker {
 };
 
 template <int OUT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
                      const __grid_constant__ Int8Params p) {
   extern __shared__ unsigned char smem_raw[];
@@ -388,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1)
   const long long first = blockIdx.x / 2, step = gridDim.x / 2;
   if (threadIdx.x == 0) {
     for (int q = 0; q < PAIR_STAGES; ++q) { mbar_init(&sm.full[q], 1); mbar_init(&sm.empty[q], 1); }
-    for (int q = 0; q < 2; ++q) { mbar_init(&sm.acc_full[q], 1); mbar_init(&sm.acc_empty[q], 8); }
+    for (int q = 0; q < 2; ++q) { mbar_init(&sm.acc_full[q], 1); mbar_init(&sm.acc_empty[q], 16); }
     mbar_init(&sm.drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -449,18 +454,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1)
     }
     __syncwarp();
   } else {
-    const uint32_t mine = tmem + ((uint32_t)(32 * (warp % 4)) << 16);
+    const int half = warp < 6 ? 0 : PAIR_T / 2;
+    const uint32_t mine = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + half;
     unsigned i = 0;
     for (long long t = first; walk.find(p, tiles_n, t, row0, n_tile); t += step, ++i) {
-      const int n = (2 * n_tile + rank) * CH + 32 * (warp % 4) + lane, rows = min(walk.end - row0, PAIR_T);
+      const int n = (2 * n_tile + rank) * CH + 32 * (warp % 4) + lane, rows = min(walk.end - row0 - half, PAIR_T / 2);
       const bool real = n < p.N;
       const float sb = real ? __ldg(p.scale_b + (long long)walk.g * p.sb_group + (long long)n * p.sb_stride) : 0.0f;
       const float bias = real ? bias_at(p, (long long)walk.g * p.bias_group + n) : 0.0f;
-      const float scale = row_scales<32>(p, row0, rows);
+      const float scale = row_scales<32>(p, row0 + half, rows);
       ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.acc_full[i & 1], (i >> 1) & 1, p.wait_polls));
       if (!ok) break;
       fence_after();
-      write_rows<OUT, PAIR_T>(p, mine + (i & 1) * PAIR_T, true, row0, rows, n, real, sb, bias, scale);
+      write_rows<OUT, PAIR_T>(p, mine + (i & 1) * PAIR_T, true, row0 + half, rows, n, real, sb, bias, scale);
       fence_before();
       __syncwarp();
       if (lane == 0) arrive_remote(leader_addr(&sm.acc_empty[i & 1]));
@@ -562,6 +568,21 @@ int sms() {
   return n;
 }
 
+// Shared memory of a kernel beyond the default, asked for once per device (1 us of every call otherwise).
+struct SmemLimit {
+  std::atomic<unsigned long long> done{0};
+  cudaError_t set(const void* kern, size_t bytes) {
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return err;
+  }
+};
+
 struct Maps { CUtensorMap w, a; };
 
 template <int BT, int OUT>
@@ -569,7 +590,8 @@ cudaError_t launch_tile(const Int8Params& p, const Maps& m, int parts, unsigned 
   auto kern = int8_tile_kernel<BT, OUT>;
   constexpr size_t SMEM = sizeof(SmemTile<BT>) + 1024;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
-  cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+  static SmemLimit limit;
+  const cudaError_t err = limit.set(reinterpret_cast<const void*>(kern), SMEM);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.tiles_n * parts), tiles_t);
@@ -589,10 +611,11 @@ cudaError_t launch_pair(const Int8Params& p, const Maps& m, long long tiles, cud
   auto kern = int8_pair_kernel<OUT>;
   constexpr size_t SMEM = sizeof(SmemPair) + 1024;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
-  const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+  static SmemLimit limit;
+  const cudaError_t err = limit.set(reinterpret_cast<const void*>(kern), SMEM);
   if (err != cudaSuccess) return err;
   const long long pairs = sms() / 2;
-  kern<<<(unsigned)(2 * (tiles < pairs ? tiles : pairs)), TILE_THREADS, SMEM, st>>>(m.w, m.a, p);
+  kern<<<(unsigned)(2 * (tiles < pairs ? tiles : pairs)), PAIR_THREADS, SMEM, st>>>(m.w, m.a, p);
   return cudaGetLastError();
 }
 template <int BT>
@@ -606,7 +629,16 @@ cudaError_t launch_out(const Int8Params& p, const Maps& m, int parts, unsigned t
 
 }  // namespace
 
-cudaError_t int8_status_word(int** word) { return cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_int8_status); }
+cudaError_t int8_status_word(int** word) {
+  static std::atomic<int*> cached[64];
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev >= 0 && dev < 64 && (*word = cached[dev].load(std::memory_order_acquire)) != nullptr) return cudaSuccess;
+  err = cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_int8_status);
+  if (err == cudaSuccess && dev >= 0 && dev < 64) cached[dev].store(*word, std::memory_order_release);
+  return err;
+}
 
 size_t int8_workspace_bytes(const Int8Params& p) {
   size_t n = 0;
@@ -658,8 +690,11 @@ cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st
   p.tiles_n = (p.N + CH - 1) / CH;
   // rows of a tile: a power of two that holds the rows of a group, at most 256
   const long long per_group = ((long long)p.T + p.E - 1) / p.E;
-  const bool pair = per_group >= 192 && p.K > 0;
-  const int bt = per_group <= 16 ? 16 : per_group <= 32 ? 32 : per_group <= 64 ? 64 : per_group <= 128 ? 128 : 256;
+  bool pair = per_group >= 192 && p.K > 0;
+ if (getenv("MMB_PAIR")) pair = atoi(getenv("MMB_PAIR"));
+  int bt = per_group <= 16 ? 16 : per_group <= 32 ? 32 : per_group <= 64 ? 64 : per_group <= 128 ? 128 : 256;
+ if (getenv("MMB_BT")) bt = atoi(getenv("MMB_BT"));
+ if (pair) bt=256;
   const long long tiles_t = p.offs ? (long long)p.T / bt + (p.E < p.T ? p.E : p.T) : ((long long)p.T + bt - 1) / bt;
   if (tiles_t > 65535) return cudaErrorInvalidValue;
   Maps m;
@@ -682,6 +717,7 @@ cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st
   int parts = 1;
   const long long ctas = (long long)p.tiles_n * tiles_t;
   while (parts < 8 && bt <= 64 && ctas * parts * 2 <= 2ll * sms() && p.k_blocks >= 4 * parts) parts *= 2;
+  if (getenv("MMB_PARTS")) parts = atoi(getenv("MMB_PARTS"));
   switch (bt) {
     case 16: err = launch_out<16>(p, m, parts, (unsigned)tiles_t, st); break;
     case 32: err = launch_out<32>(p, m, parts, (unsigned)tiles_t, st); break;

@@ -1,9 +1,9 @@
 // Symmetric int8 quantisation with one scale per row: the operands of the int8 products (kernel_int8.cu).
 //
 // Per row: amax = max |x|, scale = RN32(amax / 127), code = the integer nearest to the real number 127 x / amax, ties to
-// even. The codes are decided exactly, so they do not depend on how a division or a reciprocal rounds: t = RN(x * RN(127 /
-// amax)) is off by less than 127 * 2^-22.9 = 1.7e-5, so its nearest integer is the answer unless t lies within 2e-5 of a
-// half; there 254 |x| and (2 q + 1) amax are compared, both exact in fp64 (31 bits). A zero row has scale 0 and codes 0; a
+// even. The codes are decided exactly, so they do not depend on how a division or a reciprocal rounds: x * RN(127 / amax) is
+// off by less than 127 * 2^-24 = 7.6e-6, so its nearest integer is the answer unless it lies within 2e-5 of a half; there
+// 254 |x| and (2 q + 1) amax are compared, both exact in fp64 (31 bits). A zero row has scale 0 and codes 0; a
 // row with a NaN or an infinity has scale NaN and codes 0, so every product with it is NaN.
 //
 // What bounds it: one read of x and one write of the codes. A row is read once into registers (16-byte loads) by as many
@@ -17,85 +17,95 @@ namespace mmb {
 namespace {
 
 constexpr float SMALL = 7.8886090522101181e-31f;      // 2^-100: below it 127 / amax may overflow
+constexpr float RAISE = 1.2676506002282294e+30f;      // 2^100
 
+// A 16-byte vector of a type: how many values, their largest magnitude, their values in fp32. The magnitudes are kept as
+// bit patterns, which order like the numbers, NaN above infinity; 16-bit ones in pairs.
 template <int T>
-struct Elem;
-template <>
-struct Elem<MMB200_HP_F32> {
-  static constexpr int SIZE = 4, PER16 = 4;
-  static __device__ __forceinline__ float get(const void* p, long long i) { return __ldg(static_cast<const float*>(p) + i); }
-  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
-    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+struct Elem {
+  static constexpr int SIZE = T == MMB200_HP_F32 ? 4 : 2, PER16 = 16 / SIZE;
+  static __device__ __forceinline__ uint32_t top_of(uint32_t top, const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) top = SIZE == 4 ? max(top, w[q] & 0x7FFFFFFFu) : __vmaxu2(top, w[q] & 0x7FFF7FFFu);
+    return top;
   }
-};
-template <>
-struct Elem<MMB200_HP_BF16> {
-  static constexpr int SIZE = 2, PER16 = 8;
-  static __device__ __forceinline__ float get(const void* p, long long i) {
-    return __uint_as_float((uint32_t)__ldg(static_cast<const uint16_t*>(p) + i) << 16);
+  static __device__ __forceinline__ float amax_of(uint32_t top) {     // of a maximum over all threads
+    if (SIZE == 4) return __uint_as_float(top);
+    const uint16_t h = (uint16_t)max(top & 0xFFFFu, top >> 16);
+    return T == MMB200_HP_BF16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
   }
-  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[PER16]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      f[2 * q] = __uint_as_float(w[q] << 16);
-      f[2 * q + 1] = __uint_as_float(w[q] & 0xFFFF0000u);
-    }
-  }
-};
-template <>
-struct Elem<MMB200_HP_F16> {
-  static constexpr int SIZE = 2, PER16 = 8;
-  static __device__ __forceinline__ float get(const void* p, long long i) { return __half2float(__ldg(static_cast<const __half*>(p) + i)); }
-  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
-      f[2 * q] = g.x;
-      f[2 * q + 1] = g.y;
+      if constexpr (SIZE == 4) {
+        f[q] = __uint_as_float(w[q]);
+      } else if constexpr (T == MMB200_HP_BF16) {
+        f[2 * q] = __uint_as_float(w[q] << 16);
+        f[2 * q + 1] = __uint_as_float(w[q] & 0xFFFF0000u);
+      } else {
+        const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
+        f[2 * q] = g.x;
+        f[2 * q + 1] = g.y;
+      }
     }
   }
 };
 
-// What a row's codes are computed with.
+// What a row's codes are computed with. Rows of tiny values are raised by 2^100 first (exact).
 struct RowScale {
   float amax, inv;
-  bool zero, exact;      // no codes but 0; decide every code in fp64
+  bool zero, tiny;
 };
 __device__ __forceinline__ RowScale row_scale(float amax) {
   RowScale r;
-  r.amax = amax;
   r.zero = !(amax > 0.0f) || !(amax < __int_as_float(0x7F800000));
-  r.exact = amax < SMALL;
-  r.inv = r.zero || r.exact ? 0.0f : __fdiv_rn(127.0f, amax);
+  r.tiny = amax < SMALL;
+  r.amax = r.tiny ? __fmul_rn(amax, RAISE) : amax;
+  r.inv = r.zero ? 0.0f : __fdiv_rn(127.0f, r.amax);
   return r;
 }
 __device__ __forceinline__ float scale_of(float amax) {
   return amax < __int_as_float(0x7F800000) ? __fdiv_rn(amax, 127.0f) : __uint_as_float(CANON_NAN32);
 }
-// Nearest integer of 127 x / amax by exact comparison: 254 |x| against (2 q + 1) amax for q = the floor.
-__device__ __noinline__ int code_exact(float x, float amax) {
-  const double twice = 254.0 * (double)fabsf(x), a = (double)amax;
-  double q = floor(twice / (2.0 * a));                 // at most one off; put right below
-  if (2.0 * q * a > twice) q -= 1.0;
-  else if (2.0 * (q + 1.0) * a <= twice) q += 1.0;
-  const double mid = (2.0 * q + 1.0) * a;
-  int c = (int)q;
-  if (twice > mid || (twice == mid && (c & 1))) ++c;
-  return x < 0.0f ? -c : c;
+// Nearest integer of 127 x / amax where it is near a half: 254 |x| against (2 q + 1) amax, q the floor.
+__device__ __forceinline__ uint32_t code_at_border(float x, const RowScale& r) {
+  const int q = (int)floorf(__fmul_rn(fabsf(x), r.inv));
+  const double twice = 254.0 * (double)fabsf(x), mid = (double)(2 * q + 1) * (double)r.amax;
+  const int c = q + (twice > mid || (twice == mid && (q & 1)) ? 1 : 0);
+  return (uint32_t)(x < 0.0f ? -c : c);
 }
-__device__ __forceinline__ int code_of(float x, const RowScale& r) {
-  const float t = __fmul_rn(x, r.inv), q = rintf(t);
-  int c = (int)q;
-  if (r.exact || fabsf(t - q) > 0.49998f) c = code_exact(x, r.amax);
-  return c;
+// The codes of N values, packed. In [2^23, 2^24) one ulp is 1, so RN(x inv + 1.5 * 2^23) holds the nearest integer in its
+// low bits (ties to even, two's complement): four instructions per value, none on the quarter-rate conversion pipe. `off`
+// collects the largest distance from the integer, so that borders cost one test per vector.
+template <int N>
+__device__ __forceinline__ void codes_of(float (&x)[N], const RowScale& r, uint32_t (&w)[N / 4]) {
+  constexpr float MAGIC = 12582912.0f, NEAR = 0.49998f;
+  uint32_t b[N];
+  float off = 0.0f;
+  if (r.tiny) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) x[q] = __fmul_rn(x[q], RAISE);
+  }
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    const float m = __fmaf_rn(x[q], r.inv, MAGIC);
+    off = fmaxf(off, fabsf(__fmaf_rn(x[q], r.inv, -__fsub_rn(m, MAGIC))));
+    b[q] = __float_as_uint(m);
+  }
+  if (off > NEAR) {
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      if (fabsf(__fmaf_rn(x[q], r.inv, -__fsub_rn(__uint_as_float(b[q]), MAGIC))) > NEAR) b[q] = code_at_border(x[q], r);
+  }
+#pragma unroll
+  for (int q = 0; q < N / 4; ++q)
+    w[q] = r.zero ? 0u : __byte_perm(__byte_perm(b[4 * q], b[4 * q + 1], 0x0040), __byte_perm(b[4 * q + 2], b[4 * q + 3], 0x0040), 0x5410);
 }
-// max(a, |b|) with NaN kept as +infinity's successor: non-negative floats order like their bit patterns, NaN above infinity.
-__device__ __forceinline__ uint32_t abs_max(uint32_t a, float b) { return max(a, __float_as_uint(b) & 0x7FFFFFFFu); }
 
-// THREADS threads per row (a warp, or the whole block), up to VPT 16-byte vectors each. The last vector of a row may be
-// partial. Rows longer than THREADS * VPT vectors are read twice.
+// The row's threads (a warp, or the whole block) hold VPT 16-byte vectors each. The last vector of a row may be partial.
+// Rows longer than that are read twice.
 template <int T, int BLOCK, bool WARP_ROW, int VPT>
 __global__ void __launch_bounds__(BLOCK) quantise_kernel(const __grid_constant__ QuantiseParams p) {
   using E = Elem<T>;
@@ -107,24 +117,22 @@ __global__ void __launch_bounds__(BLOCK) quantise_kernel(const __grid_constant__
   int8_t* out = p.codes + row * p.ldc;
   const int vecs = (p.K + PER - 1) / PER;
   const bool vec_in = p.vec_in, vec_out = p.vec_out;
-  auto load = [&](int v, float* f) {
-    if (vec_in && (v + 1) * PER <= p.K) {
-      E::unpack(__ldg(reinterpret_cast<const uint4*>(x) + v), f);
-    } else {
+  auto load = [&](int v) -> uint4 {
+    if (vec_in && (v + 1) * PER <= p.K) return __ldg(reinterpret_cast<const uint4*>(x) + v);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int q = 0; q < PER; ++q) f[q] = v * PER + q < p.K ? E::get(x, v * PER + q) : 0.0f;
+    for (int q = 0; q < PER; ++q) {
+      if (v * PER + q >= p.K) break;
+      if constexpr (E::SIZE == 4) w[q] = __ldg(reinterpret_cast<const uint32_t*>(x) + v * PER + q);
+      else w[q / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(x) + v * PER + q) << (16 * (q % 2));
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   };
-  auto store = [&](int v, const float* f, const RowScale& r) {
+  auto store = [&](int v, const uint4& raw, const RowScale& r) {
+    float f[PER];
     uint32_t w[PER / 4];
-#pragma unroll
-    for (int q = 0; q < PER / 4; ++q) {
-      w[q] = 0;
-      if (!r.zero) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) w[q] |= (uint32_t)(code_of(f[4 * q + b], r) & 0xFF) << (8 * b);
-      }
-    }
+    E::unpack(raw, f);
+    codes_of<PER>(f, r, w);
     if (vec_out && (v + 1) * PER <= p.K) {
       if (PER == 8) *reinterpret_cast<uint2*>(out + v * PER) = make_uint2(w[0], w[PER / 4 - 1]);
       else *reinterpret_cast<uint32_t*>(out + v * PER) = w[0];
@@ -134,26 +142,14 @@ __global__ void __launch_bounds__(BLOCK) quantise_kernel(const __grid_constant__
         if (v * PER + q < p.K) out[v * PER + q] = (int8_t)(w[q / 4] >> (8 * (q % 4)));
     }
   };
-  float f[VPT][PER];
+  uint4 raw[VPT];
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int v = i * GROUP + tid;
-    if (v < vecs) load(v, f[i]);
-    else
+  for (int i = 0; i < VPT; ++i) raw[i] = i * GROUP + tid < vecs ? load(i * GROUP + tid) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-      for (int q = 0; q < PER; ++q) f[i][q] = 0.0f;
-  }
-#pragma unroll
-  for (int i = 0; i < VPT; ++i)
-#pragma unroll
-    for (int q = 0; q < PER; ++q) top = abs_max(top, f[i][q]);
-  for (int v = VPT * GROUP + tid; v < vecs; v += GROUP) {
-    float g[PER];
-    load(v, g);
-#pragma unroll
-    for (int q = 0; q < PER; ++q) top = abs_max(top, g[q]);
-  }
+  for (int i = 0; i < VPT; ++i) top = E::top_of(top, raw[i]);
+  for (int v = VPT * GROUP + tid; v < vecs; v += GROUP) top = E::top_of(top, load(v));
+  if (E::SIZE == 2) top = max(top & 0xFFFFu, top >> 16);
   top = __reduce_max_sync(0xFFFFFFFFu, top);
   if constexpr (!WARP_ROW) {
     __shared__ uint32_t part[BLOCK / 32];
@@ -162,19 +158,13 @@ __global__ void __launch_bounds__(BLOCK) quantise_kernel(const __grid_constant__
     top = part[threadIdx.x % (BLOCK / 32)];
     top = __reduce_max_sync(0xFFFFFFFFu, top);
   }
-  const float amax = __uint_as_float(top);
+  const float amax = E::amax_of(top);
   const RowScale r = row_scale(amax);
   if (tid == 0) p.scale[row] = scale_of(amax);
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int v = i * GROUP + tid;
-    if (v < vecs) store(v, f[i], r);
-  }
-  for (int v = VPT * GROUP + tid; v < vecs; v += GROUP) {
-    float g[PER];
-    load(v, g);
-    store(v, g, r);
-  }
+  for (int i = 0; i < VPT; ++i)
+    if (i * GROUP + tid < vecs) store(i * GROUP + tid, raw[i], r);
+  for (int v = VPT * GROUP + tid; v < vecs; v += GROUP) store(v, load(v), r);
 }
 
 template <int T>

@@ -16,9 +16,6 @@ current stream of the operands' device, do not synchronise and can be captured i
 """
 from __future__ import annotations
 
-import ctypes
-import os
-
 import torch
 
 from . import _lib
@@ -43,18 +40,12 @@ def _device(t: torch.Tensor) -> torch.device:
     return dev
 
 
-def _tensor(who: str, name: str, t) -> None:
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{who}(): argument '{name}' must be Tensor, not {type(t).__name__}")
+def _not_a_tensor(who: str, name: str, t) -> TypeError:
+    return TypeError(f"{who}(): argument '{name}' must be Tensor, not {type(t).__name__}")
 
 
-def _no_grad(who: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise UnsupportedFeatureError(f"{who}(): inference only: an input requires grad while grad mode is enabled")
-
-
-def _stream(dev: torch.device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(dev.index))
+def _no_grad(who: str) -> UnsupportedFeatureError:
+    return UnsupportedFeatureError(f"{who}(): inference only: an input requires grad while grad mode is enabled")
 
 
 def quantize_int8(x):
@@ -64,55 +55,82 @@ def quantize_int8(x):
     exactly (int8, the shape of x, contiguous; between -127 and 127). A row of zeros has scale 0; a row with a NaN or an
     infinity has scale NaN and codes 0, which makes every product with it NaN. Rows quantised this way are the operands of
     int8_scaled_mm: activations [M, K] give scale_a [M, 1], weights [N, K] give scale_b.t() [1, N]."""
-    _tensor("quantize_int8", "x", x)
+    if not isinstance(x, torch.Tensor):
+        raise _not_a_tensor("quantize_int8", "x", x)
     code = _REAL_CODES.get(x.dtype)
     if code is None:
         raise TypeError(f"quantize_int8(): x must be float32, bfloat16 or float16, got {x.dtype}")
-    if x.dim() == 0:
+    shape = x.shape
+    if not shape:
         raise ValueError("quantize_int8(): x must have at least one dimension")
-    _no_grad("quantize_int8", x)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise _no_grad("quantize_int8")
     dev = _device(x)
-    K = x.shape[-1]
-    if x.dim() != 2 or (x.stride(1) != 1 and K > 1) or (x.stride(0) < K and x.shape[0] > 1):
-        rows = x.detach().reshape(-1, K) if K else x.detach().reshape(x.shape[:-1].numel(), 0)
-        if (rows.stride(1) != 1 and K > 1) or (rows.stride(0) < K and rows.shape[0] > 1):
-            rows = rows.contiguous()
-    else:
-        rows = x
-    codes = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty(x.shape[:-1] + (1,), dtype=torch.float32, device=dev)
-    n = rows.shape[0]
+    K = shape[-1]
+    rows, n = x, shape[0]
+    if len(shape) != 2:
+        n = shape[:-1].numel()
+        rows = x.detach().reshape(n, K)
+    ld = rows.stride(0) if n > 1 else K
+    if (ld < K or rows.stride(1) != 1) and K > 1:
+        rows = rows.detach().contiguous()
+        ld = K
+    codes = torch.empty(shape, dtype=torch.int8, device=dev)
+    scale = torch.empty((*shape[:-1], 1), dtype=torch.float32, device=dev)
     if n == 0:
         return codes, scale
-    L = _lib.load()
     with _on_device(dev):
-        rc = L.mmb200_quantize_int8(rows.data_ptr(), rows.stride(0) if n > 1 else K, code, codes.data_ptr(), K,
-                                    scale.data_ptr(), n, K, _stream(dev))
+        rc = _lib.load().mmb200_quantize_int8(rows.data_ptr(), ld, code, codes.data_ptr(), K, scale.data_ptr(), n, K,
+                                              torch._C._cuda_getCurrentRawStream(dev.index))
     if rc:
         _lib.check("mmb200_quantize_int8", rc)
     return codes, scale
 
 
-def _matrix(who: str, t: torch.Tensor, rows: int, K: int):
+def _check_operands(who, input, mat2, scale_a, scale_b, others) -> None:
+    """Types, one device, no gradients; `others`: (name, tensor or None) pairs."""
+    for name, t in (("input", input), ("mat2", mat2), ("scale_a", scale_a), ("scale_b", scale_b)):
+        if not isinstance(t, torch.Tensor):
+            raise _not_a_tensor(who, name, t)
+    if input.dtype != torch.int8 or mat2.dtype != torch.int8:
+        raise TypeError(f"{who}(): input and mat2 must be int8, got {input.dtype} and {mat2.dtype}")
+    dev = input.device
+    grad = scale_a.requires_grad or scale_b.requires_grad
+    for name, t in others:
+        if t is not None:
+            if not isinstance(t, torch.Tensor):
+                raise _not_a_tensor(who, name, t)
+            grad = grad or t.requires_grad
+            if t.device != dev:
+                raise ValueError(f"{who}(): expected all tensors on one device, found {dev} and {t.device}")
+    for t in (mat2, scale_a, scale_b):
+        if t.device != dev:
+            raise ValueError(f"{who}(): expected all tensors on one device, found {dev} and {t.device}")
+    if grad and torch.is_grad_enabled():
+        raise _no_grad(who)
+    if scale_a.dtype != torch.float32 or scale_b.dtype != torch.float32:
+        raise ValueError(f"{who}(): scale_a and scale_b must be float32, got {scale_a.dtype} and {scale_b.dtype}")
+
+
+def _rows_of(t: torch.Tensor, rows: int, K: int):
     """(tensor, row stride) of a [rows, K] int8 operand whose rows the kernels can read: unit stride along K, no overlap."""
-    t = t.detach()
-    if (K > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < K):
-        t = t.contiguous()
-    return t, (t.stride(0) if rows > 1 else K)
+    ld, unit = t.stride()
+    if (unit != 1 and K > 1) or (rows > 1 and ld < K):
+        return t.contiguous(), K
+    return t, (ld if rows > 1 else K)
 
 
 def _scale_a(who, scale_a, rows):
-    if scale_a.dtype != torch.float32:
-        raise ValueError(f"{who}(): scale_a must be float32, got {scale_a.dtype}")
+    """Stride of scale_a over the rows; 0: one element."""
     if scale_a.numel() == 1:
         return 0
-    if tuple(scale_a.shape) != (rows, 1):
+    if scale_a.dim() != 2 or scale_a.shape[0] != rows or scale_a.shape[1] != 1:
         raise ValueError(f"{who}(): scale_a must have one element or shape {(rows, 1)}, got {tuple(scale_a.shape)}")
     return scale_a.stride(0)
 
 
-def _output(who, out, out_dtype, rows, N):
-    """(dtype, its code) of the output; out checked."""
+def _output(who, out, out_dtype, rows, N, dev):
+    """(tensor, row stride, code of the dtype) of the output."""
     if out_dtype is not None and not isinstance(out_dtype, torch.dtype):
         raise TypeError(f"{who}(): argument 'out_dtype' must be torch.dtype, not {type(out_dtype).__name__}")
     if out is not None and out_dtype is not None and out_dtype != out.dtype:
@@ -121,61 +139,39 @@ def _output(who, out, out_dtype, rows, N):
     code = _OUT_CODES.get(dtype)
     if code is None:
         raise ValueError(f"{who}(): the output is float32, bfloat16 or float16, got {dtype}")
-    if out is not None and (tuple(out.shape) != (rows, N) or (N > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < N)):
+    if out is None:
+        return (torch.empty((rows, N), dtype=dtype, device=dev) if dev.type == "cuda" else None), N, code
+    if tuple(out.shape) != (rows, N) or (N > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < N):
         raise ValueError(f"{who}(): out must be a row-major tensor of shape {(rows, N)}, got shape {tuple(out.shape)} with strides "
                          f"{tuple(out.stride())}")
-    return dtype, code
+    return out, (out.stride(0) if rows > 1 else N), code
 
 
 def _bias(who, bias, shape):
-    """(tensor or None, pointer or None, code of the dtype)"""
-    if bias is None:
-        return None, None, 0
+    """(tensor, code of the dtype)"""
     code = _REAL_CODES.get(bias.dtype)
     if code is None:
         raise ValueError(f"{who}(): bias must be float32, bfloat16 or float16, got {bias.dtype}")
     if tuple(bias.shape) != shape:
         raise ValueError(f"{who}(): bias must have shape {shape}, got {tuple(bias.shape)}")
-    bias = bias.detach().contiguous()
-    return bias, bias.data_ptr(), code
+    return bias.detach().contiguous(), code
 
 
-def _check_operands(who, input, mat2, scale_a, scale_b, bias, out, others=()):
-    _tensor(who, "input", input)
-    _tensor(who, "mat2", mat2)
-    _tensor(who, "scale_a", scale_a)
-    _tensor(who, "scale_b", scale_b)
-    if bias is not None:
-        _tensor(who, "bias", bias)
-    if out is not None:
-        _tensor(who, "out", out)
-    if input.dtype != torch.int8 or mat2.dtype != torch.int8:
-        raise TypeError(f"{who}(): input and mat2 must be int8, got {input.dtype} and {mat2.dtype}")
-    dev = input.device
-    for t in (mat2, scale_a, scale_b, bias, out, *others):
-        if isinstance(t, torch.Tensor) and t.device != dev:
-            raise ValueError(f"{who}(): expected all tensors on one device, found {dev} and {t.device}")
-    _no_grad(who, scale_a, scale_b, bias, out)
-
-
-def _run(who, dev, a, lda, w, ldw, gsw, y, ldd, code, T, N, K, E, offs, scale_a, sa, scale_b, sb_group, sb, bias, bias_code,
-         bias_group, zero_rest):
+def _run(dev, ap, lda, wp, ldw, gsw, y, ldd, code, T, N, K, E, offs, scale_a, sa, scale_b, sb_group, sb, bias, bias_code, bias_group,
+         zero_rest):
     L = _lib.load()
-    ap, wp = a.data_ptr(), w.data_ptr()
     with _on_device(dev):
         ws, ws_ptr, n = None, None, 0
         if (ap | wp | lda | ldw | gsw) & 15 or (E > 1 and not gsw):     # rows that TMA cannot read in place: room for copies
-            n = int(L.mmb200_int8_workspace_bytes(ap, lda, wp, ldw, gsw, T, N, K, E))
+            n = L.mmb200_int8_workspace_bytes(ap, lda, wp, ldw, gsw, T, N, K, E)
             if n:
                 ws = torch.empty(n, dtype=torch.uint8, device=dev)
                 ws_ptr = ws.data_ptr()
-        stream = _stream(dev)
         rc = L.mmb200_int8_scaled_mm(ap, lda, wp, ldw, gsw, y.data_ptr(), ldd, code, T, N, K, E, offs, scale_a.data_ptr(), sa,
-                                     scale_b.data_ptr(), sb_group, sb, bias, bias_code, bias_group, zero_rest, ws_ptr, n, stream)
+                                     scale_b.data_ptr(), sb_group, sb, None if bias is None else bias.data_ptr(), bias_code, bias_group,
+                                     zero_rest, ws_ptr, n, torch._C._cuda_getCurrentRawStream(dev.index))
         if rc:
             _lib.check("mmb200_int8_scaled_mm", rc)
-        if os.environ.get("MMAEMU_B200_CHECK_STATUS") == "1":
-            _lib.check("mmb200_int8_status", L.mmb200_int8_status(stream))
     return y
 
 
@@ -188,34 +184,38 @@ def int8_scaled_mm(input, mat2, scale_a, scale_b, bias=None, out_dtype=None, *, 
     K <= 131071, M <= 2^23. Rows of any alignment and stride are served; those that do not start on 16 bytes are copied
     first."""
     who = "int8_scaled_mm"
-    _check_operands(who, input, mat2, scale_a, scale_b, bias, out)
-    if input.dim() != 2 or mat2.dim() != 2 or input.shape[1] != mat2.shape[0]:
-        raise ValueError(f"{who}(): expected input [M, K] and mat2 [K, N], got {tuple(input.shape)} and {tuple(mat2.shape)}")
-    (M, K), N = input.shape, mat2.shape[1]
+    _check_operands(who, input, mat2, scale_a, scale_b, (("bias", bias), ("out", out)))
+    sizes, sizes2 = input.shape, mat2.shape
+    if len(sizes) != 2 or len(sizes2) != 2 or sizes[1] != sizes2[0]:
+        raise ValueError(f"{who}(): expected input [M, K] and mat2 [K, N], got {tuple(sizes)} and {tuple(sizes2)}")
+    (M, K), N = sizes, sizes2[1]
     if K > MAX_K or M > MAX_ROWS:
         raise ValueError(f"{who}(): K is at most {MAX_K} (int32 sums) and M at most {MAX_ROWS}, got K = {K}, M = {M}")
-    if K > 1 and N > 0 and mat2.stride(0) != 1:
+    unit, ldw = mat2.stride()
+    if K > 1 and N > 0 and unit != 1:
         raise ValueError(f"{who}(): mat2 must be column-major (the transpose of a row-major [N, K] weight), got strides "
-                         f"{tuple(mat2.stride())}")
+                         f"{(unit, ldw)}")
     sa = _scale_a(who, scale_a, M)
-    if scale_b.dtype != torch.float32:
-        raise ValueError(f"{who}(): scale_b must be float32, got {scale_b.dtype}")
     if scale_b.numel() == 1:
         sb = 0
-    elif tuple(scale_b.shape) == (1, N):
+    elif scale_b.dim() == 2 and scale_b.shape[0] == 1 and scale_b.shape[1] == N:
         sb = scale_b.stride(1)
     else:
         raise ValueError(f"{who}(): scale_b must have one element or shape {(1, N)}, got {tuple(scale_b.shape)}")
-    bias, bias_ptr, bias_code = _bias(who, bias, (N,))
-    dtype, code = _output(who, out, out_dtype, M, N)
+    bias_code = 0
+    if bias is not None:
+        bias, bias_code = _bias(who, bias, (N,))
+    y, ldd, code = _output(who, out, out_dtype, M, N, input.device)
     dev = _device(input)
-    y = torch.empty((M, N), dtype=dtype, device=dev) if out is None else out
-    ldd = y.stride(0) if M > 1 else N
     if M == 0 or N == 0:
         return y
-    a, lda = _matrix(who, input, M, K)
-    w, ldw = _matrix(who, mat2.t(), N, K)
-    return _run(who, dev, a, lda, w, ldw, 0, y, ldd, code, M, N, K, 1, None, scale_a, sa, scale_b, 0, sb, bias_ptr, bias_code, 0, 0)
+    a, lda = _rows_of(input, M, K)
+    if N == 1:
+        ldw = K
+    elif ldw < K:                                        # overlapping rows
+        mat2, ldw = mat2.t().contiguous(), K
+    return _run(dev, a.data_ptr(), lda, mat2.data_ptr(), ldw, 0, y, ldd, code, M, N, K, 1, None, scale_a, sa, scale_b, 0, sb, bias,
+                bias_code, 0, 0)
 
 
 def int8_grouped_scaled_mm(input, mat2, offs, scale_a, scale_b, bias=None, out_dtype=None, *, out=None):
@@ -228,44 +228,45 @@ def int8_grouped_scaled_mm(input, mat2, offs, scale_a, scale_b, bias=None, out_d
     [T, 1]; scale_b: one element or [E, 1, N]; bias: [E, N]. Rows behind the last group (a padded batch) are zero in a new
     output and keep their contents in `out`. Everything else as int8_scaled_mm; E <= 4096."""
     who = "int8_grouped_scaled_mm"
-    _tensor(who, "offs", offs)
-    _check_operands(who, input, mat2, scale_a, scale_b, bias, out, (offs,))
-    if input.dim() != 2 or mat2.dim() != 3 or input.shape[1] != mat2.shape[1]:
-        raise ValueError(f"{who}(): expected input [T, K] and mat2 [E, K, N], got {tuple(input.shape)} and {tuple(mat2.shape)}")
-    (T, K), E, N = input.shape, mat2.shape[0], mat2.shape[2]
+    if not isinstance(offs, torch.Tensor):
+        raise _not_a_tensor(who, "offs", offs)
+    _check_operands(who, input, mat2, scale_a, scale_b, (("bias", bias), ("out", out), ("offs", offs)))
+    sizes, sizes2 = input.shape, mat2.shape
+    if len(sizes) != 2 or len(sizes2) != 3 or sizes[1] != sizes2[1]:
+        raise ValueError(f"{who}(): expected input [T, K] and mat2 [E, K, N], got {tuple(sizes)} and {tuple(sizes2)}")
+    (T, K), (E, _, N) = sizes, sizes2
     if K > MAX_K or T > MAX_ROWS or E > MAX_GROUPS:
         raise ValueError(f"{who}(): K is at most {MAX_K} (int32 sums), T at most {MAX_ROWS} and E at most {MAX_GROUPS}, got K = {K}, "
                          f"T = {T}, E = {E}")
-    if offs.dtype != torch.int32 or tuple(offs.shape) != (E,):
+    if offs.dtype != torch.int32 or offs.dim() != 1 or offs.shape[0] != E:
         raise ValueError(f"{who}(): offs must be int32 of shape {(E,)}, got {offs.dtype} of shape {tuple(offs.shape)}")
-    if K > 1 and N > 0 and E > 0 and mat2.stride(1) != 1:
+    gsw, unit, ldw = mat2.stride()
+    if K > 1 and N > 0 and E > 0 and unit != 1:
         raise ValueError(f"{who}(): every matrix of mat2 must be column-major (the transpose of row-major [E, N, K] weights), got "
-                         f"strides {tuple(mat2.stride())}")
+                         f"strides {(gsw, unit, ldw)}")
     sa = _scale_a(who, scale_a, T)
-    if scale_b.dtype != torch.float32:
-        raise ValueError(f"{who}(): scale_b must be float32, got {scale_b.dtype}")
     if scale_b.numel() == 1:
         sb_group = sb = 0
     elif tuple(scale_b.shape) == (E, 1, N):
-        sb_group, sb = scale_b.stride(0), scale_b.stride(2)
+        sb_group, _, sb = scale_b.stride()
     else:
         raise ValueError(f"{who}(): scale_b must have one element or shape {(E, 1, N)}, got {tuple(scale_b.shape)}")
-    bias, bias_ptr, bias_code = _bias(who, bias, (E, N))
-    dtype, code = _output(who, out, out_dtype, T, N)
+    bias_code = 0
+    if bias is not None:
+        bias, bias_code = _bias(who, bias, (E, N))
+    y, ldd, code = _output(who, out, out_dtype, T, N, input.device)
     dev = _device(input)
-    y = torch.empty((T, N), dtype=dtype, device=dev) if out is None else out
-    ldd = y.stride(0) if T > 1 else N
     if T == 0 or N == 0:
         return y
     if E == 0:
         return y.zero_() if out is None else y
-    a, lda = _matrix(who, input, T, K)
-    w = mat2.detach()
-    if N > 1 and w.stride(2) < K:
-        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    a, lda = _rows_of(input, T, K)
+    if N > 1 and ldw < K:                                # overlapping rows
+        mat2 = mat2.transpose(1, 2).contiguous()
+        gsw, ldw = N * K, K
     offs = offs.contiguous()
-    return _run(who, dev, a, lda, w, w.stride(2) if N > 1 else K, w.stride(0) if E > 1 else 0, y, ldd, code, T, N, K, E,
-                offs.data_ptr(), scale_a, sa, scale_b, sb_group, sb, bias_ptr, bias_code, N, int(out is None))
+    return _run(dev, a.data_ptr(), lda, mat2.data_ptr(), ldw if N > 1 else K, gsw if E > 1 else 0, y, ldd, code, T, N, K, E,
+                offs.data_ptr(), scale_a, sa, scale_b, sb_group, sb, bias, bias_code, N, int(out is None))
 
 
 # torch.compile must not trace into these entry points (they call a foreign library through ctypes)
