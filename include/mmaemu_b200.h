@@ -233,12 +233,14 @@ int mmb200_kernel_for(const void *A_dev, int64_t lda, const void *B_dev, int64_t
  * B + e * group_stride_b, the scales scale_a_dev[e * sa_stride] and scale_b_dev[e * sb_stride] (stride 0: one scale for all
  * groups) and the split decision splits[e], schemes[e] (NULL: no group is split). The result has the bits of a loop of
  * mmb200_scaled_mm_ws calls, whatever kernel runs. m_splits, splits and schemes are HOST arrays of E entries, read during
- * the call (the split decision of the emulated platform depends on a group's rows). Scratch memory as there:
+ * the call (the split decision of the emulated platform depends on a group's rows). With scratch memory the unsplit groups
+ * run in one pass of launches (up to 8 GiB of decoded operands), the others one after the other. Scratch memory as there:
  * mmb200_grouped_workspace_bytes; mmb200_grouped_status synchronises `stream` and reports whether a bounded wait of the call
  * that last used it ran out (the outputs of that group then keep their previous contents). The reference has no grouped
  * call. */
 #define MMB200_MAX_GROUPS 4096
-size_t mmb200_grouped_workspace_bytes(const int *m_splits, const int *splits, int E, int N, int K);
+size_t mmb200_grouped_workspace_bytes(const int *m_splits, const int *splits, int E, int N, int K, int fmt_a, int fmt_b,
+                                      int nfma, int fast);
 int mmb200_grouped_scaled_mm(const void *A_dev, int64_t lda, int fmt_a, const void *B_dev, int64_t ldb,
                              int64_t group_stride_b, int fmt_b, void *D_dev, int64_t ldd, int out_dtype,
                              const int *m_splits, const int *splits, const int *schemes, int E, int N, int K, int nfma,

@@ -104,7 +104,7 @@ def load():
         L.mmb200_kernel_for.argtypes = [vp, i64, vp, i64, ci, ci, ci]
         L.mmb200_kernel_for.restype = ci
         sz = ctypes.c_size_t
-        L.mmb200_grouped_workspace_bytes.argtypes = [vp, vp, ci, ci, ci]
+        L.mmb200_grouped_workspace_bytes.argtypes = [vp, vp, ci, ci, ci, ci, ci, ci, ci]
         L.mmb200_grouped_workspace_bytes.restype = sz
         L.mmb200_grouped_scaled_mm.argtypes = [vp, i64, ci, vp, i64, i64, ci, vp, i64, ci, vp, vp, vp, ci, ci, ci, ci, ci, vp, ci,
                                                vp, ci, vp, ci, vp, sz, vp]

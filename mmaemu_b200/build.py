@@ -20,9 +20,9 @@ SOURCES = ("api.cu", "kernel_integer.cu", "kernel_fast.cu", "kernel_umma.cu", "k
            "static_scratch.cu")
 # translation units: (source, extra defines). kernel_fast.cu is compiled once per FP8 format pair and kind of kernel
 # (tensor cores: parts 0..3, CUDA cores: 4..7), in parallel.
-UNITS = (("api.cu", ()), ("kernel_integer.cu", ()), ("static_scratch.cu", ()), ("kernel_umma.cu", ()),
+UNITS = (("api.cu", ()), ("kernel_integer.cu", ()), ("static_scratch.cu", ()), ("kernel_umma.cu", ("-DMMB_GROUPED=0",)),
          *(("kernel_fast.cu", (f"-DMMB_PART={part}",)) for part in range(8)),
-         ("kernel_int8.cu", ()), ("kernel_quantise.cu", ()))
+         ("kernel_int8.cu", ()), ("kernel_quantise.cu", ()), ("kernel_umma.cu", ("-DMMB_GROUPED=1",)))
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "--fmad=false", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 OBJ = PKG / "csrc" / "_obj"

@@ -522,18 +522,60 @@ int mmb200_scaled_mm_host(const void* A, int64_t lda, int fmt_a, const void* B, 
   return MMB200_OK;
 }
 
-// Scratch memory of a grouped call: a status word for all its launches, then the scratch memory of one group after the other.
+// Scratch memory of a grouped call: a status word for all its launches, then that of the fused launches, or of one group
+// after the other.
 constexpr size_t GROUPED_HEADER = 256;
+constexpr size_t GROUPED_SCRATCH_LIMIT = (size_t)8 << 30;       // decoded operands of all groups at once: at most this much
 
-size_t mmb200_grouped_workspace_bytes(const int* m_splits, const int* splits, int E, int N, int K) {
+namespace {
+// What the fused launches need to know of a grouped call: formats, sizes and the plan.
+mmb::Params grouped_params(long long rows, int N, int K, int fmt_a, int fmt_b, int fast) {
+  mmb::Params p;
+  std::memset(&p, 0, sizeof(p));
+  p.M = (int)rows; p.N = N; p.K = K;
+  p.fmt_a = fmt_a; p.fmt_b = fmt_b;
+  p.fast = fast ? 1 : 0;
+  p.S = 1;
+  p.no_tensor_epass = mmb::tensor_cores_off() ? 1 : 0;
+  return p;
+}
+// The groups of the fused launches: those with rows and an unsplit plan; `any` is false when there are fewer than two (a single
+// one has the whole choice of kernels).
+struct FusedGroups {
+  unsigned char use[MMB200_MAX_GROUPS];
+  bool any;
+  FusedGroups(const int* m_splits, const int* splits, int E) {
+    int n = 0;
+    for (int e = 0; e < E; ++e) {
+      use[e] = m_splits[e] > 0 && (!splits || splits[e] == 1);
+      n += use[e];
+    }
+    any = n >= 2;
+  }
+};
+size_t fused_bytes(const mmb::Params& p, int nfma, const int* m_splits, const FusedGroups& g, int E) {
+  const size_t n = g.any ? mmb::grouped_workspace_bytes(p, nfma, m_splits, g.use, E) : 0;
+  return n <= GROUPED_SCRATCH_LIMIT ? n : 0;
+}
+}  // namespace
+
+size_t mmb200_grouped_workspace_bytes(const int* m_splits, const int* splits, int E, int N, int K, int fmt_a, int fmt_b, int nfma,
+                                      int fast) {
   if (!m_splits || E <= 0 || E > MMB200_MAX_GROUPS || N <= 0 || K <= 0) return 0;
+  long long rows = 0;
+  for (int e = 0; e < E; ++e) rows += m_splits[e] > 0 ? m_splits[e] : 0;
+  if (rows > 0x7FFFFFFFLL) return 0;
+  const mmb::Params p = grouped_params(rows, N, K, fmt_a, fmt_b, fast);
+  const FusedGroups groups(m_splits, splits, E);
+  const size_t fused = fused_bytes(p, nfma, m_splits, groups, E);
   size_t most = 0;
   for (int e = 0; e < E; ++e) {
-    if (m_splits[e] <= 0) continue;
+    if (m_splits[e] <= 0 || (fused && groups.use[e])) continue;
     const size_t n = mmb::staged_workspace_bytes(m_splits[e], N, K, splits ? splits[e] : 1, true, false, mmb::tensor_cores_off());
     if (n > most) most = n;
   }
-  return most ? GROUPED_HEADER + most : 0;
+  most = most ? GROUPED_HEADER + most : 0;
+  return fused > most ? fused : most;
 }
 
 int mmb200_grouped_status(const void* workspace, void* stream) {
@@ -546,11 +588,10 @@ int mmb200_grouped_status(const void* workspace, void* stream) {
   return word ? MMB200_ERR_TIMEOUT : MMB200_OK;
 }
 
-int mmb200_grouped_scaled_mm(const void* A, int64_t lda, int fmt_a, const void* B, int64_t ldb, int64_t group_stride_b, int fmt_b,
-                             void* D, int64_t ldd, int out_dtype, const int* m_splits, const int* splits, const int* schemes,
-                             int E, int N, int K, int nfma, int fast, const float* scale_a, int sa_stride, const float* scale_b,
-                             int sb_stride, const float* scale_result, int kernel, void* workspace, size_t workspace_bytes,
-                             void* stream) {
+static int grouped_run(const void* A, int64_t lda, int fmt_a, const void* B, int64_t ldb, int64_t group_stride_b, int fmt_b, void* D,
+                       int64_t ldd, int out_dtype, const int* m_splits, const int* splits, const int* schemes, int E, int N, int K,
+                       int nfma, int fast, const float* scale_a, int sa_stride, const float* scale_b, int sb_stride,
+                       const float* scale_result, int kernel, void* workspace, size_t workspace_bytes, void* stream) {
   if (E < 0 || N < 0 || K < 0 || (E > 0 && !m_splits) || !splits != !schemes) return MMB200_ERR_BAD_ARG;
   if (E > MMB200_MAX_GROUPS) return MMB200_ERR_TOO_LARGE;
   if (!scale_a || !scale_b || sa_stride < 0 || sb_stride < 0 || group_stride_b < 0) return MMB200_ERR_BAD_ARG;
@@ -561,32 +602,76 @@ int mmb200_grouped_scaled_mm(const void* A, int64_t lda, int fmt_a, const void* 
     rows += m_splits[e];
   }
   if (rows > 0x7FFFFFFFLL) return MMB200_ERR_TOO_LARGE;
+  if (rows == 0 || N == 0) return fmt_ok(fmt_a) && fmt_ok(fmt_b) ? MMB200_OK : MMB200_ERR_BAD_ARG;
   const size_t es = out_size(out_dtype);
-  const uint8_t* a = static_cast<const uint8_t*>(A);
-  uint8_t* d = static_cast<uint8_t*>(D);
   int* word = nullptr;
-  if (workspace && workspace_bytes > GROUPED_HEADER && rows > 0 && N > 0) {
+  const FusedGroups groups(m_splits, splits, E);
+  bool fused = false;
+  if (workspace && workspace_bytes > GROUPED_HEADER) {
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int rc = current_device_ok();
     if (rc != MMB200_OK) return rc;
     word = static_cast<int*>(workspace);
-    const cudaError_t err = cudaMemsetAsync(word, 0, sizeof(int), static_cast<cudaStream_t>(stream));
-    if (err != cudaSuccess) return cuda_fail(err);
+    // the fused launches take what the loop below would give to the scratch-memory kernels
+    const bool valid = fmt_ok(fmt_a) && fmt_ok(fmt_b) && A && B && D && lda >= K && ldb >= K && ldd >= N && K < (1 << 24);
+    if (valid && kernel != MMB200_KERNEL_INTEGER && !(reinterpret_cast<uintptr_t>(workspace) & 127)) {
+      mmb::Params p = grouped_params(rows, N, K, fmt_a, fmt_b, fast);
+      p.A = static_cast<const uint8_t*>(A);
+      p.B = static_cast<const uint8_t*>(B);
+      p.D = D;
+      p.scale_a = scale_a; p.scale_b = scale_b; p.scale_result = scale_result;
+      p.lda = lda; p.ldb = ldb; p.ldd = ldd;
+      p.out_dtype = out_dtype;
+      p.epilogue = p.patch_nonfinite = 1;
+      p.group_stride_b = group_stride_b;
+      p.sa_stride = sa_stride; p.sb_stride = sb_stride;
+      const size_t need = fused_bytes(p, nfma, m_splits, groups, E);
+      const bool named = kernel == MMB200_KERNEL_FAST && !(mmb::staged_vector_supports(p, nfma) && !(group_stride_b & 15));
+      if (need && workspace_bytes >= need && !named) {
+        int launches = 0;
+        const cudaError_t err = mmb::launch_grouped(p, nfma, m_splits, groups.use, E, workspace, workspace_bytes, st, &launches);
+        g_launches.fetch_add(launches, std::memory_order_relaxed);
+        if (err != cudaSuccess) return cuda_fail(err);
+        fused = true;
+      }
+    }
+    if (!fused) {
+      const cudaError_t err = cudaMemsetAsync(word, 0, sizeof(int), st);
+      if (err != cudaSuccess) return cuda_fail(err);
+    }
     workspace = static_cast<unsigned char*>(workspace) + GROUPED_HEADER;
     workspace_bytes -= GROUPED_HEADER;
   } else {
     workspace = nullptr;
     workspace_bytes = 0;
   }
+  const uint8_t* a = static_cast<const uint8_t*>(A);
+  uint8_t* d = static_cast<uint8_t*>(D);
   for (int e = 0; e < E; ++e) {
-    const int rc = run(a, lda, fmt_a, static_cast<const uint8_t*>(B) + (size_t)e * (size_t)group_stride_b, ldb, fmt_b, d, ldd,
-                       out_dtype, m_splits[e], N, K, nfma, fast, splits ? splits[e] : 1, splits ? schemes[e] : 0,
-                       scale_a + (size_t)e * sa_stride, scale_b + (size_t)e * sb_stride, scale_result, 1, 1, kernel, stream,
-                       workspace, workspace_bytes, nullptr, 0, 0, nullptr, nullptr, 0, nullptr, mmb::tensor_cores_off(), word);
-    if (rc != MMB200_OK) return rc;
+    if (!fused || !groups.use[e]) {
+      const int rc = run(a, lda, fmt_a, static_cast<const uint8_t*>(B) + (size_t)e * (size_t)group_stride_b, ldb, fmt_b, d, ldd,
+                         out_dtype, m_splits[e], N, K, nfma, fast, splits ? splits[e] : 1, splits ? schemes[e] : 0,
+                         scale_a + (size_t)e * sa_stride, scale_b + (size_t)e * sb_stride, scale_result, 1, 1, kernel, stream,
+                         workspace, workspace_bytes, nullptr, 0, 0, nullptr, nullptr, 0, nullptr, mmb::tensor_cores_off(), word);
+      if (rc != MMB200_OK) return rc;
+    }
     a += (size_t)m_splits[e] * (size_t)lda;
     d += (size_t)m_splits[e] * (size_t)ldd * es;
   }
   return MMB200_OK;
+}
+
+int mmb200_grouped_scaled_mm(const void* A, int64_t lda, int fmt_a, const void* B, int64_t ldb, int64_t group_stride_b, int fmt_b,
+                             void* D, int64_t ldd, int out_dtype, const int* m_splits, const int* splits, const int* schemes,
+                             int E, int N, int K, int nfma, int fast, const float* scale_a, int sa_stride, const float* scale_b,
+                             int sb_stride, const float* scale_result, int kernel, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  try {                                      // the lists of K slices are host memory
+    return grouped_run(A, lda, fmt_a, B, ldb, group_stride_b, fmt_b, D, ldd, out_dtype, m_splits, splits, schemes, E, N, K, nfma, fast,
+                       scale_a, sa_stride, scale_b, sb_stride, scale_result, kernel, workspace, workspace_bytes, stream);
+  } catch (...) {
+    return cuda_fail(cudaErrorMemoryAllocation);
+  }
 }
 
 int mmb200_quantize_int8(const void* X, int64_t ldx, int x_dtype, int8_t* codes, int64_t ldc, float* scale, int64_t rows, int K,

@@ -20,6 +20,8 @@ constexpr int PRESET_B200_MMA_SYNC = MMB200_PRESET_B200_MMA_SYNC;   // late-accu
 constexpr uint32_t CANON_NAN32 = 0x7FFFFFFFu;
 #define MMB200_MAX_SLICES 32
 
+struct RowTile;
+
 // Everything a kernel needs; passed by value (__grid_constant__).
 struct Params {
   const uint8_t* A;   // [M, K] codes, row stride lda
@@ -87,7 +89,17 @@ struct Params {
   int byte_loads;        // the operands cannot be read with 16-byte loads (staged kernels: they read single codes)
   int umma;              // the launch runs on the tcgen05 kernels: chain results are laid out [column][row] per tile
   int wide_tiles;        // tcgen05, unsplit: 256 columns per CTA instead of 128
+  // Ragged groups (launch_grouped): row tiles listed one by one in scratch memory instead of every 128 (16) rows. Rows, and
+  // with them A, D and the row flags, are numbered through all groups; B, its flags and the scales are the group's.
+  const RowTile* ws_tiles;       // [tiles_m]
+  const int* ws_slots;           // group of every decoded B
+  int slots;                     // decoded Bs
+  long long group_stride_b;
+  int sa_stride, sb_stride;
 };
+
+// One tile of rows of a grouped launch: rows [m0, m_end) of group g, whose flags (and decoded tiles) of B are number `slot`.
+struct __align__(16) RowTile { int m0, m_end, g, slot; };
 
 // ---------------------------------------------------------------------------------------------------------------
 // FP8 decode of one code byte into (magnitude significand, clamped exponent, sign, class).
@@ -196,10 +208,11 @@ struct Epilogue {
   float alpha, scale_result;
   int has_scale_result, out_dtype, enabled, n_peers;
   void* const* peers;
-  __device__ __forceinline__ void init(const Params& p) {
+  __device__ __forceinline__ void init(const Params& p) { init(p, p.scale_a, p.scale_b); }
+  __device__ __forceinline__ void init(const Params& p, const float* scale_a, const float* scale_b) {
     enabled = p.epilogue;
     out_dtype = p.out_dtype;
-    const float sa = p.scale_a ? *p.scale_a : 1.0f, sb = p.scale_b ? *p.scale_b : 1.0f;
+    const float sa = scale_a ? *scale_a : 1.0f, sb = scale_b ? *scale_b : 1.0f;
     alpha = __fmul_rn(sa, sb);
     has_scale_result = p.scale_result != nullptr;
     scale_result = has_scale_result ? *p.scale_result : 1.0f;
@@ -278,15 +291,15 @@ struct Epilogue {
                                                         b[q + 4] | (b[q + 5] << 8) | (b[q + 6] << 16) | (b[q + 7] << 24));
     }
   }
-  // `rows`: how many rows of the image (from its first) were parked
+  // `rows`: how many rows of the image (from its first) were parked; m_end: the first row behind the problem (the group)
   __device__ __forceinline__ void flush(const Params& p, const unsigned char* tile, int m0, int n0, int tid,
-                                        int nthreads, int rows = TILE_DIM) const {
+                                        int nthreads, int rows, int m_end) const {
     const int es = elem_size(), pitch = tile_pitch(), per_row = TILE_DIM * es / 16, per_piece = 16 / es;
     bool vec = (reinterpret_cast<uintptr_t>(p.D) % 16 == 0) && ((p.ldd * es) % 16 == 0);
     for (int q = 0; q < n_peers; ++q) vec = vec && (reinterpret_cast<uintptr_t>(peers[q]) % 16 == 0);
     for (int idx = tid; idx < rows * per_row; idx += nthreads) {
       const int row = idx / per_row, piece = idx % per_row, gm = m0 + row, gn = n0 + piece * per_piece;
-      if (gm >= p.M || gn >= p.N) continue;
+      if (gm >= m_end || gn >= p.N) continue;
       const unsigned char* src = tile + row * pitch + piece * 16;
       const long long off = ((long long)gm * p.ldd + gn) * es;
       if (vec && gn + per_piece <= p.N) {
@@ -309,6 +322,13 @@ cudaError_t launch_integer(const Params& p, int nfma, cudaStream_t stream);
 cudaError_t launch_fast(const Params& p, int nfma, cudaStream_t stream);
 // tcgen05 kernels (kernel_umma.cu), called by the staged launches: operand images, then the GEMM; p filled in by them.
 cudaError_t launch_umma(const Params& p, int nfma, cudaStream_t stream, int* launches);
+cudaError_t launch_umma_grouped(const Params& p, int nfma, cudaStream_t stream, int* launches);
+// Ragged groups with unsplit plans on the tensor cores: scratch bytes (0: not served; the caller goes group by group), and the
+// launch. `rows`: rows of each of the E groups, `use`: whether the launch takes the group (null: all of them). p: the operands,
+// K, N and formats of the call, p.M its rows.
+size_t grouped_workspace_bytes(const Params& p, int nfma, const int* rows, const unsigned char* use, int E);
+cudaError_t launch_grouped(const Params& p, int nfma, const int* rows, const unsigned char* use, int E, void* workspace,
+                           size_t workspace_bytes, cudaStream_t stream, int* launches);
 bool fast_supports(const Params& p, int nfma);
 // Staged fast kernel: scratch bytes it needs for a shape (0: a shape it does not take), and the launch (pre-decode of both
 // operands, then the GEMM).

@@ -37,6 +37,7 @@
 // its arithmetic.
 #include <atomic>
 #include <cstdlib>
+#include <cstring>
 #include <vector>
 
 #include "common.cuh"
@@ -533,7 +534,7 @@ __device__ __forceinline__ void split_end(float (&acc)[TM][TN], float (*part)[TH
 // ends a chain every 4 k-tiles (128 elements). MODE 1, any plan by its tile sequence: the entry says whether a chain or
 // the split ends here. MODE 2, one K slice of a plan: every finished chain is cut and stored for the combine kernel.
 constexpr int MODE_ORDER = 0, MODE_PLAN = 1, MODE_SLICED = 2;
-template <bool SLOW, int MODE, int TMI, bool TC>
+template <bool SLOW, int MODE, int TMI, bool TC, int CHAIN_FLOATS = TM * TN * THREADS>
 __device__ __forceinline__ void after_tile(const Params& p, float (&acc)[TM][TN], float (*part)[THREADS], int t,
                                            uint32_t entry, int tid, int& chain, int half = -1, int group = 0) {
   if (MODE == MODE_SLICED) {
@@ -544,7 +545,7 @@ __device__ __forceinline__ void after_tile(const Params& p, float (&acc)[TM][TN]
       // warps stores its own four column slots.
       const int owner = half < 0 ? tid : (group / 4) * (THREADS / 2) + tid % (THREADS / 2);
       const int slot0 = half < 0 ? 0 : 2 * (group % 4);
-      float* dst = p.ws_chains + ((size_t)blockIdx.x * p.n_chains + chain) * (TM * TN * THREADS) + owner;
+      float* dst = p.ws_chains + ((size_t)blockIdx.x * p.n_chains + chain) * CHAIN_FLOATS + owner;
 #pragma unroll
       for (int i = 0; i < TMI; ++i)
 #pragma unroll
@@ -568,6 +569,7 @@ __device__ __forceinline__ void after_tile(const Params& p, float (&acc)[TM][TN]
 // Second pass of the K-sliced execution: one thread per output adds the stored chain results in the plan's order
 // (chains into the split's sum for slow accumulation, split partials into the reduction by their roles), then the
 // non-finite patch and the epilogue. Grid: (output tiles, 64 outputs per thread of the first pass), 256 threads.
+template <bool GROUPED>
 __global__ void __launch_bounds__(THREADS) combine_kernel(const __grid_constant__ Params p) {
   const int tid = threadIdx.x, idx = blockIdx.y, i = idx / TN, j = idx % TN;
   int tile_m, tile_n;
@@ -575,13 +577,14 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const __grid_constant_
   const Lane ln(tid);
   // the position of a chain result in its tile: by the threads of the first pass, or [column][row] (tcgen05 kernels)
   const int lin = idx * THREADS + tid;
-  const int gm = tile_m * BM + (p.umma ? lin % BM : ln.row(i)), gn = tile_n * BN + (p.umma ? lin / BM : ln.col(j));
-  if (gm >= p.M || gn >= p.N) return;
+  const RowTile rt = row_tile<GROUPED, BM>(p, tile_m);
+  const int gm = rt.m0 + (p.umma ? lin % BM : ln.row(i)), gn = tile_n * BN + (p.umma ? lin / BM : ln.col(j));
+  if (gm >= rt.m_end || gn >= p.N) return;
   if (p.status && *reinterpret_cast<volatile int*>(p.status)) return;   // a slice gave up waiting: no output, as in the other modes
-  const float* src = p.ws_chains + (size_t)blockIdx.x * p.n_chains * (TM * TN * THREADS) + (size_t)idx * THREADS + tid;
+  constexpr size_t STRIDE = (size_t)(GROUPED ? 2 : TM) * TN * THREADS;
+  const float* src = p.ws_chains + (size_t)blockIdx.x * p.n_chains * STRIDE + (size_t)idx * THREADS + tid;
   const bool slow = p.plan_group != 0;
   float tot = 0.0f, slot = 0.0f, part = 0.0f, last = 0.0f;
-  constexpr size_t STRIDE = (size_t)TM * TN * THREADS;
   constexpr int BLOCK = 16;
   // The chain results are read sixteen at a time, the next sixteen while the current ones are added (the loads do not
   // depend on the additions); every chain then consumes the list entries up to the one that completes it.
@@ -626,14 +629,15 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const __grid_constant_
     if (entry & SEQ_SPLIT_END) split_end(entry);
   }
   float v = tot;
-  if (p.patch_nonfinite && (p.ws_flag_a[gm] | p.ws_flag_b[gn])) {
+  const int flag = p.ws_flag_a[gm] | flags_b<GROUPED>(p, rt)[gn];
+  if (p.patch_nonfinite && flag) {
     uint32_t bits;
-    if (nonfinite_patch(p.ws_flag_a[gm] | p.ws_flag_b[gn], p.A + (long long)gm * p.lda, p.B + (long long)gn * p.ldb, p.K,
-                        p.fmt_a, p.fmt_b, bits))
+    if (nonfinite_patch(flag, p.A + (long long)gm * p.lda, operand_b<GROUPED>(p, rt) + (long long)gn * p.ldb, p.K, p.fmt_a, p.fmt_b,
+                        bits))
       v = __uint_as_float(bits);
   }
   Epilogue epi;
-  epi.init(p);
+  init_epilogue<GROUPED>(epi, p, rt);
   epi.store(p.D, (long long)gm * p.ldd + gn, v);
 }
 
@@ -674,17 +678,19 @@ __global__ void plan_sequence_kernel(Plan plan, int K, uint32_t* out, uint32_t* 
 // Non-finite patch and epilogue for the thread's outputs. flag_a / flag_b: per-row classes of the tile's rows / columns.
 // The converted elements are parked in `tile` (shared memory that no thread reads any more: the caller has
 // synchronised the CTA) and written out row-wise by the whole CTA.
-template <bool SLOW, int TMI>
+template <bool SLOW, int TMI, bool GROUPED = false>
 __device__ __forceinline__ void write_tile(const Params& p, const float (&acc)[TM][TN], float (*part)[THREADS],
-                                           const int* flag_a, const int* flag_b, int m0, int n0, const Lane& ln,
+                                           const int* flag_a, const int* flag_b, const RowTile& rt, int n0, const Lane& ln,
                                            int tid, unsigned char* tile, const float* tot = nullptr,
                                            int rows = BM) {
   Epilogue epi;
-  epi.init(p);
+  init_epilogue<GROUPED>(epi, p, rt);
+  const uint8_t* B = operand_b<GROUPED>(p, rt);
+  const int m0 = rt.m0;
 #pragma unroll
   for (int i = 0; i < TMI; ++i) {
     const int lr = ln.row(i), gm = m0 + lr;
-    if (gm >= p.M) continue;
+    if (gm >= rt.m_end) continue;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int lc = ln.col(j), gn = n0 + lc;
@@ -692,7 +698,7 @@ __device__ __forceinline__ void write_tile(const Params& p, const float (&acc)[T
       float v = tot ? tot[(i * TN + j) * THREADS + tid] : (SLOW ? part[i * TN + j][tid] : acc[i][j]);
       if (p.patch_nonfinite && (flag_a[lr] | flag_b[lc])) {
         uint32_t bits;
-        if (nonfinite_patch(flag_a[lr] | flag_b[lc], p.A + (long long)gm * p.lda, p.B + (long long)gn * p.ldb, p.K,
+        if (nonfinite_patch(flag_a[lr] | flag_b[lc], p.A + (long long)gm * p.lda, B + (long long)gn * p.ldb, p.K,
                             p.fmt_a, p.fmt_b, bits))
           v = __uint_as_float(bits);
       }
@@ -700,7 +706,7 @@ __device__ __forceinline__ void write_tile(const Params& p, const float (&acc)[T
     }
   }
   __syncthreads();
-  epi.flush(p, tile, m0, n0, tid, THREADS, rows);
+  epi.flush(p, tile, m0, n0, tid, THREADS, rows, rt.m_end);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -764,7 +770,7 @@ __global__ void __launch_bounds__(THREADS, 1) fast_kernel(const __grid_constant_
   }
   if (!SLOW || (p.K % 128) != 0) chain_end<SLOW, TM, false>(acc, sm.part, tid);
   __syncthreads();
-  write_tile<SLOW, TM>(p, acc, sm.part, sm.flag_a, sm.flag_b, m0, n0, ln, tid, smem_raw);
+  write_tile<SLOW, TM>(p, acc, sm.part, sm.flag_a, sm.flag_b, RowTile{m0, p.M, 0, 0}, n0, ln, tid, smem_raw);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -778,7 +784,7 @@ __global__ void __launch_bounds__(THREADS) predecode_kernel(const __grid_constan
   Tile& tile = reinterpret_cast<Tile*>(IS_A ? p.ws_a : p.ws_b)[(long long)rb * p.k_tiles + kt];
   int* flags = IS_A ? p.ws_flag_a : p.ws_flag_b;
   const int lrow = tid % 128, lhalf = tid / 128, row = rb * 128 + lrow, k = kt * KT + 16 * lhalf;
-  const uint4 raw = load_codes16<IS_A>(p, row, rows, k);
+  const uint4 raw = load_codes16<IS_A>(p, IS_A ? p.A : p.B, row, rows, k);
   const uint32_t cls = decode16<FA, FB, IS_A>(raw, tile, lrow, 16 * lhalf);
   if (cls) atomicOr(&flags[row], (int)cls);
 }
@@ -806,7 +812,7 @@ __global__ void __launch_bounds__(THREADS) predecode_tc_kernel(const __grid_cons
   TileTC& tile = reinterpret_cast<TileTC*>(IS_A ? p.ws_a : p.ws_b)[(long long)rb * p.k_tiles + kt];
   int* flags = IS_A ? p.ws_flag_a : p.ws_flag_b;
   const int lrow = tid % 128, lhalf = tid / 128, row = rb * 128 + lrow, k0 = kt * KT + 16 * lhalf;
-  const uint4 raw = load_codes16<IS_A>(p, row, rows, k0);
+  const uint4 raw = load_codes16<IS_A>(p, IS_A ? p.A : p.B, row, rows, k0);
   const uint32_t seen = decode16_tc<FA, FB, IS_A>(raw, tile, lrow, lhalf);
   if (seen) atomicOr(&flags[row], (int)seen);
 }
@@ -922,7 +928,7 @@ __device__ __forceinline__ void staged_body(const Params& p, unsigned char* smem
   }
   if (SLICED) return;                        // a slice has stored its chains; the combine kernel writes the output
   if (!PLAN && (!SLOW || (T % 4) != 0)) chain_end<SLOW, TMI, TC>(acc, sm.part, tid);
-  write_tile<SLOW, TMI>(p, acc, sm.part, p.ws_flag_a + m0, p.ws_flag_b + n0, m0, n0, ln, tid, smem_raw,
+  write_tile<SLOW, TMI>(p, acc, sm.part, p.ws_flag_a + m0, p.ws_flag_b + n0, RowTile{m0, p.M, 0, 0}, n0, ln, tid, smem_raw,
                         PLAN ? p.ws_tot + (size_t)blockIdx.x * (TM * TN * THREADS) : nullptr);
 }
 
@@ -946,7 +952,7 @@ template <bool TC> constexpr size_t smem_few(bool with_part) {
 // copies. One barrier of the CTA per k-tile; no waits that can run out. The row and column flags of non-finite codes go
 // to the same scratch arrays as in the pre-decoded kernels (a K slice sees only its part of K; the combine kernel runs
 // after all slices).
-template <int NFMA, int FA, int FB, bool SLOW, int MODE, bool TC>
+template <int NFMA, int FA, int FB, bool SLOW, int MODE, bool TC, bool GROUPED = false>
 __device__ __forceinline__ void few_rows_body(const Params& p, unsigned char* smem_raw) {
   constexpr int TMI = 2;
   static_assert(STRIPS == 2, "the 16-row kernels split the column strips between the two halves of the warps");
@@ -957,8 +963,12 @@ __device__ __forceinline__ void few_rows_body(const Params& p, unsigned char* sm
   int tile_m, tile_n;
   tile_of_cta(p, (int)blockIdx.x, tile_m, tile_n);
   const int group = (int)blockIdx.z;         // 16-row group of the 128-row tile
-  const int m0 = tile_m * BM + 16 * group, n0 = tile_n * BN;
-  if (m0 >= p.M) return;                     // the whole CTA: no barrier has been reached
+  RowTile rt = row_tile<GROUPED, BM>(p, tile_m);
+  if (!GROUPED) rt.m0 += 16 * group;         // (the tiles of ragged groups have 16 rows)
+  const int m0 = rt.m0, n0 = tile_n * BN;
+  if (m0 >= rt.m_end) return;                // the whole CTA: no barrier has been reached
+  const uint8_t* B = operand_b<GROUPED>(p, rt);
+  int* flag_b = const_cast<int*>(flags_b<GROUPED>(p, rt));
   const Lane ln(tid, STRIPS == 2);
   const int t0 = SLICED ? p.slice_start[blockIdx.y] : 0;
   const int T = SLICED ? p.slice_start[blockIdx.y + 1] - t0 : (PLAN ? p.seq_len : p.k_tiles);
@@ -971,8 +981,8 @@ __device__ __forceinline__ void few_rows_body(const Params& p, unsigned char* sm
   auto fetch = [&](int t) {
     const int kt = PLAN ? (int)(__ldg(p.ws_seq + t0 + t) & SEQ_TILE_MASK) : t;
     const int k = kt * KT + 16 * lhalf;
-    raw_b = load_codes16<false>(p, n0 + lrow, p.N, k);
-    if (a_row) raw_a = load_codes16<true>(p, m0 + lrow, p.M, k);
+    raw_b = load_codes16<false>(p, B, n0 + lrow, p.N, k);
+    if (a_row) raw_a = load_codes16<true>(p, p.A, m0 + lrow, rt.m_end, k);
   };
   auto decode = [&](int t) {
     Stage& st = sm.stage[t & 1];
@@ -984,7 +994,7 @@ __device__ __forceinline__ void few_rows_body(const Params& p, unsigned char* sm
       cb = decode16<FA, FB, false>(raw_b, st.b, lrow, 16 * lhalf);
       if (a_row) ca = decode16<FA, FB, true>(raw_a, st.a, lrow, 16 * lhalf, a_pos);
     }
-    if (cb) atomicOr(&p.ws_flag_b[n0 + lrow], (int)cb);
+    if (cb) atomicOr(&flag_b[n0 + lrow], (int)cb);
     if (ca) atomicOr(&p.ws_flag_a[m0 + lrow], (int)ca);
   };
   float acc[TM][TN];
@@ -1013,12 +1023,12 @@ __device__ __forceinline__ void few_rows_body(const Params& p, unsigned char* sm
 #pragma unroll 1
       for (int c0 = 0; c0 < KT; c0 += NFMA) block_step<NFMA, FA, FB, TMI>(acc, st.a, st.b, c0, ln, tid % 32);
     }
-    after_tile<SLOW, MODE, TMI, TC>(p, acc, sm.part, t, entry, tid, chain, ln.half, group);
+    after_tile<SLOW, MODE, TMI, TC, GROUPED ? 2 * TN * THREADS : TM * TN * THREADS>(p, acc, sm.part, t, entry, tid, chain, ln.half, group);
     __syncthreads();                         // the next k-tile is decoded; nobody reads this one any more
   }
   if (SLICED) return;                        // a slice has stored its chains; the combine kernel writes the output
   if (!PLAN && (!SLOW || (T % 4) != 0)) chain_end<SLOW, TMI, TC>(acc, sm.part, tid);
-  write_tile<SLOW, TMI>(p, acc, sm.part, p.ws_flag_a + m0, p.ws_flag_b + n0, m0, n0, ln, tid, smem_raw, nullptr, 16);
+  write_tile<SLOW, TMI, GROUPED>(p, acc, sm.part, p.ws_flag_a + m0, flag_b + n0, rt, n0, ln, tid, smem_raw, nullptr, 16);
 }
 
 template <int NFMA, int FA, int FB, bool SLOW, int MODE, int TMI>
@@ -1032,6 +1042,13 @@ __global__ void __launch_bounds__(THREADS, TMI == 2 ? 2 : 1) staged_tc_kernel(co
   extern __shared__ __align__(128) unsigned char smem_raw[];
   if constexpr (TMI == 2) few_rows_body<NFMA, FA, FB, SLOW, MODE, true>(p, smem_raw);
   else staged_body<NFMA, FA, FB, SLOW, MODE, true, TMI>(p, smem_raw);
+}
+
+// The 16-row kernels on the row tiles of ragged groups.
+template <int NFMA, int FA, int FB, bool SLOW, int MODE>
+__global__ void __launch_bounds__(THREADS, 2) grouped_rows16_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  few_rows_body<NFMA, FA, FB, SLOW, MODE, true, true>(p, smem_raw);
 }
 
 // SMs of the current device (cached per device; 148 if the query fails).
@@ -1066,6 +1083,30 @@ cudaError_t launch_direct(const Params& p, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
+// 16-row tiles of ragged groups: one pass, or K slices (slow accumulation) and their combination.
+template <int NFMA, int FA, int FB>
+cudaError_t launch_grouped_rows16(const Params& p, cudaStream_t stream, int* launches) {
+  const unsigned tiles = (unsigned)((long long)p.tiles_m * p.tiles_n);
+  auto go = [&](auto kern, size_t smem) -> cudaError_t {
+    if ((long long)tiles * p.slices <= sm_count() && smem < ((size_t)120 << 10)) smem = (size_t)120 << 10;   // as launch_staged_main
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    kern<<<dim3(tiles, (unsigned)p.slices), THREADS, smem, stream>>>(p);
+    e = cudaGetLastError();
+    if (e == cudaSuccess) *launches += 1;
+    return e;
+  };
+  if (p.slices == 1)
+    return p.fast ? go(grouped_rows16_kernel<NFMA, FA, FB, false, MODE_ORDER>, smem_few<true>(false))
+                  : go(grouped_rows16_kernel<NFMA, FA, FB, true, MODE_ORDER>, smem_few<true>(true));
+  cudaError_t err = go(grouped_rows16_kernel<NFMA, FA, FB, true, MODE_SLICED>, smem_few<true>(false));
+  if (err != cudaSuccess) return err;
+  combine_kernel<true><<<dim3(tiles, 2 * TN), THREADS, 0, stream>>>(p);
+  err = cudaGetLastError();
+  if (err == cudaSuccess) *launches += 1;
+  return err;
+}
+
 // The main launch of a staged call (after the pre-decode launches): K slices + combine, a plan walk, or k order; with
 // two row slots per thread when the problem has at most 16 rows.
 template <int NFMA, int FA, int FB, bool TC>
@@ -1097,7 +1138,7 @@ cudaError_t launch_staged_main(const Params& p, cudaStream_t stream, int* launch
                                : go(MMB_KERNEL(false, MODE_SLICED, TM), small, (unsigned)p.slices);
     if (err != cudaSuccess) return err;
     // one CTA per (tile, output slot of the first pass's threads); with at most 16 rows only the row slots 0 and 1 exist
-    combine_kernel<<<dim3(tiles, p.M <= 16 ? 2 * TN : TM * TN), THREADS, 0, stream>>>(p);
+    combine_kernel<false><<<dim3(tiles, p.M <= 16 ? 2 * TN : TM * TN), THREADS, 0, stream>>>(p);
     err = cudaGetLastError();
     if (err == cudaSuccess) *launches += 2;
     return err;
@@ -1113,6 +1154,9 @@ cudaError_t launch_staged_main(const Params& p, cudaStream_t stream, int* launch
 template <int NFMA, int FA, int FB, bool TC>
 cudaError_t launch_staged_fmt(const Params& p, cudaStream_t stream, int* launches) {
   cudaError_t err = cudaSuccess;
+  if constexpr (TC && !(FA == MMB200_FMT_E5M2 && FB == MMB200_FMT_E5M2)) {
+    if (p.ws_tiles) return launch_grouped_rows16<NFMA, FA, FB>(p, stream, launches);
+  }
   // the kernels for at most 16 rows decode both operands themselves (few_rows_body)
   const bool direct = !p.only_b && p.few_rows && (p.slices > 1 || p.S == 1);
   if (direct) return launch_staged_main<NFMA, FA, FB, TC>(p, stream, launches);
@@ -1347,6 +1391,41 @@ void staged_wait_limits(int* wait_polls, int* announce_extra) {
   *announce_extra = g_announce_extra.load();
 }
 
+namespace {
+// Kernel choice by estimated time, in microseconds per k-tile of 32 and wave of CTAs (measured on whole calls at K = 4096,
+// overheads taken off): a 16-row CTA, alone on an SM or two sharing it; a 128 x 128 tile on tcgen05 (16 / 32 products
+// per block) or on mma.sync; 256 columns per tcgen05 CTA. K slices add two launches (slice_launch) and, per chain, the
+// traffic of the chain results. On the CUDA cores (MMAEMU_B200_TC_EPASS=0) a 16-row CTA takes 0.26 of a tile's time, two on
+// an SM 0.364, and the launches are small beside both (256-cube, slow: 22.7 us in two slices, 32.9 in one pass; 1024-cube,
+// fast, 16 products: 298 us on 16-row CTAs, 392 on tiles).
+struct KernelTimes {
+  bool one_sum;                              // one exponent sum per block: 256 columns per tcgen05 CTA are possible
+  double umma, mma, rows16, rows16_pair, slice_launch, predecode, margin;
+  KernelTimes(const Params& p, int nfma) {
+    const bool alu = p.no_tensor_epass != 0;
+    one_sum = nfma == 16 || (p.fmt_a == MMB200_FMT_E4M3 && p.fmt_b == MMB200_FMT_E4M3);
+    umma = nfma == 16 ? 2.2 : (one_sum ? 1.3 : 1.65);
+    mma = alu ? 8.0 : (nfma == 16 ? 3.3 : 3.0);
+    rows16 = alu ? 0.26 * mma : (nfma == 32 ? 0.95 : 1.25);
+    rows16_pair = alu ? 0.364 * mma : (nfma == 32 ? 1.35 : 1.75);
+    slice_launch = alu ? 0.0 : 8.0;
+    predecode = alu ? 0.0 : 12.0;
+    margin = alu ? 0.9 : 0.95;
+  }
+  double waves16(long long n, long long sms) const {
+    const long long pairs = n / (2 * sms), rest = n % (2 * sms);
+    return pairs * rows16_pair + (rest == 0 ? 0.0 : (rest <= sms ? rows16 : rows16_pair));
+  }
+  // 256 columns per CTA take 1.35 to 1.5 times as long a wave as 128 with fast accumulation, 1.6 to 1.67 with slow (4096-cube:
+  // 0.92 against 1.20 ms, 1.21 against 1.31 ms), so they pay unless half as many tiles leave much of a wave idle
+  static double wide_wave(bool fast) { return fast ? 1.45 : 1.65; }
+};
+bool env_off(const char* name) {
+  const char* env = std::getenv(name);
+  return env && env[0] == '0' && env[1] == 0;
+}
+}  // namespace
+
 cudaError_t launch_staged(const Params& p_in, int nfma, void* workspace, size_t workspace_bytes, cudaStream_t stream,
                           int* launches) {
   Params p = p_in;
@@ -1368,10 +1447,6 @@ cudaError_t launch_staged(const Params& p_in, int nfma, void* workspace, size_t 
     const long long tiles16 = (long long)w.tiles_n * ((p.M + 15) / 16);
     bool rows16 = !p.a_hp && p.M <= 16;
     int chains = 1;
-    auto env_off = [](const char* name) {
-      const char* env = std::getenv(name);
-      return env && env[0] == '0' && env[1] == 0;
-    };
     // MMAEMU_B200_SLICES=0: never slice; MMAEMU_B200_ROW_GROUPS=0: 16-row kernels only for calls of at most 16 rows
     // (both: tests that aim at the other kernels on small shapes)
     const bool can_slice = !env_off("MMAEMU_B200_SLICES") && wx.chains_bytes && workspace_bytes >= wx.total &&
@@ -1389,23 +1464,12 @@ cudaError_t launch_staged(const Params& p_in, int nfma, void* workspace, size_t 
       const size_t need = (size_t)tiles * (size_t)chains * TM * TN * THREADS * sizeof(float);
       return (n >= 2 && need <= wx.chains_bytes) ? n : 1;
     };
-    // Kernel choice by estimated time, in microseconds per k-tile of 32 and wave of CTAs (measured on whole calls at K = 4096,
-    // overheads taken off): a 16-row CTA, alone on an SM or two sharing it; a 128 x 128 tile on tcgen05 (16 / 32 products
-    // per block) or on mma.sync; 256 columns per tcgen05 CTA. K slices add two launches (SLICE_LAUNCH) and, per chain, the
-    // traffic of the chain results. On the CUDA cores (MMAEMU_B200_TC_EPASS=0) a 16-row CTA takes 0.26 of a tile's time, two on
-    // an SM 0.364, and the launches are small beside both (256-cube, slow: 22.7 us in two slices, 32.9 in one pass; 1024-cube,
-    // fast, 16 products: 298 us on 16-row CTAs, 392 on tiles).
     const long long sms = sm_count();
     const bool umma_any = umma_supports(p) && !(shared_b && p.S > 1), umma_whole = umma_any && p.S == 1;
-    const bool one_sum = nfma == 16 || (p.fmt_a == MMB200_FMT_E4M3 && p.fmt_b == MMB200_FMT_E4M3);
-    const double UMMA = nfma == 16 ? 2.2 : (one_sum ? 1.3 : 1.65), MMA = alu ? 8.0 : (nfma == 16 ? 3.3 : 3.0);
-    const double ROWS16 = alu ? 0.26 * MMA : (nfma == 32 ? 0.95 : 1.25);
-    const double ROWS16_PAIR = alu ? 0.364 * MMA : (nfma == 32 ? 1.35 : 1.75);
-    const double SLICE_LAUNCH = alu ? 0.0 : 8.0, PREDECODE = alu ? 0.0 : 12.0, MARGIN = alu ? 0.9 : 0.95;
-    auto waves16 = [&](long long n) {
-      const long long pairs = n / (2 * sms), rest = n % (2 * sms);
-      return pairs * ROWS16_PAIR + (rest == 0 ? 0.0 : (rest <= sms ? ROWS16 : ROWS16_PAIR));
-    };
+    const KernelTimes kt(p, nfma);
+    const bool one_sum = kt.one_sum;
+    const double UMMA = kt.umma, MMA = kt.mma, SLICE_LAUNCH = kt.slice_launch, PREDECODE = kt.predecode, MARGIN = kt.margin;
+    auto waves16 = [&](long long n) { return kt.waves16(n, sms); };
     auto sliced = [&](double per_tile, int n) { return per_tile * w.k_tiles / n + (n > 1 ? SLICE_LAUNCH : 0.0); };
     const int s128 = slices_for(tiles);
     const double umma_tile = (double)((tiles * s128 + sms - 1) / sms) * (umma_any ? UMMA : MMA);
@@ -1433,12 +1497,9 @@ cudaError_t launch_staged(const Params& p_in, int nfma, void* workspace, size_t 
     if (slices > 1)
       for (uint32_t entry : seq)
         if (entry & SEQ_EMPTY) p.umma = 0;     // splits without k-tiles: the general walkers
-    // 256 columns per CTA (one exponent sum per block): a wave of them takes 1.35 to 1.5 times as long as one of 128 columns
-    // with fast accumulation, 1.6 to 1.67 with slow (4096-cube: 0.92 against 1.20 ms, 1.21 against 1.31 ms), so they pay
-    // unless half as many tiles leave much of a wave idle
     const long long wide = (long long)w.tiles_m * ((w.tiles_n + 1) / 2);
     p.wide_tiles = p.umma && slices == 1 && one_sum &&
-                   (double)((wide + sms - 1) / sms) * (p.fast ? 1.45 : 1.65) < (double)((tiles + sms - 1) / sms);
+                   (double)((wide + sms - 1) / sms) * KernelTimes::wide_wave(p.fast != 0) < (double)((tiles + sms - 1) / sms);
     if (slices >= 2) {
       w = wx;
       p.slices = slices;
@@ -1486,12 +1547,217 @@ cudaError_t launch_staged(const Params& p_in, int nfma, void* workspace, size_t 
   if (p.umma) {
     err = launch_umma(p, nfma, stream, launches);
     if (err != cudaSuccess || p.slices == 1) return err;
-    combine_kernel<<<dim3((unsigned)(w.tiles_m * w.tiles_n), TM * TN), THREADS, 0, stream>>>(p);
+    combine_kernel<false><<<dim3((unsigned)(w.tiles_m * w.tiles_n), TM * TN), THREADS, 0, stream>>>(p);
     err = cudaGetLastError();
     if (err == cudaSuccess) *launches += 1;
     return err;
   }
   return dispatch_formats(p, nfma, stream, true, launches);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Ragged groups, unsplit plans: all groups in one pass of launches. Groups of up to `few` rows run on 16-row tiles, the others
+// on 128-row tcgen05 tiles; both walk a list of row tiles that a small kernel writes from the group sizes.
+namespace {
+
+struct GroupEntry { int g, row0, rows, slot, first_tile, tile_rows; };      // first_tile: in the list
+template <int CAP>
+struct GroupTable { GroupEntry e[CAP]; };
+
+template <int CAP>
+__global__ void __launch_bounds__(THREADS) group_table_kernel(const __grid_constant__ GroupTable<CAP> table, int n, RowTile* tiles, int* slots,
+                                                              uint4* zero, long long zero_vecs) {
+  const int b = (int)blockIdx.x, tid = (int)threadIdx.x;
+  if (b >= n) {                              // the other blocks clear the flags and the status word
+    for (long long i = (long long)(b - n) * THREADS + tid; i < zero_vecs; i += (long long)(gridDim.x - n) * THREADS) zero[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const GroupEntry e = table.e[b];
+  if (tid == 0) slots[e.slot] = e.g;
+  const int end = e.row0 + e.rows, count = (e.rows + e.tile_rows - 1) / e.tile_rows;
+  for (int t = tid; t < count; t += THREADS) {
+    const int m0 = e.row0 + t * e.tile_rows;
+    tiles[e.first_tile + t] = RowTile{m0, min(end, m0 + e.tile_rows), e.g, e.slot};
+  }
+}
+
+struct GroupedPlan {
+  int few = 0;                               // rows up to which a group takes 16-row tiles
+  long long n16 = 0, n128 = 0;               // row tiles
+  int slots = 0, slots128 = 0;               // groups; those on 128-row tiles, numbered first
+  int tiles_n = 0, k_tiles = 0, slices = 1, chains = 1;
+  bool wide = false;
+  size_t flag_a = 0, flag_b = 0, tiles = 0, slot_list = 0, a = 0, b = 0, seq = 0, chain_results = 0, total = 0;   // total 0: not served
+};
+
+GroupedPlan grouped_plan(const Params& p, int nfma, const int* rows, const unsigned char* use, int E) {
+  GroupedPlan best;
+  if (!umma_supports(p) || (nfma != 16 && nfma != 32) || p.K <= 0 || p.N <= 0) return best;
+  const KernelTimes kt(p, nfma);
+  const long long sms = sm_count();
+  const int k_tiles = (p.K + KT - 1) / KT, tiles_n = (p.N + BN - 1) / BN;
+  const int chains = p.fast ? 1 : (k_tiles + 3) / 4;
+  double least = 0.0;
+  const int choices[] = {16, 32, 64, 0x7FFFFFFF};
+  for (int few : choices) {
+    if (few > 16 && env_off("MMAEMU_B200_ROW_GROUPS")) break;
+    GroupedPlan g;
+    g.few = few;
+    g.tiles_n = tiles_n;
+    g.k_tiles = k_tiles;
+    g.chains = chains;
+    for (int e = 0; e < E; ++e) {
+      if (rows[e] <= 0 || (use && !use[e])) continue;
+      g.slots += 1;
+      if (rows[e] > few) {
+        g.n128 += ((long long)rows[e] + 127) / 128;
+        g.slots128 += 1;
+      } else {
+        g.n16 += ((long long)rows[e] + 15) / 16;
+      }
+    }
+    if (g.slots == 0 || g.n128 > 65535 || tiles_n > 65535 || (g.n128 + g.n16) * tiles_n > 0x7FFFFFFFLL) continue;
+    double time = 0.0;
+    if (g.n128) {
+      const long long tiles = g.n128 * tiles_n, wide = g.n128 * ((tiles_n + 1) / 2);
+      const double narrow_waves = (double)((tiles + sms - 1) / sms), wide_waves = (double)((wide + sms - 1) / sms) * KernelTimes::wide_wave(p.fast != 0);
+      g.wide = kt.one_sum && wide_waves < narrow_waves;
+      // the decode passes read 4 KB and write 16 KB per 128 rows and k-tile, at about 5 TB/s
+      time += (g.wide ? wide_waves : narrow_waves) * kt.umma * k_tiles + kt.predecode + (double)(g.n128 + (long long)g.slots128 * tiles_n) * k_tiles * 20480.0 / 5e6;
+    }
+    if (g.n16) {
+      const long long ctas = g.n16 * tiles_n;
+      double t16 = kt.waves16(ctas, sms) * k_tiles;
+      long long s = env_off("MMAEMU_B200_SLICES") ? 1 : SLICE_CTA_TARGET / ctas;
+      s = s > MMB200_MAX_SLICES ? MMB200_MAX_SLICES : s;
+      s = s > chains ? chains : s;
+      if (s > 1 && (size_t)ctas * chains * 2 * TN * THREADS * sizeof(float) <= SLICE_SCRATCH_LIMIT) {
+        const double ts = kt.waves16(ctas * s, sms) * k_tiles / (double)s + kt.slice_launch;
+        if (ts < t16) {
+          t16 = ts;
+          g.slices = (int)s;
+        }
+      }
+      time += t16;
+    }
+    if (best.slots && time >= least) continue;
+    least = time;
+    best = g;
+  }
+  if (best.slots == 0) return best;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  GroupedPlan& g = best;
+  g.flag_a = 256;                            // the status word comes first
+  g.flag_b = g.flag_a + up(((size_t)p.M + BM) * sizeof(int));
+  g.tiles = g.flag_b + up((size_t)g.slots * tiles_n * BN * sizeof(int));
+  g.slot_list = g.tiles + up((size_t)(g.n16 + g.n128) * sizeof(RowTile));
+  g.a = g.slot_list + up((size_t)g.slots * sizeof(int));
+  g.b = g.a + (size_t)g.n128 * k_tiles * TC_TILE;
+  g.seq = g.b + (size_t)g.slots128 * tiles_n * k_tiles * TC_TILE;
+  g.chain_results = g.seq + (g.slices > 1 ? up(2 * ((size_t)k_tiles + 8) * sizeof(uint32_t)) : 0);
+  g.total = g.chain_results + (g.slices > 1 ? (size_t)g.n16 * tiles_n * chains * 2 * TN * THREADS * sizeof(float) : 0);
+  return best;
+}
+
+}  // namespace
+
+size_t grouped_workspace_bytes(const Params& p, int nfma, const int* rows, const unsigned char* use, int E) {
+  return grouped_plan(p, nfma, rows, use, E).total;
+}
+
+cudaError_t launch_grouped(const Params& p_in, int nfma, const int* rows, const unsigned char* use, int E, void* workspace,
+                           size_t workspace_bytes, cudaStream_t stream, int* launches) {
+  Params p = p_in;
+  const GroupedPlan g = grouped_plan(p, nfma, rows, use, E);
+  if (!g.total || !workspace || workspace_bytes < g.total || (reinterpret_cast<uintptr_t>(workspace) & 127)) return cudaErrorInvalidValue;
+  unsigned char* base = static_cast<unsigned char*>(workspace);
+  p.status = reinterpret_cast<int*>(base);
+  p.ws_flag_a = reinterpret_cast<int*>(base + g.flag_a);
+  p.ws_flag_b = reinterpret_cast<int*>(base + g.flag_b);
+  p.ws_slots = reinterpret_cast<const int*>(base + g.slot_list);
+  p.ws_a = base + g.a;
+  p.ws_b = base + g.b;
+  p.tiles_n = g.tiles_n;
+  p.k_tiles = g.k_tiles;
+  p.byte_loads = vector_loads(p) && !(p.group_stride_b & 15) ? 0 : 1;
+  p.S = 1;
+  p.scheme = MMB200_SCHEME_NONE;
+  p.row_groups = 1;
+  staged_wait_limits(&p.wait_polls, &p.test_announce_extra);
+  const Plan plan = make_plan(p.K, p.fast, 1, MMB200_SCHEME_NONE);
+  p.plan_group = plan.group;
+  RowTile* tiles = reinterpret_cast<RowTile*>(base + g.tiles);
+  cudaError_t err;
+  // the lists, and the clearing of the flags: a launch per 512 groups, one block each
+  {
+    constexpr int CAP = 512, SMALL = 32;
+    GroupTable<CAP> table;
+    int n = 0, slot128 = 0, slot16 = g.slots128;
+    long long row0 = 0, t128 = 0, t16 = g.n128, zero_vecs = (long long)(g.tiles / 16);
+    auto flush = [&]() -> cudaError_t {
+      const long long blocks = (zero_vecs + THREADS * 4 - 1) / (THREADS * 4), most = 4 * sm_count();
+      const unsigned grid = (unsigned)(n + (blocks < most ? blocks : most));
+      int* slots = const_cast<int*>(p.ws_slots);
+      uint4* zero = reinterpret_cast<uint4*>(base);
+      if (n <= SMALL) {
+        GroupTable<SMALL> small;
+        std::memcpy(&small, &table, sizeof(GroupEntry) * n);
+        group_table_kernel<SMALL><<<grid, THREADS, 0, stream>>>(small, n, tiles, slots, zero, zero_vecs);
+      } else {
+        group_table_kernel<CAP><<<grid, THREADS, 0, stream>>>(table, n, tiles, slots, zero, zero_vecs);
+      }
+      const cudaError_t e = cudaGetLastError();
+      if (e == cudaSuccess) *launches += 1;
+      n = 0;
+      zero_vecs = 0;
+      return e;
+    };
+    for (int e = 0; e < E; ++e) {
+      if (rows[e] > 0 && (!use || use[e])) {
+        const bool tall = rows[e] > g.few;
+        table.e[n++] = GroupEntry{e, (int)row0, rows[e], tall ? slot128++ : slot16++, (int)(tall ? t128 : t16), tall ? 128 : 16};
+        if (tall) t128 += ((long long)rows[e] + 127) / 128;
+        else t16 += ((long long)rows[e] + 15) / 16;
+        if (n == CAP && (err = flush()) != cudaSuccess) return err;
+      }
+      row0 += rows[e];
+    }
+    if (n && (err = flush()) != cudaSuccess) return err;
+  }
+  if (g.n128) {
+    Params q = p;
+    q.ws_tiles = tiles;
+    q.tiles_m = (int)g.n128;
+    q.slots = g.slots128;
+    q.slices = 1;
+    q.umma = 1;
+    q.wide_tiles = g.wide ? 1 : 0;
+    if ((err = launch_umma_grouped(q, nfma, stream, launches)) != cudaSuccess) return err;
+  }
+  if (g.n16) {
+    p.ws_tiles = tiles + g.n128;
+    p.tiles_m = (int)g.n16;
+    p.slots = g.slots;
+    p.few_rows = 1;
+    p.slices = g.slices;
+    if (g.slices > 1) {
+      std::vector<uint32_t> seq((size_t)plan_sequence(plan, p.K, nullptr));
+      plan_sequence(plan, p.K, seq.data());
+      p.seq_len = (int)seq.size();
+      p.n_chains = plan_chains(seq.data(), p.seq_len, plan.group);
+      if (p.n_chains != g.chains || 2 * (size_t)p.seq_len * sizeof(uint32_t) > g.chain_results - g.seq) return cudaErrorInvalidValue;
+      plan_slices(seq.data(), p.seq_len, plan.group, p.n_chains, p.slices, p.slice_start, p.chain_base);
+      for (uint32_t entry : seq) p.n_events += (seq_emits(entry, plan.group ? 1 : 0) || (entry & SEQ_SPLIT_END)) ? 1 : 0;
+      p.ws_seq = reinterpret_cast<const uint32_t*>(base + g.seq);
+      p.ws_events = p.ws_seq + p.seq_len;
+      p.ws_chains = reinterpret_cast<float*>(base + g.chain_results);
+      plan_sequence_kernel<<<1, THREADS, 0, stream>>>(plan, p.K, reinterpret_cast<uint32_t*>(base + g.seq), const_cast<uint32_t*>(p.ws_events));
+      if ((err = cudaGetLastError()) != cudaSuccess) return err;
+      *launches += 1;
+    }
+    if ((err = dispatch_formats(p, nfma, stream, true, launches)) != cudaSuccess) return err;
+  }
+  return cudaSuccess;
 }
 #endif  // part 0
 

@@ -116,13 +116,17 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ float chain_result4(float acc) { return __fmul_rn(fm::chain_cut(acc), 0.25f); }
 
 // One CTA per (k-tile, 128-row block) of one operand: writes the operand image and ORs the non-finite classes of the rows.
-template <int FA, int FB, bool IS_A>
+// GROUPED: blockIdx.y is a row tile of the list for A; for B blockIdx.z is the number of the decoded operand.
+template <int FA, int FB, bool IS_A, bool GROUPED>
 __global__ void __launch_bounds__(THREADS) predecode_umma_kernel(const __grid_constant__ Params p) {
-  const int tid = threadIdx.x, kt = blockIdx.x, rb = blockIdx.y, rows = IS_A ? p.M : p.N;
-  UmmaTile& tile = reinterpret_cast<UmmaTile*>(IS_A ? p.ws_a : p.ws_b)[(long long)rb * p.k_tiles + kt];
-  int* flags = IS_A ? p.ws_flag_a : p.ws_flag_b;
-  const int lrow = tid % 128, lhalf = tid / 128, row = rb * 128 + lrow;
-  const uint4 raw = load_codes16<IS_A>(p, row, rows, kt * KT + 16 * lhalf);
+  const int tid = threadIdx.x, kt = blockIdx.x, rb = blockIdx.y;
+  RowTile rt = row_tile<GROUPED && IS_A, 128>(p, rb);
+  if (!IS_A) rt = RowTile{rb * 128, p.N, GROUPED ? __ldg(p.ws_slots + blockIdx.z) : 0, GROUPED ? (int)blockIdx.z : 0};
+  const int rows = rt.m_end;
+  UmmaTile& tile = reinterpret_cast<UmmaTile*>(IS_A ? p.ws_a : p.ws_b)[((GROUPED && !IS_A ? (long long)rt.slot * p.tiles_n : 0ll) + rb) * p.k_tiles + kt];
+  int* flags = IS_A ? p.ws_flag_a : const_cast<int*>(flags_b<GROUPED>(p, rt));
+  const int lrow = tid % 128, lhalf = tid / 128, row = rt.m0 + lrow;
+  const uint4 raw = load_codes16<IS_A>(p, IS_A ? p.A : operand_b<GROUPED>(p, rt), row, rows, kt * KT + 16 * lhalf);
   uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w}, seen = 0, v[4][2], e[4][2];
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -139,7 +143,7 @@ __global__ void __launch_bounds__(THREADS) predecode_umma_kernel(const __grid_co
   if (seen) atomicOr(&flags[row], (int)seen);
 }
 
-template <int NFMA, int FA, int FB, bool SLOW, int NW, bool SLICED>
+template <int NFMA, int FA, int FB, bool SLOW, int NW, bool SLICED, bool GROUPED>
 __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_constant__ Params p) {
   constexpr bool PARTS = SLOW && !SLICED && NW == 128; // running sums in shared memory
   using Smem = SmemUmma<NW, PARTS>;
@@ -158,7 +162,8 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_cons
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   int tile_m, tile_n;                                  // tile_n in units of 2 NW columns
   tile_of_cta(p.tiles_m, (p.N + 2 * NW - 1) / (2 * NW), BAND * 64 / NW, (int)blockIdx.x, tile_m, tile_n);
-  const int m0 = tile_m * BM, n0 = tile_n * 2 * NW;
+  const RowTile rt = row_tile<GROUPED, BM>(p, tile_m);
+  const int m0 = rt.m0, n0 = tile_n * 2 * NW;
   // k-tiles in order, or this K slice's part of the plan's sequence
   const int t0 = SLICED ? p.slice_start[blockIdx.y] : 0;
   const int T = SLICED ? p.slice_start[blockIdx.y + 1] - t0 : p.k_tiles, NB = T * BPT;
@@ -185,7 +190,8 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_cons
     if (lane == 0) {
       const UmmaTile* ga = reinterpret_cast<const UmmaTile*>(p.ws_a) + (long long)tile_m * p.k_tiles;
       const int nb = (NW == 128 && n0 + 128 < p.N) ? 2 : 1;                           // 128-column images of B
-      const UmmaTile* gb = reinterpret_cast<const UmmaTile*>(p.ws_b) + (long long)tile_n * (NW / 64) * p.k_tiles;
+      const UmmaTile* gb = reinterpret_cast<const UmmaTile*>(p.ws_b) +
+                           ((GROUPED ? (long long)rt.slot * p.tiles_n : 0ll) + (long long)tile_n * (NW / 64)) * p.k_tiles;
       int issued = 0;
       for (int t = 0; t < T; ++t) {
         const int s = t % RING, kt = SLICED ? (int)(__ldg(p.ws_seq + t0 + t) & SEQ_TILE_MASK) : t;
@@ -262,7 +268,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_cons
     __syncwarp();
   } else if (h < H) {
     // ---- the scalar steps: block start of block b, from R of block b - 1
-    const bool rows = m0 + 32 * (warp % 4) < p.M;      // a warp without rows of the problem only keeps the barriers
+    const bool rows = m0 + 32 * (warp % 4) < rt.m_end; // a warp without rows of the problem only keeps the barriers
     uint32_t zero[CHUNK];
 #pragma unroll
     for (int q = 0; q < CHUNK; ++q) zero[q] = R_ZERO;
@@ -347,9 +353,11 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_cons
   const bool bad = __syncthreads_or(ok ? 0 : 1) != 0;
   if (!SLICED && !bad && warp < EPI_WARPS) {           // a K slice has stored its chains; the combine kernel writes the output
     Epilogue epi;
-    epi.init(p);
+    init_epilogue<GROUPED>(epi, p, rt);
     const int lr = 32 * (warp % 4) + lane, gm = m0 + lr;
-    const int row_flag = p.patch_nonfinite && gm < p.M ? p.ws_flag_a[gm] : 0;
+    const int row_flag = p.patch_nonfinite && gm < rt.m_end ? p.ws_flag_a[gm] : 0;
+    const int* column_flags = flags_b<GROUPED>(p, rt);
+    const uint8_t* B = operand_b<GROUPED>(p, rt);
     // an image of 128 x 128 outputs for both halves (NW = 64) or for one after the other; rows of it are written out by all
     // the warps. Elements beyond M or N are parked too and not written out.
 #pragma unroll 1
@@ -373,14 +381,14 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_cons
             for (int q = 0; q < CHUNK; ++q) v[q] = SLOW ? __uint_as_float(r[q]) : chain_result4(fm::mma_end(__uint_as_float(r[q])));
           }
           // non-finite classes: one look for the warp's rows and these columns, then element by element where one is set
-          const int col = gn + lane % CHUNK, col_flag = p.patch_nonfinite && col < p.N ? p.ws_flag_b[col] : 0;
+          const int col = gn + lane % CHUNK, col_flag = p.patch_nonfinite && col < p.N ? column_flags[col] : 0;
           if (__any_sync(0xFFFFFFFFu, row_flag | col_flag)) {
 #pragma unroll
             for (int q = 0; q < CHUNK; ++q) {
               const int flag = row_flag | __shfl_sync(0xFFFFFFFFu, col_flag, q);
               uint32_t bits;
-              if (flag && gm < p.M && gn + q < p.N &&
-                  nonfinite_patch(flag, p.A + (long long)gm * p.lda, p.B + (long long)(gn + q) * p.ldb, p.K, p.fmt_a, p.fmt_b, bits))
+              if (flag && gm < rt.m_end && gn + q < p.N &&
+                  nonfinite_patch(flag, p.A + (long long)gm * p.lda, B + (long long)(gn + q) * p.ldb, p.K, p.fmt_a, p.fmt_b, bits))
                 v[q] = __uint_as_float(bits);
             }
           }
@@ -388,7 +396,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_cons
         }
       }
       asm volatile("bar.sync 1, %0;" ::"n"(EPI_THREADS) : "memory");
-      epi.flush(p, smem_raw, m0, nc, tid, EPI_THREADS);
+      epi.flush(p, smem_raw, m0, nc, tid, EPI_THREADS, Epilogue::TILE_DIM, rt.m_end);
       if (NW == 128) asm volatile("bar.sync 1, %0;" ::"n"(EPI_THREADS) : "memory");
     }
   }
@@ -400,17 +408,18 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_cons
   }
 }
 
-template <int FA, int FB, bool IS_A>
+template <int FA, int FB, bool IS_A, bool GROUPED>
 cudaError_t launch_predecode(const Params& p, cudaStream_t stream, int* launches) {
-  predecode_umma_kernel<FA, FB, IS_A><<<dim3((unsigned)p.k_tiles, (unsigned)(IS_A ? p.tiles_m : p.tiles_n)), THREADS, 0, stream>>>(p);
+  const dim3 grid((unsigned)p.k_tiles, (unsigned)(IS_A ? p.tiles_m : p.tiles_n), GROUPED && !IS_A ? (unsigned)p.slots : 1u);
+  predecode_umma_kernel<FA, FB, IS_A, GROUPED><<<grid, THREADS, 0, stream>>>(p);
   const cudaError_t err = cudaGetLastError();
   if (err == cudaSuccess) *launches += 1;
   return err;
 }
 
-template <int NFMA, int FA, int FB, bool SLOW, int NW, bool SLICED>
+template <int NFMA, int FA, int FB, bool SLOW, int NW, bool SLICED, bool GROUPED>
 cudaError_t launch_kernel(const Params& p, cudaStream_t stream, int* launches) {
-  auto kern = umma_kernel<NFMA, FA, FB, SLOW, NW, SLICED>;
+  auto kern = umma_kernel<NFMA, FA, FB, SLOW, NW, SLICED, GROUPED>;
   constexpr size_t SMEM = sizeof(SmemUmma<NW, SLOW && !SLICED && NW == 128>);
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
@@ -422,40 +431,53 @@ cudaError_t launch_kernel(const Params& p, cudaStream_t stream, int* launches) {
   return err;
 }
 
-template <int NFMA, int FA, int FB>
+template <int NFMA, int FA, int FB, bool GROUPED>
 cudaError_t launch_main(const Params& p, cudaStream_t stream, int* launches) {
-  if (p.slices > 1)
-    return p.plan_group ? launch_kernel<NFMA, FA, FB, true, 64, true>(p, stream, launches)
-                        : launch_kernel<NFMA, FA, FB, false, 64, true>(p, stream, launches);
+  if constexpr (!GROUPED) {
+    if (p.slices > 1)
+      return p.plan_group ? launch_kernel<NFMA, FA, FB, true, 64, true, false>(p, stream, launches)
+                          : launch_kernel<NFMA, FA, FB, false, 64, true, false>(p, stream, launches);
+  }
   if constexpr (tc_pow_mul(FA, FB) == 8 || NFMA == 16) {
     if (p.wide_tiles)
-      return p.fast ? launch_kernel<NFMA, FA, FB, false, 128, false>(p, stream, launches)
-                    : launch_kernel<NFMA, FA, FB, true, 128, false>(p, stream, launches);
+      return p.fast ? launch_kernel<NFMA, FA, FB, false, 128, false, GROUPED>(p, stream, launches)
+                    : launch_kernel<NFMA, FA, FB, true, 128, false, GROUPED>(p, stream, launches);
   }
-  return p.fast ? launch_kernel<NFMA, FA, FB, false, 64, false>(p, stream, launches)
-                : launch_kernel<NFMA, FA, FB, true, 64, false>(p, stream, launches);
+  return p.fast ? launch_kernel<NFMA, FA, FB, false, 64, false, GROUPED>(p, stream, launches)
+                : launch_kernel<NFMA, FA, FB, true, 64, false, GROUPED>(p, stream, launches);
 }
 
-template <int FA, int FB>
+template <int FA, int FB, bool GROUPED>
 cudaError_t launch(const Params& p, int nfma, cudaStream_t stream, int* launches) {
   cudaError_t err;
-  if (!p.only_b && (err = launch_predecode<FA, FB, true>(p, stream, launches)) != cudaSuccess) return err;
+  if (!p.only_b && (err = launch_predecode<FA, FB, true, GROUPED>(p, stream, launches)) != cudaSuccess) return err;
   if (p.only_b || !p.shared_b) {
-    if ((err = launch_predecode<FA, FB, false>(p, stream, launches)) != cudaSuccess) return err;
+    if ((err = launch_predecode<FA, FB, false, GROUPED>(p, stream, launches)) != cudaSuccess) return err;
   }
   if (p.only_b) return cudaSuccess;
-  return nfma == 16 ? launch_main<16, FA, FB>(p, stream, launches) : launch_main<32, FA, FB>(p, stream, launches);
+  return nfma == 16 ? launch_main<16, FA, FB, GROUPED>(p, stream, launches) : launch_main<32, FA, FB, GROUPED>(p, stream, launches);
+}
+
+template <bool GROUPED>
+cudaError_t launch_pair(const Params& p, int nfma, cudaStream_t stream, int* launches) {
+  switch (p.fmt_a * 2 + p.fmt_b) {
+    case 0: return launch<MMB200_FMT_E4M3, MMB200_FMT_E4M3, GROUPED>(p, nfma, stream, launches);
+    case 1: return launch<MMB200_FMT_E4M3, MMB200_FMT_E5M2, GROUPED>(p, nfma, stream, launches);
+    case 2: return launch<MMB200_FMT_E5M2, MMB200_FMT_E4M3, GROUPED>(p, nfma, stream, launches);
+    default: return cudaErrorInvalidValue;             // E5M2 x E5M2: umma_supports says no
+  }
 }
 
 }  // namespace
 
-cudaError_t launch_umma(const Params& p, int nfma, cudaStream_t stream, int* launches) {
-  switch (p.fmt_a * 2 + p.fmt_b) {
-    case 0: return launch<MMB200_FMT_E4M3, MMB200_FMT_E4M3>(p, nfma, stream, launches);
-    case 1: return launch<MMB200_FMT_E4M3, MMB200_FMT_E5M2>(p, nfma, stream, launches);
-    case 2: return launch<MMB200_FMT_E5M2, MMB200_FMT_E4M3>(p, nfma, stream, launches);
-    default: return cudaErrorInvalidValue;             // E5M2 x E5M2: umma_supports says no
-  }
+// Two translation units, compiled in parallel (MMB_GROUPED; undefined: everything in one).
+#if !defined(MMB_GROUPED) || MMB_GROUPED == 0
+cudaError_t launch_umma(const Params& p, int nfma, cudaStream_t stream, int* launches) { return launch_pair<false>(p, nfma, stream, launches); }
+#endif
+#if !defined(MMB_GROUPED) || MMB_GROUPED == 1
+cudaError_t launch_umma_grouped(const Params& p, int nfma, cudaStream_t stream, int* launches) {
+  return launch_pair<true>(p, nfma, stream, launches);
 }
+#endif
 
 }  // namespace mmb

@@ -32,15 +32,40 @@ __device__ __forceinline__ void tile_of_cta(const Params& p, int idx, int& tile_
   tile_of_cta(p.tiles_m, p.tiles_n, BAND, idx, tile_m, tile_n);
 }
 
+// The row tile of a CTA of ROWS-row tiles: every ROWS rows, or from the list of a grouped launch.
+template <bool GROUPED, int ROWS>
+__device__ __forceinline__ RowTile row_tile(const Params& p, int tile_m) {
+  if constexpr (GROUPED) {
+    const int4 v = __ldg(reinterpret_cast<const int4*>(p.ws_tiles + tile_m));
+    return RowTile{v.x, v.y, v.z, v.w};
+  } else {
+    return RowTile{tile_m * ROWS, p.M, 0, 0};
+  }
+}
+template <bool GROUPED>
+__device__ __forceinline__ const uint8_t* operand_b(const Params& p, const RowTile& rt) {
+  return GROUPED ? p.B + (long long)rt.g * p.group_stride_b : p.B;
+}
+template <bool GROUPED>
+__device__ __forceinline__ const int* flags_b(const Params& p, const RowTile& rt) {
+  return GROUPED ? p.ws_flag_b + (long long)rt.slot * p.tiles_n * BN : p.ws_flag_b;
+}
+template <bool GROUPED>
+__device__ __forceinline__ void init_epilogue(Epilogue& epi, const Params& p, const RowTile& rt) {
+  if constexpr (GROUPED) epi.init(p, p.scale_a + (long long)rt.g * p.sa_stride, p.scale_b + (long long)rt.g * p.sb_stride);
+  else epi.init(p);
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // Quantise prologue (the scalar conversion is fm::quantise_e4m3 in fast_math.cuh).
 // The 16 codes of row `row` starting at element k of one operand: the caller's FP8 codes, or -- operand A with the
-// quantise prologue -- the codes of 16 activations, which are also written to the codes array.
+// quantise prologue -- the codes of 16 activations, which are also written to the codes array. `operand`: p.A, p.B or the
+// group's B.
 template <bool IS_A>
-__device__ __forceinline__ uint4 load_codes16(const Params& p, int row, int rows, int k) {
+__device__ __forceinline__ uint4 load_codes16(const Params& p, const uint8_t* operand, int row, int rows, int k) {
   if (row >= rows || k >= p.K) return make_uint4(0, 0, 0, 0);
   if (!IS_A || !p.a_hp) {
-    const uint8_t* src = (IS_A ? p.A : p.B) + (long long)row * (IS_A ? p.lda : p.ldb) + k;
+    const uint8_t* src = operand + (long long)row * (IS_A ? p.lda : p.ldb) + k;
     if (!p.byte_loads) return __ldg(reinterpret_cast<const uint4*>(src));
     // K or a leading dimension that is no multiple of 16, or an operand that is not 16-byte aligned: byte by byte
     uint32_t w[4] = {0u, 0u, 0u, 0u};

@@ -116,7 +116,8 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
     with _on_device(dev):
         ws, ws_ptr, n = None, None, 0
         if kernel not in ("integer", "direct") and not preset.late_c and os.environ.get("MMAEMU_B200_WORKSPACE", "1") != "0":
-            n = int(L.mmb200_grouped_workspace_bytes(rows, splits, E, N, K))
+            n = int(L.mmb200_grouped_workspace_bytes(rows, splits, E, N, K, _lib.FMT_CODES[fa], _lib.FMT_CODES[fb], preset.code,
+                                                     int(fast)))
             if n:
                 try:
                     ws = torch.empty(n, dtype=torch.uint8, device=dev)

@@ -192,5 +192,10 @@ def test_argument_checks_of_the_emulated_grouped_entry_point(lib):
     assert call(m=(2 ** 31 - 1, 1)) == _lib.ERR_TOO_LARGE and call(m=(1,), E=4097) == _lib.ERR_TOO_LARGE
     assert call(m=(0, 0)) == _lib.OK
     m = (ctypes.c_int * 2)(100, 300)
-    assert lib.mmb200_grouped_workspace_bytes(m, None, 2, 64, 64) >= lib.mmb200_workspace_bytes(300, 64, 64)
-    assert lib.mmb200_grouped_workspace_bytes((ctypes.c_int * 2)(0, 0), None, 2, 64, 64) == 0
+    need = lib.mmb200_grouped_workspace_bytes
+    assert need((ctypes.c_int * 2)(0, 300), None, 2, 64, 64, 0, 0, 32, 0) >= lib.mmb200_workspace_bytes(300, 64, 64)
+    assert need(m, None, 2, 64, 64, 0, 0, 32, 0) > 0
+    assert need((ctypes.c_int * 2)(0, 0), None, 2, 64, 64, 0, 0, 32, 0) == 0
+    # the decoded operands of all groups would take 16 GB: group by group
+    most = (ctypes.c_int * 64)(*[100] * 64)
+    assert need(most, None, 64, 8192, 8192, 0, 0, 32, 1) < 1 << 30
