@@ -52,14 +52,17 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
     nvcc = nvcc_path()
     # a unit is compiled again when its object is older than its source, a shared header or this file
-    shared = [*CSRC.glob("*.cuh"), *CSRC.glob("*.h"), PKG.parent / "include" / "mmaemu_b200.h", Path(__file__)]
+    shared = [*CSRC.glob("*.cuh"), PKG.parent / "include" / "mmaemu_b200.h", Path(__file__)]
     newest_shared = max(d.stat().st_mtime for d in shared)
+
+    def newest(src: Path) -> float:                      # and the private headers (*.h) that the source names
+        text = src.read_text()
+        return max(newest_shared, src.stat().st_mtime, *(h.stat().st_mtime for h in CSRC.glob("*.h") if f'"{h.name}"' in text))
     jobs = []
     for i, (src, defines) in enumerate(UNITS):
         obj = OBJ / f"{Path(src).stem}_{i}.o"
         cmd = [nvcc, *NVCC_FLAGS, *defines, *(["-Xptxas", "-v"] if verbose else []), "-c", str(CSRC / src), "-o", str(obj)]
-        fresh = (not force and not verbose and obj.exists()
-                 and obj.stat().st_mtime > max(newest_shared, (CSRC / src).stat().st_mtime))
+        fresh = not force and not verbose and obj.exists() and obj.stat().st_mtime > newest(CSRC / src)
         proc = None if fresh else subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, env=env)
         jobs.append((cmd, obj, proc))
     failed = None

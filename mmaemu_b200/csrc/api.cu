@@ -709,7 +709,7 @@ int mmb200_int8_scaled_mm(const int8_t* A, int64_t lda, const int8_t* W, int64_t
                           int out_dtype, int T, int N, int K, int E, const int* offs, const float* scale_a, int sa_stride,
                           const float* scale_b, int64_t sb_group_stride, int sb_stride, const void* bias, int bias_dtype,
                           int64_t bias_group_stride, int zero_rest, void* workspace, size_t workspace_bytes, void* stream) {
-  if (T < 0 || N < 0 || K < 0 || E < 0 || (!offs && E != 1)) return MMB200_ERR_BAD_ARG;
+  if (T < 0 || N < 0 || K < 0 || E < 1 || (!offs && E != 1)) return MMB200_ERR_BAD_ARG;
   if (out_dtype < MMB200_OUT_F32 || out_dtype > MMB200_OUT_F16) return MMB200_ERR_BAD_ARG;
   if (bias && (bias_dtype < MMB200_HP_F32 || bias_dtype > MMB200_HP_F16)) return MMB200_ERR_BAD_ARG;
   if (!scale_a || !scale_b || sa_stride < 0 || sb_stride < 0 || sb_group_stride < 0 || bias_group_stride < 0 || group_stride_w < 0)
@@ -717,7 +717,7 @@ int mmb200_int8_scaled_mm(const int8_t* A, int64_t lda, const int8_t* W, int64_t
   if (K > MMB200_INT8_MAX_K || T > MMB200_INT8_MAX_ROWS || E > MMB200_MAX_GROUPS) return MMB200_ERR_TOO_LARGE;
   if (T == 0 || N == 0) return MMB200_OK;
   if (!D || (T > 1 && ldd < N)) return MMB200_ERR_BAD_ARG;
-  if (K > 0 && E > 0 && (!A || !W || (T > 1 && lda < K) || (N > 1 && ldw < K))) return MMB200_ERR_BAD_ARG;
+  if (K > 0 && (!A || !W || (T > 1 && lda < K) || (N > 1 && ldw < K))) return MMB200_ERR_BAD_ARG;
   const uintptr_t es = out_dtype == MMB200_OUT_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(D) % es) return MMB200_ERR_BAD_ARG;
   const int rc = current_device_ok();
@@ -731,7 +731,7 @@ int mmb200_int8_scaled_mm(const int8_t* A, int64_t lda, const int8_t* W, int64_t
   p.sa_stride = sa_stride; p.sb_stride = sb_stride;
   p.bias_dtype = bias_dtype; p.out_dtype = out_dtype;
   p.zero_rest = zero_rest;
-  const size_t need = E > 0 ? mmb::int8_workspace_bytes(p) : 0;
+  const size_t need = mmb::int8_workspace_bytes(p);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) return MMB200_ERR_BAD_ARG;
   int launches = 0;
   const cudaError_t err = mmb::launch_int8(p, workspace, static_cast<cudaStream_t>(stream), &launches);

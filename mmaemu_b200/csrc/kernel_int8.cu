@@ -134,13 +134,14 @@ __device__ __forceinline__ void write_rows(const Int8Params& p, uint32_t acc, bo
 }
 
 // ---- groups. Ends are taken as a running maximum, clamped to [0, T], so that no content of offs leads out of the operands.
-struct Group { int g, start, end, tile; };       // g < 0: no such tile
+struct Group { int g, start, end, tile, last; };       // g < 0: no such tile; last: the end of the last group
 // The group of tile `slot` of BT rows, found by one warp (every lane returns it).
 template <int BT>
 __device__ __forceinline__ Group find_group(const Int8Params& p, int slot) {
-  if (!p.offs) return Group{0, 0, p.T, slot};
+  if (!p.offs) return Group{0, 0, p.T, slot, p.T};
   const int lane = threadIdx.x % 32;
   int tiles = 0, last = 0;
+  Group r{-1, 0, 0, 0, 0};
   for (int base = 0; base < p.E; base += 32) {
     int end = base + lane < p.E ? min(max(__ldg(p.offs + base + lane), 0), p.T) : 0;
 #pragma unroll
@@ -159,20 +160,25 @@ __device__ __forceinline__ Group find_group(const Int8Params& p, int slot) {
     }
     upto += tiles;
     const unsigned after = __ballot_sync(0xFFFFFFFFu, upto > slot);
-    if (after) {
+    if (after && r.g < 0) {
       const int l = __ffs(after) - 1;
-      Group r;
       r.g = base + l;
       r.start = __shfl_sync(0xFFFFFFFFu, start, l);
       r.end = __shfl_sync(0xFFFFFFFFu, end, l);
-      const int before = __shfl_sync(0xFFFFFFFFu, upto - (end - start + BT - 1) / BT, l);
-      r.tile = slot - before;
-      return r;
+      r.tile = slot - __shfl_sync(0xFFFFFFFFu, upto - (end - start + BT - 1) / BT, l);
     }
     tiles = __shfl_sync(0xFFFFFFFFu, upto, 31);
     last = __shfl_sync(0xFFFFFFFFu, end, 31);
   }
-  return Group{-1, last, p.T, 0};                 // start: the first row behind the last group
+  r.last = last;
+  return r;
+}
+// Zeros in the rows behind the last group: the channels [n0, n1), rows first, first + step, ... by `threads` threads.
+template <int OUT>
+__device__ __forceinline__ void zero_rows(const Int8Params& p, int first, int step, int n0, int n1, int thread, int threads) {
+  if (!p.zero_rest) return;
+  for (long long row = first; row < p.T; row += step)
+    for (int n = n0 + thread; n < n1; n += threads) static_cast<typename OutType<OUT>::type*>(p.d)[row * p.ldd + n] = 0;
 }
 
 template <int BT>
@@ -214,6 +220,7 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "n"(COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  wait_for_predecessor();
   if (warp == 2) {
     const Group found = find_group<BT>(p, (int)blockIdx.y);
     if (lane == 0) sm.group = found;
@@ -225,6 +232,7 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
   const Group g = sm.group;
   const int row0 = g.start + g.tile * BT;
   const bool work = g.g >= 0 && row0 < g.end;     // the same for every CTA of the cluster
+  if (warp >= 2 && rank == 0) zero_rows<OUT>(p, g.last + (int)blockIdx.y, (int)gridDim.y, n0, min(n0 + CH, p.N), threadIdx.x - 64, 128);
   bool ok = true;
   if (work && nk > 0) {
     if (warp == 0) {
@@ -319,202 +327,266 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
   }
 }
 
-// ---- pairs of CTAs
-constexpr int PAIR_STAGES = 6, PAIR_T = 256;
-constexpr int PAIR_THREADS = 320;        // warp 0: copies, warp 1: MMAs, warps 2 to 9: output (a quarter of the channels, half of the rows)
-constexpr int PAIR_BAND = 8;               // tiles of rows that share a pass over the channels (16 MB of rows at K = 8192 stay in L2)
-struct SmemPair {
-  struct Stage { unsigned char w[CH * KB], a[CH * KB]; } stage[PAIR_STAGES];
-  unsigned long long full[PAIR_STAGES];    // leader: both CTAs' copies of the stage have landed
-  unsigned long long empty[PAIR_STAGES];   // the MMAs that read the stage are done
-  unsigned long long acc_full[2];          // the accumulator is complete
-  unsigned long long acc_empty[2];         // leader: all sixteen output warps have read it
-  unsigned long long drain;
-  uint32_t tmem;
+// ---- persistent workers: one CTA per SM, or a pair of CTAs on neighbouring SMs
+// A worker's tile is CH * CTAS channels x up to BT rows. In a pair each CTA holds its channels and half of the rows.
+template <int CTAS, int BT>
+struct Worker {
+  static constexpr int ROWS = BT / CTAS;                            // rows that a CTA brings
+  static constexpr int STAGES = 196608 / ((CH + ROWS) * KB);        // 192 KB of stages
+  static constexpr int COLS = 2 * BT < 32 ? 32 : 2 * BT;            // two accumulators
+  struct Stage { unsigned char w[CH * KB], a[ROWS * KB]; };
+  struct Smem {
+    Stage stage[STAGES];
+    unsigned long long full[STAGES];       // (of the pair's first CTA) the copies of all CTAs have landed
+    unsigned long long empty[STAGES];      // the MMAs that read the stage are done
+    unsigned long long acc_full[2];        // the accumulator is complete
+    unsigned long long acc_empty[2];       // (first CTA) all output warps have read it
+    unsigned long long drain;
+    uint32_t tmem;
+  };
 };
-__device__ __forceinline__ uint32_t leader_addr(const void* ptr) {
+constexpr int WORKER_THREADS = 320;        // warp 0: copies, warp 1: MMAs, warps 2 to 9: output (a quarter of the channels, half of the rows)
+constexpr int BAND_ROWS = 2048;            // rows that share a pass over the channels (16 MB of them at K = 8192 stay in L2)
+
+template <int CTAS>
+__device__ __forceinline__ uint32_t first_cta(const void* ptr) {
+  if constexpr (CTAS == 1) return smem_addr(ptr);
   uint32_t a;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(ptr)));
   return a;
 }
-__device__ __forceinline__ void tma_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-               ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+template <int CTAS>
+__device__ __forceinline__ void load_rows(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if constexpr (CTAS == 1)
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void tma_3d_pair(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-               ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+template <int CTAS>
+__device__ __forceinline__ void load_channels(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if constexpr (CTAS == 1)
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+template <int CTAS>
+__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  if constexpr (CTAS == 1)
+    mma_i8(d, a, b, idesc, add);
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
-__device__ __forceinline__ void commit_pair(unsigned long long* bar) {       // arrives at the barrier of both CTAs
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-               ::"r"(smem_addr(bar)), "h"((uint16_t)3) : "memory");
-}
-__device__ __forceinline__ void arrive_remote(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+template <int CTAS>
+__device__ __forceinline__ void commit_all(unsigned long long* bar) {        // arrives at the barrier of every CTA of the worker
+  if constexpr (CTAS == 1)
+    commit(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(smem_addr(bar)), "h"((uint16_t)3) : "memory");
 }
 
-// The tiles of a launch in order: group by group, inside a group bands of PAIR_BAND tiles of rows, inside a band channel tile
-// by channel tile. A worker walks an increasing sequence of indices; every role of a CTA has a walker of its own.
+// The tiles of a launch in order: group by group, inside a group bands of BAND_ROWS rows, inside a band channel tile by
+// channel tile. A worker walks an increasing sequence of indices; every role of a CTA has a walker of its own.
+template <int BT>
 struct Walker {
   int g = -1, start = 0, end = 0, tiles_t = 0;
   long long base = 0, count = 0;           // tiles before the group, tiles of the group
   __device__ __forceinline__ bool find(const Int8Params& p, int tiles_n, long long t, int& row0, int& n_tile) {
+    constexpr int BAND = BAND_ROWS / BT;
     while (t >= base + count) {
       base += count;
       if (++g >= p.E) return false;
       start = end;
       end = p.offs ? max(end, min(max(__ldg(p.offs + g), 0), p.T)) : p.T;
-      tiles_t = (end - start + PAIR_T - 1) / PAIR_T;
+      tiles_t = (end - start + BT - 1) / BT;
       count = (long long)tiles_t * tiles_n;
     }
-    const long long i = t - base, per_band = (long long)PAIR_BAND * tiles_n;
-    const int band = (int)(i / per_band), j = (int)(i - band * per_band), width = min(PAIR_BAND, tiles_t - band * PAIR_BAND);
+    const long long i = t - base, per_band = (long long)BAND * tiles_n;
+    const int band = (int)(i / per_band), j = (int)(i - band * per_band), width = min(BAND, tiles_t - band * BAND);
     n_tile = j / width;
-    row0 = start + (band * PAIR_BAND + j % width) * PAIR_T;
+    row0 = start + (band * BAND + j % width) * BT;
     return true;
+  }
+  // Columns of the tile's accumulator: its rows, rounded up to what the MMA takes (16, a pair 32).
+  template <int CTAS>
+  __device__ __forceinline__ int columns(int row0) const {
+    constexpr int STEP = 16 * CTAS;
+    return min(BT, (end - row0 + STEP - 1) / STEP * STEP);
   }
 };
 
-template <int OUT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
-    int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
-                     const __grid_constant__ Int8Params p) {
+template <int CTAS, int BT, int OUT>
+__device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUtensorMap& map_a, const Int8Params& p) {
+  using W = Worker<CTAS, BT>;
+  constexpr int STAGES = W::STAGES;
   extern __shared__ unsigned char smem_raw[];
-  SmemPair& sm = *reinterpret_cast<SmemPair*>(smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u));
+  typename W::Smem& sm = *reinterpret_cast<typename W::Smem*>(smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  int rank;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  const int tiles_n = (p.N + 2 * CH - 1) / (2 * CH), nk = p.k_blocks;
-  const long long first = blockIdx.x / 2, step = gridDim.x / 2;
+  int rank = 0;
+  if (CTAS == 2) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int tiles_n = (p.N + CTAS * CH - 1) / (CTAS * CH), nk = p.k_blocks;
+  const long long first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
   if (threadIdx.x == 0) {
-    for (int q = 0; q < PAIR_STAGES; ++q) { mbar_init(&sm.full[q], 1); mbar_init(&sm.empty[q], 1); }
-    for (int q = 0; q < 2; ++q) { mbar_init(&sm.acc_full[q], 1); mbar_init(&sm.acc_empty[q], 16); }
+    for (int q = 0; q < STAGES; ++q) { mbar_init(&sm.full[q], 1); mbar_init(&sm.empty[q], 1); }
+    for (int q = 0; q < 2; ++q) { mbar_init(&sm.acc_full[q], 1); mbar_init(&sm.acc_empty[q], 8 * CTAS); }
     mbar_init(&sm.drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sm.tmem)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    if constexpr (CTAS == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "n"(W::COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "n"(W::COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
   }
   fence_before();
   __syncthreads();
-  cluster_arrive();                                 // the other CTA's barriers and TMEM are ready too
-  cluster_wait();
+  if constexpr (CTAS == 2) {                        // the other CTA's barriers and TMEM are ready too
+    cluster_arrive();
+    cluster_wait();
+  }
   fence_after();
+  wait_for_predecessor();
   const uint32_t tmem = sm.tmem;
   bool ok = true;
-  Walker walk;
+  Walker<BT> walk;
   int row0, n_tile;
   if (warp == 0) {
     if (lane == 0) {
       unsigned it = 0;
       for (long long t = first; ok && walk.find(p, tiles_n, t, row0, n_tile); t += step) {
+        const int my_row = row0 + (CTAS == 2 ? walk.template columns<CTAS>(row0) / 2 * rank : 0);
         for (int kb = 0; kb < nk; ++kb, ++it) {
-          const unsigned s = it % PAIR_STAGES, round = it / PAIR_STAGES;
+          const unsigned s = it % STAGES, round = it / STAGES;
           if (round && !mbar_wait(&sm.empty[s], (round - 1) & 1, p.wait_polls)) { ok = false; break; }
-          if (rank == 0) mbar_expect_tx(&sm.full[s], 2 * (uint32_t)sizeof(SmemPair::Stage) + (uint32_t)p.announce_extra);
-          const uint32_t bar = leader_addr(&sm.full[s]);
-          tma_3d_pair(sm.stage[s].w, &map_w, kb * KB, (2 * n_tile + rank) * CH, walk.g, bar);
-          tma_2d_pair(sm.stage[s].a, &map_a, kb * KB, row0 + CH * rank, bar);
+          if (rank == 0) mbar_expect_tx(&sm.full[s], CTAS * (uint32_t)sizeof(typename W::Stage) + (uint32_t)p.announce_extra);
+          const uint32_t bar = first_cta<CTAS>(&sm.full[s]);
+          load_channels<CTAS>(sm.stage[s].w, &map_w, kb * KB, (CTAS * n_tile + rank) * CH, walk.g, bar);
+          load_rows<CTAS>(sm.stage[s].a, &map_a, kb * KB, my_row, bar);
         }
       }
-      // no CTA of the pair ends while a copy may be in flight: the leader waits for the last copies into every stage (bounded)
+      // no CTA ends while a copy may be in flight: the worker's first CTA waits for the last copies into every stage (bounded)
       if (rank == 0)
-        for (unsigned q = it > PAIR_STAGES ? it - PAIR_STAGES : 0; q < it; ++q)
-          if (!mbar_wait(&sm.full[q % PAIR_STAGES], (q / PAIR_STAGES) & 1, p.wait_polls)) ok = false;
+        for (unsigned q = it > (unsigned)STAGES ? it - STAGES : 0; q < it; ++q)
+          if (!mbar_wait(&sm.full[q % STAGES], (q / STAGES) & 1, p.wait_polls)) ok = false;
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(PAIR_T >> 3) << 17) | ((uint32_t)(2 * CH >> 4) << 24);
+      constexpr uint32_t SHAPE = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(CTAS * CH >> 4) << 24);
       unsigned it = 0, i = 0;
       for (long long t = first; ok && walk.find(p, tiles_n, t, row0, n_tile); t += step, ++i) {
-        const uint32_t acc = tmem + (i & 1) * PAIR_T;
+        const uint32_t acc = tmem + (i & 1) * BT, idesc = SHAPE | ((uint32_t)(walk.template columns<CTAS>(row0) >> 3) << 17);
         if (i >= 2 && !mbar_wait(&sm.acc_empty[i & 1], ((i >> 1) - 1) & 1, p.wait_polls)) { ok = false; break; }
         fence_after();
         for (int kb = 0; kb < nk; ++kb, ++it) {
-          const unsigned s = it % PAIR_STAGES;
-          if (!mbar_wait(&sm.full[s], (it / PAIR_STAGES) & 1, p.wait_polls)) { ok = false; break; }
+          const unsigned s = it % STAGES;
+          if (!mbar_wait(&sm.full[s], (it / STAGES) & 1, p.wait_polls)) { ok = false; break; }
           fence_after();
           const uint64_t dw = desc_sw128(sm.stage[s].w), da = desc_sw128(sm.stage[s].a);
 #pragma unroll
-          for (int k = 0; k < KB / 32; ++k) mma_i8_pair(acc, dw + 2 * k, da + 2 * k, IDESC, kb > 0 || k > 0 ? 1u : 0u);
-          commit_pair(&sm.empty[s]);
+          for (int k = 0; k < KB / 32; ++k) multiply<CTAS>(acc, dw + 2 * k, da + 2 * k, idesc, kb > 0 || k > 0 ? 1u : 0u);
+          commit_all<CTAS>(&sm.empty[s]);
         }
-        if (ok) commit_pair(&sm.acc_full[i & 1]);
+        if (ok) commit_all<CTAS>(&sm.acc_full[i & 1]);
       }
       // nothing in flight when the TMEM is given back
-      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(&sm.drain)) : "memory");
+      if constexpr (CTAS == 1) commit(&sm.drain);
+      else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(&sm.drain)) : "memory");
       if (!mbar_wait(&sm.drain, 0, WAIT_POLLS)) ok = false;
     }
     __syncwarp();
   } else {
-    const int half = warp < 6 ? 0 : PAIR_T / 2;
+    const int half = warp < 6 ? 0 : BT / 2;
     const uint32_t mine = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + half;
     unsigned i = 0;
     for (long long t = first; walk.find(p, tiles_n, t, row0, n_tile); t += step, ++i) {
-      const int n = (2 * n_tile + rank) * CH + 32 * (warp % 4) + lane, rows = min(walk.end - row0 - half, PAIR_T / 2);
+      const int n = (CTAS * n_tile + rank) * CH + 32 * (warp % 4) + lane, rows = min(walk.end - row0 - half, BT / 2);
       const bool real = n < p.N;
       const float sb = real ? __ldg(p.scale_b + (long long)walk.g * p.sb_group + (long long)n * p.sb_stride) : 0.0f;
       const float bias = real ? bias_at(p, (long long)walk.g * p.bias_group + n) : 0.0f;
-      const float scale = row_scales<32>(p, row0 + half, rows);
+      const float scale = row_scales<(BT < 64 ? BT / 2 : 32)>(p, row0 + half, rows);
       ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.acc_full[i & 1], (i >> 1) & 1, p.wait_polls));
       if (!ok) break;
       fence_after();
-      write_rows<OUT, PAIR_T>(p, mine + (i & 1) * PAIR_T, true, row0 + half, rows, n, real, sb, bias, scale);
+      write_rows<OUT, BT / 2>(p, mine + (i & 1) * BT, true, row0 + half, rows, n, real, sb, bias, scale);
       fence_before();
       __syncwarp();
-      if (lane == 0) arrive_remote(leader_addr(&sm.acc_empty[i & 1]));
+      if (lane == 0) {
+        if constexpr (CTAS == 1) mbar_arrive(&sm.acc_empty[i & 1]);
+        else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(first_cta<CTAS>(&sm.acc_empty[i & 1])) : "memory");
+      }
     }
+    if (ok) zero_rows<OUT>(p, walk.end + (int)blockIdx.x, (int)gridDim.x, 0, p.N, threadIdx.x - 64, WORKER_THREADS - 64);   // (the walk has seen every group)
   }
   if (!ok) atomicExch(p.status, 1);
   fence_before();
   __syncthreads();
-  cluster_arrive();
-  cluster_wait();
+  if constexpr (CTAS == 2) {
+    cluster_arrive();
+    cluster_wait();
+  }
   if (warp == 1) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if constexpr (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(W::COLS));
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(W::COLS));
   }
 }
-
-// Rows behind the last group: zero.
-__global__ void __launch_bounds__(256) zero_rest_kernel(const __grid_constant__ Int8Params p) {
-  __shared__ int first;
-  if (threadIdx.x < 32) {
-    int last = 0;
-    for (int e = threadIdx.x; e < p.E; e += 32) last = max(last, min(max(__ldg(p.offs + e), 0), p.T));
-    last = __reduce_max_sync(0xFFFFFFFFu, last);
-    if (threadIdx.x == 0) first = last;
-  }
-  __syncthreads();
-  const int es = p.out_dtype == MMB200_OUT_F32 ? 4 : 2;
-  for (long long row = (long long)first + blockIdx.x; row < p.T; row += gridDim.x) {
-    unsigned char* d = static_cast<unsigned char*>(p.d) + row * p.ldd * es;
-    for (int n = threadIdx.x; n < p.N; n += 256) {
-      if (es == 4) reinterpret_cast<uint32_t*>(d)[n] = 0;
-      else reinterpret_cast<uint16_t*>(d)[n] = 0;
-    }
-  }
+template <int OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WORKER_THREADS, 1)
+    int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ Int8Params p) {
+  int8_worker<2, 256, OUT>(map_w, map_a, p);
+}
+template <int BT, int OUT>
+__global__ void __launch_bounds__(WORKER_THREADS, 1)
+    int8_single_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ Int8Params p) {
+  int8_worker<1, BT, OUT>(map_w, map_a, p);
 }
 
 // Rows of any alignment -> rows of `pitch` bytes (a multiple of 16) that TMA can read. The bytes behind K are not read.
-__global__ void __launch_bounds__(256) repack_kernel(const int8_t* src, long long ld, long long group_stride, long long rows_per_group,
-                                                     long long rows, int K, int8_t* dst, long long pitch) {
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int8_t* s = src + row / rows_per_group * group_stride + row % rows_per_group * ld;
-    int8_t* d = dst + row * pitch;
-    for (int k = threadIdx.x * 4; k < K; k += 1024) {
-      uint32_t v = 0;
+struct Repack {
+  const int8_t* src;
+  int8_t* dst;
+  long long ld, group_stride, rows_per_group, rows;
+};
+__global__ void __launch_bounds__(256) repack_kernel(const __grid_constant__ Repack r0, const __grid_constant__ Repack r1, int K, long long pitch) {
+  wait_for_predecessor();
+  for (long long i = blockIdx.x; i < r0.rows + r1.rows; i += gridDim.x) {
+    const bool second = i >= r0.rows;
+    const Repack& r = second ? r1 : r0;
+    const long long row = second ? i - r0.rows : i;
+    const int8_t* s = r.src + row / r.rows_per_group * r.group_stride + row % r.rows_per_group * r.ld;
+    int8_t* d = r.dst + row * pitch;
+    // 16 bytes a thread: the five aligned words around them, shifted (the first and last word of a row byte by byte, so that
+    // nothing outside the row is read)
+    const unsigned shift = 8 * (unsigned)(reinterpret_cast<uintptr_t>(s) & 3);
+    for (int k = threadIdx.x * 16; k < K; k += 4096) {
+      uint32_t v[4];
+      if (k >= 4 && k + 20 <= K) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(s + k - (shift >> 3));
+        uint32_t a[5];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (k + q < K) v |= (uint32_t)(uint8_t)__ldg(s + k + q) << (8 * q);
-      *reinterpret_cast<uint32_t*>(d + k) = v;
+        for (int q = 0; q < 5; ++q) a[q] = q < 4 || shift ? __ldg(w + q) : 0u;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = __funnelshift_r(a[q], a[q + 1], shift);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          v[q] = 0;
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if (k + 4 * q + b < K) v[q] |= (uint32_t)(uint8_t)__ldg(s + k + 4 * q + b) << (8 * b);
+        }
+      }
+      *reinterpret_cast<uint4*>(d + k) = make_uint4(v[0], v[1], v[2], v[3]);
     }
   }
 }
@@ -593,30 +665,29 @@ cudaError_t launch_tile(const Int8Params& p, const Maps& m, int parts, unsigned 
   static SmemLimit limit;
   const cudaError_t err = limit.set(reinterpret_cast<const void*>(kern), SMEM);
   if (err != cudaSuccess) return err;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.tiles_n * parts), tiles_t);
-  cfg.blockDim = dim3(TILE_THREADS);
-  cfg.dynamicSmemBytes = SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)parts;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, m.w, m.a, p);
+  return launch_dependent(kern, dim3((unsigned)(p.tiles_n * parts), tiles_t), TILE_THREADS, SMEM, (unsigned)parts, st, m.w, m.a, p);
 }
-template <int OUT>
-cudaError_t launch_pair(const Int8Params& p, const Maps& m, long long tiles, cudaStream_t st) {
-  auto kern = int8_pair_kernel<OUT>;
-  constexpr size_t SMEM = sizeof(SmemPair) + 1024;
+// Persistent workers on `tiles` tiles (at most).
+template <int CTAS, int BT, int OUT>
+cudaError_t launch_worker(const Int8Params& p, const Maps& m, long long tiles, cudaStream_t st) {
+  void (*kern)(CUtensorMap, CUtensorMap, Int8Params);
+  if constexpr (CTAS == 2) kern = int8_pair_kernel<OUT>;
+  else kern = int8_single_kernel<BT, OUT>;
+  constexpr size_t SMEM = sizeof(typename Worker<CTAS, BT>::Smem) + 1024;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static SmemLimit limit;
   const cudaError_t err = limit.set(reinterpret_cast<const void*>(kern), SMEM);
   if (err != cudaSuccess) return err;
-  const long long pairs = sms() / 2;
-  kern<<<(unsigned)(2 * (tiles < pairs ? tiles : pairs)), PAIR_THREADS, SMEM, st>>>(m.w, m.a, p);
-  return cudaGetLastError();
+  const long long workers = sms() / CTAS;
+  return launch_dependent(kern, dim3((unsigned)(CTAS * (tiles < workers ? tiles : workers))), WORKER_THREADS, SMEM, 0, st, m.w, m.a, p);
+}
+template <int CTAS, int BT>
+cudaError_t launch_worker_out(const Int8Params& p, const Maps& m, long long tiles, cudaStream_t st) {
+  switch (p.out_dtype) {
+    case MMB200_OUT_F32: return launch_worker<CTAS, BT, MMB200_OUT_F32>(p, m, tiles, st);
+    case MMB200_OUT_BF16: return launch_worker<CTAS, BT, MMB200_OUT_BF16>(p, m, tiles, st);
+    default: return launch_worker<CTAS, BT, MMB200_OUT_F16>(p, m, tiles, st);
+  }
 }
 template <int BT>
 cudaError_t launch_out(const Int8Params& p, const Maps& m, int parts, unsigned tiles_t, cudaStream_t st) {
@@ -648,53 +719,47 @@ size_t int8_workspace_bytes(const Int8Params& p) {
   return n;
 }
 
-namespace {
-cudaError_t launch_zero_rest(const Int8Params& p, cudaStream_t st, int* launches) {
-  if (!p.offs || !p.zero_rest) return cudaSuccess;
-  zero_rest_kernel<<<(unsigned)sms(), 256, 0, st>>>(p);
-  const cudaError_t err = cudaGetLastError();
-  if (err == cudaSuccess) *launches += 1;
-  return err;
-}
-}  // namespace
-
 cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st, int* launches) {
   Int8Params p = p_in;
-  if (p.E == 0) return launch_zero_rest(p, st, launches);
   staged_wait_limits(&p.wait_polls, &p.announce_extra);
   cudaError_t err = int8_status_word(&p.status);
   if (err != cudaSuccess) return err;
   int8_t* ws = static_cast<int8_t*>(workspace);
   if (p.K > 0) {
     const long long pitch = pitch_of(p.K);
-    const unsigned most = (unsigned)sms() * 16;
+    Repack r[2];
+    std::memset(r, 0, sizeof(r));
+    r[0].rows_per_group = r[1].rows_per_group = 1;
     if (!in_place(p.a, p.lda, p.T, 0, 1)) {
-      repack_kernel<<<(unsigned)(p.T < (int)most ? p.T : (int)most), 256, 0, st>>>(p.a, p.lda, 0, p.T, p.T, p.K, ws, pitch);
-      if ((err = cudaGetLastError()) != cudaSuccess) return err;
-      *launches += 1;
+      r[0] = Repack{p.a, ws, p.lda, 0, p.T, p.T};
       p.a = ws;
       p.lda = pitch;
       ws += (size_t)p.T * pitch;
     }
     if (!in_place(p.w, p.ldw, p.N, p.gsw, p.E)) {
-      const long long rows = (long long)p.E * p.N;
-      repack_kernel<<<(unsigned)(rows < (long long)most ? rows : (long long)most), 256, 0, st>>>(p.w, p.ldw, p.gsw, p.N, rows, p.K, ws, pitch);
-      if ((err = cudaGetLastError()) != cudaSuccess) return err;
-      *launches += 1;
+      r[1] = Repack{p.w, ws, p.ldw, p.gsw, p.N, (long long)p.E * p.N};
       p.w = ws;
       p.ldw = pitch;
       p.gsw = pitch * p.N;
+    }
+    const long long rows = r[0].rows + r[1].rows, most = 16ll * sms();
+    if (rows) {
+      err = launch_dependent(repack_kernel, dim3((unsigned)(rows < most ? rows : most)), 256, 0, 0, st, r[0], r[1], p.K, pitch);
+      if (err != cudaSuccess) return err;
+      *launches += 1;
     }
   }
   p.k_blocks = (p.K + KB - 1) / KB;
   p.tiles_n = (p.N + CH - 1) / CH;
   // rows of a tile: a power of two that holds the rows of a group, at most 256
   const long long per_group = ((long long)p.T + p.E - 1) / p.E;
-  bool pair = per_group >= 192 && p.K > 0;
- if (getenv("MMB_PAIR")) pair = atoi(getenv("MMB_PAIR"));
+  enum { TILE, SINGLE, PAIR } kind = TILE;
   int bt = per_group <= 16 ? 16 : per_group <= 32 ? 32 : per_group <= 64 ? 64 : per_group <= 128 ? 128 : 256;
- if (getenv("MMB_BT")) bt = atoi(getenv("MMB_BT"));
- if (pair) bt=256;
+  if (per_group >= 192) kind = PAIR;
+  if (getenv("MMB_KIND")) kind = (decltype(kind))atoi(getenv("MMB_KIND"));
+  if (getenv("MMB_BT")) bt = atoi(getenv("MMB_BT"));
+  if (kind == PAIR) bt = 256;
+  if (p.K == 0) { kind = TILE; }
   const long long tiles_t = p.offs ? (long long)p.T / bt + (p.E < p.T ? p.E : p.T) : ((long long)p.T + bt - 1) / bt;
   if (tiles_t > 65535) return cudaErrorInvalidValue;
   Maps m;
@@ -703,16 +768,24 @@ cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st
     // (a single row's stride is never used, but the map wants a multiple of 16)
     const long long ldw = p.N > 1 ? p.ldw : pitch_of(p.K), lda = p.T > 1 ? p.lda : pitch_of(p.K);
     err = byte_map(&m.w, p.w, p.K, p.N, ldw, p.E, p.E > 1 ? p.gsw : pitch_of(p.K), CH, true);
-    if (err == cudaSuccess) err = byte_map(&m.a, p.a, p.K, p.T, lda, 1, 0, pair ? CH : bt, false);
+    if (err == cudaSuccess) err = byte_map(&m.a, p.a, p.K, p.T, lda, 1, 0, kind == PAIR ? CH : bt, false);
     if (err != cudaSuccess) return err;
   }
-  if (pair) {
-    const long long tiles = tiles_t * ((p.N + 2 * CH - 1) / (2 * CH));      // at most
-    err = p.out_dtype == MMB200_OUT_F32 ? launch_pair<MMB200_OUT_F32>(p, m, tiles, st)
-          : p.out_dtype == MMB200_OUT_BF16 ? launch_pair<MMB200_OUT_BF16>(p, m, tiles, st) : launch_pair<MMB200_OUT_F16>(p, m, tiles, st);
+  if (kind == PAIR) {
+    err = launch_worker_out<2, 256>(p, m, tiles_t * ((p.N + 2 * CH - 1) / (2 * CH)), st);
+  } else if (kind == SINGLE) {
+    const long long tiles = tiles_t * p.tiles_n;
+    switch (bt) {
+      case 32: err = launch_worker_out<1, 32>(p, m, tiles, st); break;
+      case 64: err = launch_worker_out<1, 64>(p, m, tiles, st); break;
+      case 128: err = launch_worker_out<1, 128>(p, m, tiles, st); break;
+      default: err = launch_worker_out<1, 256>(p, m, tiles, st); break;
+    }
+  }
+  if (kind != TILE) {
     if (err != cudaSuccess) return err;
     *launches += 1;
-    return launch_zero_rest(p, st, launches);
+    return cudaSuccess;
   }
   int parts = 1;
   const long long ctas = (long long)p.tiles_n * tiles_t;
@@ -727,7 +800,7 @@ cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st
   }
   if (err != cudaSuccess) return err;
   *launches += 1;
-  return launch_zero_rest(p, st, launches);
+  return cudaSuccess;
 }
 
 }  // namespace mmb
