@@ -275,6 +275,10 @@ int mmb200_int8_scaled_mm(const int8_t *A_dev, int64_t lda, const int8_t *W_dev,
                           const float *scale_a_dev, int sa_stride, const float *scale_b_dev, int64_t sb_group_stride,
                           int sb_stride, const void *bias_dev, int bias_dtype, int64_t bias_group_stride, int zero_rest,
                           void *workspace_dev, size_t workspace_bytes, void *stream);
+/* The kernel that a call of this shape runs on: kind << 16 | rows of a tile << 4 | parts of K, kind 0: one tile per CTA (a
+ * cluster of `parts` CTAs shares a tile), 1: persistent CTAs, 2: persistent pairs of CTAs. ragged: whether offs_dev is given.
+ * Pure host logic (148 SMs are assumed where no device answers). */
+int mmb200_int8_kernel_for(int T, int N, int K, int E, int ragged);
 /* Synchronises `stream`, reads and clears the current device's status word of the int8 kernels: MMB200_ERR_TIMEOUT when a
  * bounded wait has run out since the word was last read (outputs of that call are unspecified), else MMB200_OK. With
  * MMAEMU_B200_CHECK_STATUS=1 in the environment mmb200_int8_scaled_mm ends with this call. */

@@ -26,7 +26,7 @@ EXPORTS = ("mmb200_abi_version", "mmb200_status_string", "mmb200_last_cuda_error
            "mmb200_scaled_mm_static", "mmb200_quantize_scaled_mm_ws", "mmb200_workspace_status_offset",
            "mmb200_workspace_status", "mmb200_scaled_mm_static_status", "mmb200_test_hooks", "mmb200_scaled_mm_peers", "mmb200_probe_issue_rate",
            "mmb200_grouped_workspace_bytes", "mmb200_grouped_scaled_mm", "mmb200_grouped_status", "mmb200_quantize_int8", "mmb200_int8_workspace_bytes",
-           "mmb200_int8_scaled_mm", "mmb200_int8_status")
+           "mmb200_int8_scaled_mm", "mmb200_int8_kernel_for", "mmb200_int8_status")
 
 _lock = threading.Lock()
 _lib = None
@@ -118,6 +118,8 @@ def load():
         L.mmb200_int8_scaled_mm.argtypes = [vp, i64, vp, i64, i64, vp, i64, ci, ci, ci, ci, ci, vp, vp, ci, vp, i64, ci, vp, ci,
                                             i64, ci, vp, sz, vp]
         L.mmb200_int8_scaled_mm.restype = ci
+        L.mmb200_int8_kernel_for.argtypes = [ci, ci, ci, ci, ci]
+        L.mmb200_int8_kernel_for.restype = ci
         L.mmb200_int8_status.argtypes = [vp]
         L.mmb200_int8_status.restype = ci
         L.mmb200_launch_count.argtypes = []

@@ -741,6 +741,16 @@ int mmb200_int8_scaled_mm(const int8_t* A, int64_t lda, const int8_t* W, int64_t
   return check && check[0] == '1' && !check[1] ? mmb200_int8_status(stream) : MMB200_OK;
 }
 
+int mmb200_int8_kernel_for(int T, int N, int K, int E, int ragged) {
+  if (T <= 0 || N <= 0 || K < 0 || E < 1) return MMB200_ERR_BAD_ARG;
+  static const int any = 0;
+  mmb::Int8Params p;
+  std::memset(&p, 0, sizeof(p));
+  p.T = T; p.N = N; p.K = K; p.E = E;
+  p.offs = ragged ? &any : nullptr;                 // (only whether it is given)
+  return mmb::int8_kernel_for(p);
+}
+
 int mmb200_int8_status(void* stream) {
   const int rc = current_device_ok();
   if (rc != MMB200_OK) return rc;

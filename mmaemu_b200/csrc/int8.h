@@ -67,6 +67,7 @@ struct Int8Params {
 // Scratch memory for operands that TMA cannot read in place (0: none needed).
 size_t int8_workspace_bytes(const Int8Params& p);
 cudaError_t launch_int8(const Int8Params& p, void* workspace, cudaStream_t st, int* launches);
+int int8_kernel_for(const Int8Params& p);       // mmb200_int8_kernel_for
 // The device's status word (zero until a bounded wait of an int8 kernel runs out).
 cudaError_t int8_status_word(int** word);
 

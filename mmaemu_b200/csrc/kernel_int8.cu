@@ -53,11 +53,11 @@ __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x,
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ int remote_int(uint32_t addr, int rank) {
+__device__ __forceinline__ int4 remote_int4(uint32_t addr, int rank) {        // of a CTA of the cluster
   uint32_t there;
-  int v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(there) : "memory");
+  int4 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(there));
   return v;
 }
 template <int N>
@@ -133,6 +133,44 @@ __device__ __forceinline__ void write_rows(const Int8Params& p, uint32_t acc, bo
   }
 }
 
+// The same for the sums of a cluster, [row][channel] in the shared memory of each of its CTAs: CTA `rank` writes the rows
+// rank, rank + parts, ..., a warp a row, a lane four channels. All the loads of a row are in flight at once.
+template <int OUT>
+__device__ __forceinline__ void write_sums(const Int8Params& p, const int* part, int parts, int rank, long long row0, int rows, int n0, int g) {
+  using O = typename OutType<OUT>::type;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32 - 2, n = n0 + 4 * lane;
+  float sb[4], bias[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    sb[q] = n + q < p.N ? __ldg(p.scale_b + (long long)g * p.sb_group + (long long)(n + q) * p.sb_stride) : 0.0f;
+    bias[q] = n + q < p.N ? bias_at(p, (long long)g * p.bias_group + n + q) : 0.0f;
+  }
+  for (int c = rank + parts * warp; c < rows; c += 4 * parts) {
+    const uint32_t addr = smem_addr(part + c * CH + 4 * lane);
+    int4 v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < parts) v[q] = remote_int4(addr, q);
+    const float sa = __ldg(p.scale_a + (row0 + c) * p.sa_stride);
+    int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < parts) { sum[0] += v[q].x; sum[1] += v[q].y; sum[2] += v[q].z; sum[3] += v[q].w; }
+    O* out = static_cast<O*>(p.d) + (row0 + c) * p.ldd + n;
+    O y[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) y[q] = out_bits<OUT>(__fmaf_rn(__int2float_rn(sum[q]), __fmul_rn(sa, sb[q]), bias[q]));
+    if (n + 4 <= p.N && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(O)) == 0) {
+      if constexpr (sizeof(O) == 4) *reinterpret_cast<uint4*>(out) = make_uint4(y[0], y[1], y[2], y[3]);
+      else *reinterpret_cast<uint2*>(out) = make_uint2(y[0] | ((uint32_t)y[1] << 16), y[2] | ((uint32_t)y[3] << 16));
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (n + q < p.N) out[q] = y[q];
+    }
+  }
+}
+
 // ---- groups. Ends are taken as a running maximum, clamped to [0, T], so that no content of offs leads out of the operands.
 struct Group { int g, start, end, tile, last; };       // g < 0: no such tile; last: the end of the last group
 // The group of tile `slot` of BT rows, found by one warp (every lane returns it).
@@ -182,11 +220,7 @@ __device__ __forceinline__ void zero_rows(const Int8Params& p, int first, int st
 }
 
 template <int BT>
-constexpr int tile_stages() { return
-#ifdef ST16
- BT <= 16 ? ST16 :
-#endif
- BT <= 16 ? 6 : (BT <= 32 ? 5 : 4); }
+constexpr int tile_stages() { return BT <= 16 ? 6 : (BT <= 32 ? 5 : 4); }
 template <int BT>
 struct SmemTile {
   static constexpr int STAGES = tile_stages<BT>();
@@ -301,19 +335,8 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
     const float sb = real ? __ldg(p.scale_b + (long long)g.g * p.sb_group + (long long)n * p.sb_stride) : 0.0f;
     const float bias = real ? bias_at(p, (long long)g.g * p.bias_group + n) : 0.0f;
     const int rows = min(g.end - row0, BT);
-    if (parts == 1) {
-      write_rows<OUT, BT>(p, mine, nk > 0, row0, rows, n, real, sb, bias, row_scales<(BT < 32 ? BT : 32)>(p, row0, rows));
-    } else {
-      using O = typename OutType<OUT>::type;
-      const int c1 = min(BT * (rank + 1) / parts, rows);
-      for (int c = BT * rank / parts; c < c1; ++c) {
-        int acc = 0;
-        for (int q = 0; q < parts; ++q) acc += remote_int(smem_addr(part + c * CH + lane_ch), q);
-        const long long row = row0 + c;
-        const float alpha = __fmul_rn(__ldg(p.scale_a + row * p.sa_stride), sb);
-        if (real) static_cast<O*>(p.d)[row * p.ldd + n] = out_bits<OUT>(__fmaf_rn(__int2float_rn(acc), alpha, bias));
-      }
-    }
+    if (parts == 1) write_rows<OUT, BT>(p, mine, nk > 0, row0, rows, n, real, sb, bias, row_scales<(BT < 32 ? BT : 32)>(p, row0, rows));
+    else write_sums<OUT>(p, part, parts, rank, row0, rows, n0, g.g);
   }
   if (parts > 1) {                                  // nobody leaves while its sums may be read
     cluster_arrive();
@@ -331,7 +354,8 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
 // A worker's tile is CH * CTAS channels x up to BT rows. In a pair each CTA holds its channels and half of the rows.
 template <int CTAS, int BT>
 struct Worker {
-  static constexpr int ROWS = BT / CTAS;                            // rows that a CTA brings
+  static constexpr int ROWS = BT / CTAS;                            // rows that a CTA brings, at most
+  static constexpr int BOX = ROWS < 64 ? ROWS : 64;                 // a copy's rows: only the copies that a tile needs are made
   static constexpr int STAGES = 196608 / ((CH + ROWS) * KB);        // 192 KB of stages
   static constexpr int COLS = 2 * BT < 32 ? 32 : 2 * BT;            // two accumulators
   struct Stage { unsigned char w[CH * KB], a[ROWS * KB]; };
@@ -463,14 +487,15 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
     if (lane == 0) {
       unsigned it = 0;
       for (long long t = first; ok && walk.find(p, tiles_n, t, row0, n_tile); t += step) {
-        const int my_row = row0 + (CTAS == 2 ? walk.template columns<CTAS>(row0) / 2 * rank : 0);
+        const int mine = walk.template columns<CTAS>(row0) / CTAS, my_row = row0 + mine * rank, boxes = (mine + W::BOX - 1) / W::BOX;
+        const uint32_t bytes = CTAS * (uint32_t)(sizeof(sm.stage[0].w) + boxes * W::BOX * KB);
         for (int kb = 0; kb < nk; ++kb, ++it) {
           const unsigned s = it % STAGES, round = it / STAGES;
           if (round && !mbar_wait(&sm.empty[s], (round - 1) & 1, p.wait_polls)) { ok = false; break; }
-          if (rank == 0) mbar_expect_tx(&sm.full[s], CTAS * (uint32_t)sizeof(typename W::Stage) + (uint32_t)p.announce_extra);
+          if (rank == 0) mbar_expect_tx(&sm.full[s], bytes + (uint32_t)p.announce_extra);
           const uint32_t bar = first_cta<CTAS>(&sm.full[s]);
           load_channels<CTAS>(sm.stage[s].w, &map_w, kb * KB, (CTAS * n_tile + rank) * CH, walk.g, bar);
-          load_rows<CTAS>(sm.stage[s].a, &map_a, kb * KB, my_row, bar);
+          for (int q = 0; q < boxes; ++q) load_rows<CTAS>(sm.stage[s].a + q * W::BOX * KB, &map_a, kb * KB, my_row + q * W::BOX, bar);
         }
       }
       // no CTA ends while a copy may be in flight: the worker's first CTA waits for the last copies into every stage (bounded)
@@ -517,7 +542,7 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
       ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sm.acc_full[i & 1], (i >> 1) & 1, p.wait_polls));
       if (!ok) break;
       fence_after();
-      write_rows<OUT, BT / 2>(p, mine + (i & 1) * BT, true, row0 + half, rows, n, real, sb, bias, scale);
+      write_rows<OUT, BT / 2>(p, mine + (i & 1) * BT, nk > 0, row0 + half, rows, n, real, sb, bias, scale);
       fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -698,6 +723,55 @@ cudaError_t launch_out(const Int8Params& p, const Maps& m, int parts, unsigned t
   }
 }
 
+// Kernel, rows of a tile and parts of K by estimated time, in microseconds. A CTA takes TAU per 128 bytes of K and tile (MMAs of
+// 128 channels take about 120 cycles up to 128 rows); all of them together get L2_RATE out of the caches and HBM_RATE out of
+// memory; the slowest of the three counts, and a part of the first (REST), as they overlap only in part. START and the output of
+// the last tile (OUT per row) come on top, the cluster's sum (SUM, PART each) and every further wave of one-tile CTAs (WAVE). Measured on whole calls, replayed from a graph: 1 to 2048 rows, 512 to 24576 channels, K from 512 to
+// 28672; the choice was within 5 % of the best of all of them for most, within 20 % for all.
+enum Kind { TILE, SINGLE, PAIR };
+struct Choice { Kind kind; int rows, parts; };
+long long most_row_tiles(const Int8Params& p, int rows) {               // of all groups: every one may end in a partial tile
+  return p.offs ? (long long)p.T / rows + (p.E < p.T ? p.E : p.T) : ((long long)p.T + rows - 1) / rows;
+}
+Choice choose(const Int8Params& p) {
+  constexpr double L2_RATE = 14e6, HBM_RATE = 6.1e6, OUT = 0.011, SUM = 1.8, PART = 0.1, WAVE = 2.0, REST = 0.15;
+  const long long n_sm = sms(), used = p.E < p.T ? p.E : p.T;             // groups with rows, at most
+  const double hbm = ((double)used * p.N + p.T) * p.K / HBM_RATE;
+  Choice best{TILE, 16, 1};
+  double least = 1e30;
+  auto consider = [&](Kind kind, int rows, int parts, double start, double tau) {
+    if (kind == TILE && most_row_tiles(p, rows) > 65535) return;          // grid y
+    const int ctas_per_tile = kind == PAIR ? 2 : 1, occupancy = kind == TILE ? 2 : 1;
+    const long long tiles_n = ((long long)p.N + CH * ctas_per_tile - 1) / (CH * ctas_per_tile);
+    // every group ends in a tile that is half full on average
+    const double tiles_t = p.offs ? (double)p.T / rows + 0.5 * used : (double)(((long long)p.T + rows - 1) / rows);
+    const double tiles = tiles_t * tiles_n, workers = (double)(n_sm / ctas_per_tile);
+    auto waves = [](double n, double at_once) { return n <= at_once ? 1.0 : (double)(long long)(n / at_once + 0.999); };
+    // rows that a tile copies: its own, a one-tile CTA all
+    const double copied = kind == TILE ? rows : (double)p.T / tiles_t + (p.T > 64 ? 32 : 0);
+    const double l2 = tiles * p.k_blocks * KB * (CH * ctas_per_tile + copied) / L2_RATE;
+    const double mma = tau * p.k_blocks / parts * waves(tiles * parts, workers);
+    double t = mma > l2 ? mma : l2;
+    t = t > hbm ? t : hbm;
+    t += REST * mma + start + OUT * rows + (parts > 1 ? SUM + PART * parts : 0.0) + (kind == TILE ? WAVE * (waves(tiles * parts, workers * occupancy) - 1.0) : 0.0);
+    if (parts > 1 && tiles * parts > 2.0 * n_sm) return;                 // clusters that wait for room cost more than they save
+    if (t < least) {
+      least = t;
+      best = Choice{kind, rows, parts};
+    }
+  };
+  for (int parts = 1; parts <= 8 && parts <= (p.k_blocks > 1 ? p.k_blocks : 1); parts *= 2) {
+    consider(TILE, 16, parts, 1.4, 0.25);
+    consider(TILE, 32, parts, 1.4, 0.25);
+    consider(TILE, 64, parts, 1.4, 0.26);
+  }
+  consider(SINGLE, 64, 1, 2.6, 0.27);
+  consider(SINGLE, 128, 1, 2.6, 0.28);
+  consider(SINGLE, 256, 1, 2.6, 0.40);
+  consider(PAIR, 256, 1, 3.2, 0.34);
+  return best;
+}
+
 }  // namespace
 
 cudaError_t int8_status_word(int** word) {
@@ -717,6 +791,13 @@ size_t int8_workspace_bytes(const Int8Params& p) {
   if (!in_place(p.a, p.lda, p.T, 0, 1)) n += (size_t)p.T * pitch_of(p.K);
   if (!in_place(p.w, p.ldw, p.N, p.gsw, p.E)) n += (size_t)p.E * p.N * pitch_of(p.K);
   return n;
+}
+
+int int8_kernel_for(const Int8Params& p_in) {
+  Int8Params p = p_in;
+  p.k_blocks = (p.K + KB - 1) / KB;
+  const Choice c = choose(p);
+  return c.kind << 16 | c.rows << 4 | c.parts;
 }
 
 cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st, int* launches) {
@@ -751,52 +832,29 @@ cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st
   }
   p.k_blocks = (p.K + KB - 1) / KB;
   p.tiles_n = (p.N + CH - 1) / CH;
-  // rows of a tile: a power of two that holds the rows of a group, at most 256
-  const long long per_group = ((long long)p.T + p.E - 1) / p.E;
-  enum { TILE, SINGLE, PAIR } kind = TILE;
-  int bt = per_group <= 16 ? 16 : per_group <= 32 ? 32 : per_group <= 64 ? 64 : per_group <= 128 ? 128 : 256;
-  if (per_group >= 192) kind = PAIR;
-  if (getenv("MMB_KIND")) kind = (decltype(kind))atoi(getenv("MMB_KIND"));
-  if (getenv("MMB_BT")) bt = atoi(getenv("MMB_BT"));
-  if (kind == PAIR) bt = 256;
-  if (p.K == 0) { kind = TILE; }
-  const long long tiles_t = p.offs ? (long long)p.T / bt + (p.E < p.T ? p.E : p.T) : ((long long)p.T + bt - 1) / bt;
-  if (tiles_t > 65535) return cudaErrorInvalidValue;
+  const Choice best = choose(p);
+  const int bt = best.rows;
+  const long long tiles_t = most_row_tiles(p, bt);
   Maps m;
   std::memset(&m, 0, sizeof(m));
   if (p.K > 0) {
     // (a single row's stride is never used, but the map wants a multiple of 16)
     const long long ldw = p.N > 1 ? p.ldw : pitch_of(p.K), lda = p.T > 1 ? p.lda : pitch_of(p.K);
     err = byte_map(&m.w, p.w, p.K, p.N, ldw, p.E, p.E > 1 ? p.gsw : pitch_of(p.K), CH, true);
-    if (err == cudaSuccess) err = byte_map(&m.a, p.a, p.K, p.T, lda, 1, 0, kind == PAIR ? CH : bt, false);
+    if (err == cudaSuccess) err = byte_map(&m.a, p.a, p.K, p.T, lda, 1, 0, bt < 64 ? bt : 64, false);
     if (err != cudaSuccess) return err;
   }
-  if (kind == PAIR) {
+  const long long tiles = tiles_t * p.tiles_n;
+  if (best.kind == PAIR) {
     err = launch_worker_out<2, 256>(p, m, tiles_t * ((p.N + 2 * CH - 1) / (2 * CH)), st);
-  } else if (kind == SINGLE) {
-    const long long tiles = tiles_t * p.tiles_n;
-    switch (bt) {
-      case 32: err = launch_worker_out<1, 32>(p, m, tiles, st); break;
-      case 64: err = launch_worker_out<1, 64>(p, m, tiles, st); break;
-      case 128: err = launch_worker_out<1, 128>(p, m, tiles, st); break;
-      default: err = launch_worker_out<1, 256>(p, m, tiles, st); break;
-    }
-  }
-  if (kind != TILE) {
-    if (err != cudaSuccess) return err;
-    *launches += 1;
-    return cudaSuccess;
-  }
-  int parts = 1;
-  const long long ctas = (long long)p.tiles_n * tiles_t;
-  while (parts < 8 && bt <= 64 && ctas * parts * 2 <= 2ll * sms() && p.k_blocks >= 4 * parts) parts *= 2;
-  if (getenv("MMB_PARTS")) parts = atoi(getenv("MMB_PARTS"));
-  switch (bt) {
-    case 16: err = launch_out<16>(p, m, parts, (unsigned)tiles_t, st); break;
-    case 32: err = launch_out<32>(p, m, parts, (unsigned)tiles_t, st); break;
-    case 64: err = launch_out<64>(p, m, parts, (unsigned)tiles_t, st); break;
-    case 128: err = launch_out<128>(p, m, parts, (unsigned)tiles_t, st); break;
-    default: err = launch_out<256>(p, m, parts, (unsigned)tiles_t, st); break;
+  } else if (best.kind == SINGLE) {
+    if (bt == 64) err = launch_worker_out<1, 64>(p, m, tiles, st);
+    else if (bt == 128) err = launch_worker_out<1, 128>(p, m, tiles, st);
+    else err = launch_worker_out<1, 256>(p, m, tiles, st);
+  } else {
+    if (bt == 16) err = launch_out<16>(p, m, best.parts, (unsigned)tiles_t, st);
+    else if (bt == 32) err = launch_out<32>(p, m, best.parts, (unsigned)tiles_t, st);
+    else err = launch_out<64>(p, m, best.parts, (unsigned)tiles_t, st);
   }
   if (err != cudaSuccess) return err;
   *launches += 1;

@@ -67,6 +67,45 @@ def test_product_bits(M, N, K, out):
     same(mm.int8_scaled_mm(a, w.t(), sa, sb, out_dtype=DT[out]), want_bits(a, w, sa, sb, DT[out]))
 
 
+# every kernel, by the rule's choice: (kind, rows of a tile, parts of K) -> rows, channels, K; a worker's second and third tile,
+# ragged rows, channels and K among them
+KERNELS = [((0, 16, 1), 40, 300, 100), ((0, 16, 2), 1, 5000, 2000), ((0, 16, 4), 300, 16, 2000), ((0, 16, 8), 7, 130, 2001),
+           ((0, 32, 1), 3000, 16, 48), ((0, 32, 2), 17, 5000, 2000), ((0, 32, 4), 700, 16, 2000), ((0, 32, 8), 300, 17, 5000),
+           ((0, 64, 1), 33, 20000, 17), ((0, 64, 2), 3000, 16, 5000), ((0, 64, 4), 1500, 16, 2000), ((0, 64, 8), 700, 16, 5000),
+           ((1, 64, 1), 65, 20000, 130), ((1, 128, 1), 1000, 2064, 1936), ((1, 128, 1), 1030, 5000, 300), ((1, 256, 1), 5000, 500, 1000),
+           ((2, 256, 1), 2050, 5000, 300), ((2, 256, 1), 2000, 8200, 528)]
+RAGGED = [((0, 16, 8), [0, 33, 0, 1], 16, 5000), ((0, 64, 1), [16, 0, 5], 20000, 40), ((1, 64, 1), [25, 0, 70, 3] * 10, 2000, 500),
+          ((1, 128, 1), [300, 0, 1, 128, 129, 900, 42, 600], 4100, 300), ((1, 256, 1), [3, 257, 256, 0, 484, 0, 0, 0], 2000, 1000),
+          ((2, 256, 1), [1, 800, 256, 0, 1300, 33, 1610], 2050, 1040)]
+
+
+def kind_of(T, N, K, E=1, ragged=0):
+    c = _lib.load().mmb200_int8_kernel_for(T, N, K, E, ragged)
+    return c >> 16, (c >> 4) & 0xFFF, c & 15
+
+
+@pytest.mark.parametrize("out", DT)
+@pytest.mark.parametrize("kind,M,N,K", KERNELS, ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else str(v))
+def test_every_kernel(kind, M, N, K, out):
+    assert kind_of(M, N, K) == kind
+    a, w = codes(M, K, seed=M), codes(N, K, seed=N + 1)
+    sa, sb = scales(M, 1, seed=K), scales(1, N, seed=K + 1)
+    for _ in range(2):
+        same(mm.int8_scaled_mm(a, w.t(), sa, sb, out_dtype=DT[out]), want_bits(a, w, sa, sb, DT[out]))
+
+
+@pytest.mark.parametrize("kind,sizes,N,K", RAGGED, ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else None)
+@pytest.mark.parametrize("spare", [0, 37])
+def test_every_kernel_with_ragged_groups(kind, sizes, N, K, spare):
+    E, T = len(sizes), sum(sizes) + spare
+    if not spare:
+        assert kind_of(T, N, K, E, 1) == kind
+    a, w = codes(T, K, seed=T), codes(E, N, K, seed=N)
+    sa, sb = scales(T, 1, seed=1), scales(E, 1, N, seed=2)
+    ends = torch.tensor(sizes, device=DEV).cumsum(0).to(torch.int32)
+    same(mm.int8_grouped_scaled_mm(a, w.transpose(1, 2), ends, sa, sb), grouped_want(a, w, ends.tolist(), sa, sb, torch.bfloat16))
+
+
 @pytest.mark.parametrize("M", [1, 16, 130, 300])
 @pytest.mark.parametrize("K", [131071, 131056])
 def test_largest_sums(M, K):
@@ -396,10 +435,11 @@ def test_streams_and_graphs():
         same(got, step())
 
 
-@pytest.mark.parametrize("M", [4, 100, 400])
-def test_a_wait_that_runs_out_is_reported(M):
+@pytest.mark.parametrize("M,N,K", [(4, 512, 2048), (100, 512, 2048), (400, 512, 2048), (65, 20000, 1300), (1000, 2064, 1936), (5000, 500, 1000),
+                                   (2000, 8200, 1280)])
+def test_a_wait_that_runs_out_is_reported(M, N, K):
     """The test hook announces more bytes than arrive: the bounded waits run out, the call reports it, the next call works."""
-    a, w = codes(M, 2048, seed=1), codes(512, 2048, seed=2)
+    a, w = codes(M, K, seed=1), codes(N, K, seed=2)
     one = torch.ones(1, device=DEV)
     want = mm.int8_scaled_mm(a, w.t(), one, one)
     L = _lib.load()
