@@ -317,6 +317,37 @@ struct Epilogue {
   }
 };
 
+// ---------------------------------------------------------------------------------------------------------------
+// Programmatic dependent launch: a kernel launched this way starts while the previous one of the stream is still running, and
+// every thread of it waits, before its first access to memory, until that has completed -- so a kernel is never complete before
+// its predecessors are. The next kernel may start as soon as every CTA of this one has called dependent_launch_next; a kernel
+// with tensor memory does so after its allocation, so that the next one cannot take what it still needs.
+__device__ __forceinline__ void dependent_launch_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void dependent_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// cluster: CTAs per cluster (0: the kernel's own).
+template <class... P, class... A>
+cudaError_t launch_dependent_cluster(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t st,
+                                     const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+template <class... P, class... A>
+cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const A&... args) {
+  return launch_dependent_cluster(kern, grid, threads, smem, 0, st, args...);
+}
+
 // Launchers implemented by the kernel translation units; each returns a cudaError_t.
 cudaError_t launch_integer(const Params& p, int nfma, cudaStream_t stream);
 cudaError_t launch_fast(const Params& p, int nfma, cudaStream_t stream);

@@ -7,34 +7,6 @@
 
 namespace mmb {
 
-#if defined(__CUDACC__)
-// Programmatic dependent launch: these kernels start while the previous one of the stream is still running, set up barriers and
-// TMEM, and wait here, before their first access to memory, until it has completed. Every thread waits, so a kernel is never
-// complete before its predecessors are. The next kernel may start as soon as every CTA of this one has.
-__device__ __forceinline__ void wait_for_predecessor() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-// Launch with that attribute; `cluster`: CTAs per cluster (0: the kernel's own).
-template <class... P, class... A>
-cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t st, const A&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = cluster;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, args...);
-}
-#endif
-
 struct QuantiseParams {
   const void* x;          // [rows, K], row stride ldx elements
   int8_t* codes;          // [rows, K], row stride ldc

@@ -571,6 +571,10 @@ __device__ __forceinline__ void after_tile(const Params& p, float (&acc)[TM][TN]
 // non-finite patch and the epilogue. Grid: (output tiles, 64 outputs per thread of the first pass), 256 threads.
 template <bool GROUPED>
 __global__ void __launch_bounds__(THREADS) combine_kernel(const __grid_constant__ Params p) {
+  if (GROUPED) {
+    dependent_launch_wait();
+    dependent_launch_next();
+  }
   const int tid = threadIdx.x, idx = blockIdx.y, i = idx / TN, j = idx % TN;
   int tile_m, tile_n;
   tile_of_cta(p, (int)blockIdx.x, tile_m, tile_n);
@@ -642,9 +646,9 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const __grid_constant_
 }
 
 #if !defined(MMB_PART) || MMB_PART == 0
-// Writes the tile sequence and, behind it (`events`, when not null), the entries that matter to the second pass of
+// By one block of THREADS threads: writes the tile sequence and, behind it (`events`, when not null), the entries that matter to the second pass of
 // K-sliced execution in the same order: those after which a chain or a split is complete.
-__global__ void plan_sequence_kernel(Plan plan, int K, uint32_t* out, uint32_t* events) {
+__device__ __forceinline__ void write_sequence(const Plan& plan, int K, uint32_t* out, uint32_t* events) {
   const int n = plan_sequence(plan, K, out, (int)threadIdx.x, (int)blockDim.x);
   if (!events) return;
   // order-preserving compaction by the whole block, 256 entries at a time (ballots inside the warps, then the warps'
@@ -673,6 +677,7 @@ __global__ void plan_sequence_kernel(Plan plan, int K, uint32_t* out, uint32_t* 
     __syncthreads();
   }
 }
+__global__ void plan_sequence_kernel(Plan plan, int K, uint32_t* out, uint32_t* events) { write_sequence(plan, K, out, events); }
 #endif
 
 // Non-finite patch and epilogue for the thread's outputs. flag_a / flag_b: per-row classes of the tile's rows / columns.
@@ -1048,6 +1053,8 @@ __global__ void __launch_bounds__(THREADS, TMI == 2 ? 2 : 1) staged_tc_kernel(co
 template <int NFMA, int FA, int FB, bool SLOW, int MODE>
 __global__ void __launch_bounds__(THREADS, 2) grouped_rows16_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
+  dependent_launch_wait();
+  dependent_launch_next();
   few_rows_body<NFMA, FA, FB, SLOW, MODE, true, true>(p, smem_raw);
 }
 
@@ -1091,8 +1098,7 @@ cudaError_t launch_grouped_rows16(const Params& p, cudaStream_t stream, int* lau
     if ((long long)tiles * p.slices <= sm_count() && smem < ((size_t)120 << 10)) smem = (size_t)120 << 10;   // as launch_staged_main
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    kern<<<dim3(tiles, (unsigned)p.slices), THREADS, smem, stream>>>(p);
-    e = cudaGetLastError();
+    e = launch_dependent(kern, dim3(tiles, (unsigned)p.slices), THREADS, smem, stream, p);
     if (e == cudaSuccess) *launches += 1;
     return e;
   };
@@ -1101,8 +1107,7 @@ cudaError_t launch_grouped_rows16(const Params& p, cudaStream_t stream, int* lau
                   : go(grouped_rows16_kernel<NFMA, FA, FB, true, MODE_ORDER>, smem_few<true>(true));
   cudaError_t err = go(grouped_rows16_kernel<NFMA, FA, FB, true, MODE_SLICED>, smem_few<true>(false));
   if (err != cudaSuccess) return err;
-  combine_kernel<true><<<dim3(tiles, 2 * TN), THREADS, 0, stream>>>(p);
-  err = cudaGetLastError();
+  err = launch_dependent(combine_kernel<true>, dim3(tiles, 2 * TN), THREADS, 0, stream, p);
   if (err == cudaSuccess) *launches += 1;
   return err;
 }
@@ -1566,10 +1571,18 @@ struct GroupTable { GroupEntry e[CAP]; };
 
 template <int CAP>
 __global__ void __launch_bounds__(THREADS) group_table_kernel(const __grid_constant__ GroupTable<CAP> table, int n, RowTile* tiles, int* slots,
-                                                              uint4* zero, long long zero_vecs) {
+                                                              uint4* zero, long long zero_vecs, Plan plan, int K, uint32_t* seq,
+                                                              uint32_t* events) {
+  dependent_launch_wait();
+  dependent_launch_next();
   const int b = (int)blockIdx.x, tid = (int)threadIdx.x;
-  if (b >= n) {                              // the other blocks clear the flags and the status word
-    for (long long i = (long long)(b - n) * THREADS + tid; i < zero_vecs; i += (long long)(gridDim.x - n) * THREADS) zero[i] = make_uint4(0, 0, 0, 0);
+  if (seq && b == (int)gridDim.x - 1) {      // the last block: the tile sequence of K slices
+    write_sequence(plan, K, seq, events);
+    return;
+  }
+  if (b >= n) {                              // the others behind the groups: clear the flags and the status word
+    const int blocks = (int)gridDim.x - n - (seq ? 1 : 0);
+    for (long long i = (long long)(b - n) * THREADS + tid; i < zero_vecs; i += (long long)blocks * THREADS) zero[i] = make_uint4(0, 0, 0, 0);
     return;
   }
   const GroupEntry e = table.e[b];
@@ -1688,28 +1701,39 @@ cudaError_t launch_grouped(const Params& p_in, int nfma, const int* rows, const 
   p.plan_group = plan.group;
   RowTile* tiles = reinterpret_cast<RowTile*>(base + g.tiles);
   cudaError_t err;
-  // the lists, and the clearing of the flags: a launch per 512 groups, one block each
+  uint32_t* seq = nullptr;
+  int seq_len = 0;
+  if (g.slices > 1) {
+    seq = reinterpret_cast<uint32_t*>(base + g.seq);
+    seq_len = plan_sequence(plan, p.K, nullptr);
+    if (2 * (size_t)seq_len * sizeof(uint32_t) > g.chain_results - g.seq) return cudaErrorInvalidValue;
+  }
+  // the lists, the sequence and the clearing of the flags: a launch per 512 groups, one block each
   {
     constexpr int CAP = 512, SMALL = 32;
     GroupTable<CAP> table;
     int n = 0, slot128 = 0, slot16 = g.slots128;
     long long row0 = 0, t128 = 0, t16 = g.n128, zero_vecs = (long long)(g.tiles / 16);
+    uint32_t* first_seq = seq;               // the first launch writes it
     auto flush = [&]() -> cudaError_t {
       const long long blocks = (zero_vecs + THREADS * 4 - 1) / (THREADS * 4), most = 4 * sm_count();
-      const unsigned grid = (unsigned)(n + (blocks < most ? blocks : most));
+      const unsigned grid = (unsigned)(n + (blocks < most ? blocks : most) + (first_seq ? 1 : 0));
       int* slots = const_cast<int*>(p.ws_slots);
       uint4* zero = reinterpret_cast<uint4*>(base);
+      cudaError_t e;
       if (n <= SMALL) {
         GroupTable<SMALL> small;
         std::memcpy(&small, &table, sizeof(GroupEntry) * n);
-        group_table_kernel<SMALL><<<grid, THREADS, 0, stream>>>(small, n, tiles, slots, zero, zero_vecs);
+        e = launch_dependent(group_table_kernel<SMALL>, dim3(grid), THREADS, 0, stream, small, n, tiles, slots, zero, zero_vecs, plan, p.K,
+                             first_seq, first_seq ? first_seq + seq_len : nullptr);
       } else {
-        group_table_kernel<CAP><<<grid, THREADS, 0, stream>>>(table, n, tiles, slots, zero, zero_vecs);
+        e = launch_dependent(group_table_kernel<CAP>, dim3(grid), THREADS, 0, stream, table, n, tiles, slots, zero, zero_vecs, plan, p.K,
+                             first_seq, first_seq ? first_seq + seq_len : nullptr);
       }
-      const cudaError_t e = cudaGetLastError();
       if (e == cudaSuccess) *launches += 1;
       n = 0;
       zero_vecs = 0;
+      first_seq = nullptr;
       return e;
     };
     for (int e = 0; e < E; ++e) {
@@ -1741,19 +1765,16 @@ cudaError_t launch_grouped(const Params& p_in, int nfma, const int* rows, const 
     p.few_rows = 1;
     p.slices = g.slices;
     if (g.slices > 1) {
-      std::vector<uint32_t> seq((size_t)plan_sequence(plan, p.K, nullptr));
-      plan_sequence(plan, p.K, seq.data());
-      p.seq_len = (int)seq.size();
-      p.n_chains = plan_chains(seq.data(), p.seq_len, plan.group);
-      if (p.n_chains != g.chains || 2 * (size_t)p.seq_len * sizeof(uint32_t) > g.chain_results - g.seq) return cudaErrorInvalidValue;
-      plan_slices(seq.data(), p.seq_len, plan.group, p.n_chains, p.slices, p.slice_start, p.chain_base);
-      for (uint32_t entry : seq) p.n_events += (seq_emits(entry, plan.group ? 1 : 0) || (entry & SEQ_SPLIT_END)) ? 1 : 0;
-      p.ws_seq = reinterpret_cast<const uint32_t*>(base + g.seq);
-      p.ws_events = p.ws_seq + p.seq_len;
+      std::vector<uint32_t> host((size_t)seq_len);
+      plan_sequence(plan, p.K, host.data());
+      p.seq_len = seq_len;
+      p.n_chains = plan_chains(host.data(), seq_len, plan.group);
+      if (p.n_chains != g.chains) return cudaErrorInvalidValue;
+      plan_slices(host.data(), seq_len, plan.group, p.n_chains, p.slices, p.slice_start, p.chain_base);
+      for (uint32_t entry : host) p.n_events += (seq_emits(entry, plan.group ? 1 : 0) || (entry & SEQ_SPLIT_END)) ? 1 : 0;
+      p.ws_seq = seq;
+      p.ws_events = seq + seq_len;
       p.ws_chains = reinterpret_cast<float*>(base + g.chain_results);
-      plan_sequence_kernel<<<1, THREADS, 0, stream>>>(plan, p.K, reinterpret_cast<uint32_t*>(base + g.seq), const_cast<uint32_t*>(p.ws_events));
-      if ((err = cudaGetLastError()) != cudaSuccess) return err;
-      *launches += 1;
     }
     if ((err = dispatch_formats(p, nfma, stream, true, launches)) != cudaSuccess) return err;
   }

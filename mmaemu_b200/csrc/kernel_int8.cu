@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "n"(COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  wait_for_predecessor();
+  dependent_launch_wait();
   if (warp == 2) {
     const Group found = find_group<BT>(p, (int)blockIdx.y);
     if (lane == 0) sm.group = found;
@@ -262,6 +262,7 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
   fence_before();
   __syncthreads();
   fence_after();
+  dependent_launch_next();
   const uint32_t tmem = sm.tmem;
   const Group g = sm.group;
   const int row0 = g.start + g.tile * BT;
@@ -478,7 +479,8 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
     cluster_wait();
   }
   fence_after();
-  wait_for_predecessor();
+  dependent_launch_wait();
+  dependent_launch_next();
   const uint32_t tmem = sm.tmem;
   bool ok = true;
   Walker<BT> walk;
@@ -583,7 +585,8 @@ struct Repack {
   long long ld, group_stride, rows_per_group, rows;
 };
 __global__ void __launch_bounds__(256) repack_kernel(const __grid_constant__ Repack r0, const __grid_constant__ Repack r1, int K, long long pitch) {
-  wait_for_predecessor();
+  dependent_launch_wait();
+  dependent_launch_next();
   for (long long i = blockIdx.x; i < r0.rows + r1.rows; i += gridDim.x) {
     const bool second = i >= r0.rows;
     const Repack& r = second ? r1 : r0;
@@ -690,7 +693,7 @@ cudaError_t launch_tile(const Int8Params& p, const Maps& m, int parts, unsigned 
   static SmemLimit limit;
   const cudaError_t err = limit.set(reinterpret_cast<const void*>(kern), SMEM);
   if (err != cudaSuccess) return err;
-  return launch_dependent(kern, dim3((unsigned)(p.tiles_n * parts), tiles_t), TILE_THREADS, SMEM, (unsigned)parts, st, m.w, m.a, p);
+  return launch_dependent_cluster(kern, dim3((unsigned)(p.tiles_n * parts), tiles_t), TILE_THREADS, SMEM, (unsigned)parts, st, m.w, m.a, p);
 }
 // Persistent workers on `tiles` tiles (at most).
 template <int CTAS, int BT, int OUT>
@@ -704,7 +707,7 @@ cudaError_t launch_worker(const Int8Params& p, const Maps& m, long long tiles, c
   const cudaError_t err = limit.set(reinterpret_cast<const void*>(kern), SMEM);
   if (err != cudaSuccess) return err;
   const long long workers = sms() / CTAS;
-  return launch_dependent(kern, dim3((unsigned)(CTAS * (tiles < workers ? tiles : workers))), WORKER_THREADS, SMEM, 0, st, m.w, m.a, p);
+  return launch_dependent(kern, dim3((unsigned)(CTAS * (tiles < workers ? tiles : workers))), WORKER_THREADS, SMEM, st, m.w, m.a, p);
 }
 template <int CTAS, int BT>
 cudaError_t launch_worker_out(const Int8Params& p, const Maps& m, long long tiles, cudaStream_t st) {
@@ -825,7 +828,7 @@ cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st
     }
     const long long rows = r[0].rows + r[1].rows, most = 16ll * sms();
     if (rows) {
-      err = launch_dependent(repack_kernel, dim3((unsigned)(rows < most ? rows : most)), 256, 0, 0, st, r[0], r[1], p.K, pitch);
+      err = launch_dependent(repack_kernel, dim3((unsigned)(rows < most ? rows : most)), 256, 0, st, r[0], r[1], p.K, pitch);
       if (err != cudaSuccess) return err;
       *launches += 1;
     }

@@ -109,7 +109,8 @@ __device__ __forceinline__ void codes_of(float (&x)[N], const RowScale& r, uint3
 template <int T, int BLOCK, bool WARP_ROW, int VPT>
 __global__ void __launch_bounds__(BLOCK) quantise_kernel(const __grid_constant__ QuantiseParams p) {
   using E = Elem<T>;
-  wait_for_predecessor();
+  dependent_launch_wait();
+  dependent_launch_next();
   constexpr int PER = E::PER16, GROUP = WARP_ROW ? 32 : BLOCK;
   const int tid = WARP_ROW ? threadIdx.x % 32 : threadIdx.x;
   const long long row = WARP_ROW ? (long long)blockIdx.x * (BLOCK / 32) + threadIdx.x / 32 : (long long)blockIdx.x;
@@ -171,10 +172,10 @@ __global__ void __launch_bounds__(BLOCK) quantise_kernel(const __grid_constant__
 template <int T>
 cudaError_t launch(const QuantiseParams& p, cudaStream_t st) {
   const int vecs = (p.K + Elem<T>::PER16 - 1) / Elem<T>::PER16;
-  if (vecs <= 64) return launch_dependent(quantise_kernel<T, 128, true, 2>, dim3((unsigned)((p.rows + 3) / 4)), 128, 0, 0, st, p);
-  if (vecs <= 256) return launch_dependent(quantise_kernel<T, 128, false, 2>, dim3((unsigned)p.rows), 128, 0, 0, st, p);
-  if (vecs <= 1024) return launch_dependent(quantise_kernel<T, 256, false, 4>, dim3((unsigned)p.rows), 256, 0, 0, st, p);
-  return launch_dependent(quantise_kernel<T, 512, false, 4>, dim3((unsigned)p.rows), 512, 0, 0, st, p);
+  if (vecs <= 64) return launch_dependent(quantise_kernel<T, 128, true, 2>, dim3((unsigned)((p.rows + 3) / 4)), 128, 0, st, p);
+  if (vecs <= 256) return launch_dependent(quantise_kernel<T, 128, false, 2>, dim3((unsigned)p.rows), 128, 0, st, p);
+  if (vecs <= 1024) return launch_dependent(quantise_kernel<T, 256, false, 4>, dim3((unsigned)p.rows), 256, 0, st, p);
+  return launch_dependent(quantise_kernel<T, 512, false, 4>, dim3((unsigned)p.rows), 512, 0, st, p);
 }
 
 }  // namespace

@@ -119,6 +119,10 @@ __device__ __forceinline__ float chain_result4(float acc) { return __fmul_rn(fm:
 // GROUPED: blockIdx.y is a row tile of the list for A; for B blockIdx.z is the number of the decoded operand.
 template <int FA, int FB, bool IS_A, bool GROUPED>
 __global__ void __launch_bounds__(THREADS) predecode_umma_kernel(const __grid_constant__ Params p) {
+  if (GROUPED) {
+    dependent_launch_wait();
+    dependent_launch_next();
+  }
   const int tid = threadIdx.x, kt = blockIdx.x, rb = blockIdx.y;
   RowTile rt = row_tile<GROUPED && IS_A, 128>(p, rb);
   if (!IS_A) rt = RowTile{rb * 128, p.N, GROUPED ? __ldg(p.ws_slots + blockIdx.z) : 0, GROUPED ? (int)blockIdx.z : 0};
@@ -159,6 +163,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_cons
   static_assert(NW == 64 || !TWO_SUMS, "TMEM holds one set of sums for 256 columns");
   extern __shared__ __align__(128) unsigned char smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  if (GROUPED) dependent_launch_wait();
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   int tile_m, tile_n;                                  // tile_n in units of 2 NW columns
   tile_of_cta(p.tiles_m, (p.N + 2 * NW - 1) / (2 * NW), BAND * 64 / NW, (int)blockIdx.x, tile_m, tile_n);
@@ -181,6 +186,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_cons
   fence_before();
   __syncthreads();
   fence_after();
+  if (GROUPED) dependent_launch_next();
   const uint32_t tmem = sm.tmem;
   bool ok = true;
   const int h = (warp % EPI_WARPS) / 8;                                               // the warp's half (scalar steps)
@@ -411,8 +417,14 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_cons
 template <int FA, int FB, bool IS_A, bool GROUPED>
 cudaError_t launch_predecode(const Params& p, cudaStream_t stream, int* launches) {
   const dim3 grid((unsigned)p.k_tiles, (unsigned)(IS_A ? p.tiles_m : p.tiles_n), GROUPED && !IS_A ? (unsigned)p.slots : 1u);
-  predecode_umma_kernel<FA, FB, IS_A, GROUPED><<<grid, THREADS, 0, stream>>>(p);
-  const cudaError_t err = cudaGetLastError();
+  auto kern = predecode_umma_kernel<FA, FB, IS_A, GROUPED>;
+  cudaError_t err;
+  if constexpr (GROUPED) {
+    err = launch_dependent(kern, grid, THREADS, 0, stream, p);
+  } else {
+    kern<<<grid, THREADS, 0, stream>>>(p);
+    err = cudaGetLastError();
+  }
   if (err == cudaSuccess) *launches += 1;
   return err;
 }
@@ -425,8 +437,13 @@ cudaError_t launch_kernel(const Params& p, cudaStream_t stream, int* launches) {
   cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
   if (err != cudaSuccess) return err;
   const long long tiles = (long long)p.tiles_m * ((p.N + 2 * NW - 1) / (2 * NW));
-  kern<<<dim3((unsigned)tiles, SLICED ? (unsigned)p.slices : 1u), UMMA_THREADS, SMEM, stream>>>(p);
-  err = cudaGetLastError();
+  const dim3 grid((unsigned)tiles, SLICED ? (unsigned)p.slices : 1u);
+  if constexpr (GROUPED) {
+    err = launch_dependent(kern, grid, UMMA_THREADS, SMEM, stream, p);
+  } else {
+    kern<<<grid, UMMA_THREADS, SMEM, stream>>>(p);
+    err = cudaGetLastError();
+  }
   if (err == cudaSuccess) *launches += 1;
   return err;
 }

@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from .api import (_check_argument_types, _check_like_cublas, _check_like_torch, _check_scope, _emit_maturity, _kernel_choice,
-                  _kernel_code, _misaligned, _on_device, _require_device, _scalar_ptr, _stream_ptr)
+                  _kernel_code, _on_device, _require_device, _scalar_ptr, _stream_ptr)
 from .errors import ReferenceRejectsError
 from .formats import OUT_DTYPE_NAMES, fmt_of
 from .numerics import check_plan, get_preset
@@ -35,11 +35,11 @@ def _sizes(m_splits, E: int, T: int) -> list:
         if m_splits.is_floating_point() or m_splits.is_complex() or m_splits.dtype == torch.bool:
             raise TypeError(f"grouped_scaled_mm(): m_splits must hold integers, got {m_splits.dtype}")
         m_splits = m_splits.tolist()
-    if not isinstance(m_splits, (list, tuple)) or any(isinstance(m, bool) or not isinstance(m, int) for m in m_splits):
+    if not isinstance(m_splits, (list, tuple)) or not all(type(m) is int for m in m_splits):
         raise TypeError("grouped_scaled_mm(): m_splits must be a list of ints (or a CPU tensor of integers)")
     if len(m_splits) != E:
         raise ValueError(f"grouped_scaled_mm(): mat2 has {E} matrices, m_splits {len(m_splits)} entries")
-    if any(m < 0 for m in m_splits) or sum(m_splits) != T:
+    if min(m_splits) < 0 or sum(m_splits) != T:
         raise ValueError(f"grouped_scaled_mm(): m_splits must be non-negative and add up to the {T} rows of input, got a sum of "
                          f"{sum(m_splits)}")
     return list(m_splits)
@@ -74,8 +74,10 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
         raise ValueError(f"grouped_scaled_mm(): between 1 and {MAX_GROUPS} groups, got {E}")
     sizes = _sizes(m_splits, E, T)
     sa, sb = _group_scale("scale_a", scale_a, E), _group_scale("scale_b", scale_b, E)
-    scaling, od = _check_like_torch(input, mat2[0], scale_a.reshape(-1)[:1], scale_b.reshape(-1)[:1], None, scale_result, out_dtype,
-                                    out)
+    w0 = mat2[0]
+    scaling, od = _check_like_torch(input, w0, scale_a if scale_a.numel() == 1 else scale_a[:1],
+                                    scale_b if scale_b.numel() == 1 else scale_b[:1], None, scale_result,
+                                    out_dtype, out)
     prof = get_profile(profile)
     preset = get_preset(prof.preset)
     if out is not None and (tuple(out.shape) != (T, N) or (N > 1 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N)):
@@ -83,8 +85,8 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
                          f"strides {tuple(out.stride())}")
     if T == 0 or N == 0 or K == 0:
         return torch.zeros((T, N), dtype=od, device=input.device) if out is None else out.zero_()
-    mat1 = _check_like_cublas(input, mat2[0], scaling, od)
-    if E > 1 and _misaligned(mat2[1]):
+    mat1 = _check_like_cublas(input, w0, scaling, od)
+    if E > 1 and mat2.stride(0) % 16:
         raise ReferenceRejectsError("CUBLAS_STATUS_NOT_SUPPORTED when calling cublasLtMatmul (operand pointer not 16-byte aligned)")
     fa, fb = fmt_of(mat1.dtype), fmt_of(mat2.dtype)
     rule = prof.rejection(fa, fb, od)
@@ -92,13 +94,21 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
         raise ReferenceRejectsError(f"{rule.message} [profile {prof.name}]")
     _check_scope(scaling, None, (mat1, mat2, scale_a, scale_b, scale_result))
     _emit_maturity(prof, preset)
-    layout_std = mat1.is_contiguous() and mat2[0].t().is_contiguous()
-    plans = {}                                           # rows of a group -> (splits, scheme)
-    for m in sizes:
-        if m and m not in plans:
-            d = resolve_splitk(m, N, K, a_dtype=mat1.dtype, b_dtype=mat2.dtype, out_dtype=od, use_fast_accum=fast, profile=prof,
-                               splitk=splitk, layout_std=layout_std, dry=False)
-            plans[m] = (d.S, check_plan(preset, K, d.S, d.scheme, fast))
+    layout_std = mat1.is_contiguous() and w0.t().is_contiguous()
+
+    def plan_of(m):
+        d = resolve_splitk(m, N, K, a_dtype=mat1.dtype, b_dtype=mat2.dtype, out_dtype=od, use_fast_accum=fast, profile=prof, splitk=splitk,
+                           layout_std=layout_std, dry=False)
+        return d.S, check_plan(preset, K, d.S, d.scheme, fast)
+
+    # (splits, scheme) of the groups by their rows; a split given by the caller holds for all of them
+    if isinstance(splitk, str) and splitk == "auto":
+        plans = {m: plan_of(m) for m in set(sizes) if m}
+        split = any(S > 1 for S, _ in plans.values())
+    else:
+        plan = plan_of(T)
+        split = plan[0] > 1
+        plans = dict.fromkeys(sizes, plan) if split else None
     kernel = _kernel_choice(backend)
     dev = mat1.device
     _require_device(dev)
@@ -108,7 +118,7 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
     y = torch.empty((T, N), dtype=od, device=dev) if out is None else out
     ints = ctypes.c_int * E
     rows, splits, schemes = ints(*sizes), None, None
-    if any(S > 1 for S, _ in plans.values()):
+    if split:
         splits = ints(*[plans[m][0] if m else 1 for m in sizes])
         schemes = ints(*[_lib.SCHEME_CODES[plans[m][1]] if m else 0 for m in sizes])
     keep_r, pr = (None, None) if scale_result is None else _scalar_ptr(scale_result, dev)

@@ -165,6 +165,9 @@ def test_layouts():
     strided = torch.stack([sa, sb], 1)
     y = mm.grouped_scaled_mm(a2, w2.transpose(1, 2), torch.tensor(sizes), strided[:, 0], strided[:, 1], **kw)
     assert np.array_equal(bits(y), bits(want))
+    same = sa[:1].expand(E)                                          # one scale, expanded
+    y = mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, same, same, **kw)
+    assert np.array_equal(bits(y), bits(loop(ta, tw, sizes, same, same, **kw)))
     big = torch.full((T + 2, N + 7), 3.0, dtype=torch.bfloat16, device=DEV)
     out = big[1:T + 1, 4:N + 4]
     assert mm.grouped_scaled_mm(a2, w2.transpose(1, 2), sizes, sa, sb, out=out, profile="hopper", splitk=1) is out
