@@ -202,13 +202,19 @@ def _kernel_choice(backend: str) -> str:
     raise ValueError(f"unknown backend {backend!r}; expected one of {', '.join(BACKEND_NAMES)}")
 
 
+_SUPPORTED: set = set()            # indices of CUDA devices that were asked before and can run the kernels
+
+
 def _require_device(device: torch.device) -> None:
+    if device.type == "cuda" and device.index in _SUPPORTED:
+        return
     if device.type != "cuda":
         raise BackendUnavailableError(f"mmaemu_b200 runs on sm_100 CUDA devices only and has no CPU fallback; got "
                                       f"tensors on {device}")
     L = _lib.load()
     idx = device.index if device.index is not None else torch.cuda.current_device()
     _lib.check("mmb200_device_supported", L.mmb200_device_supported(idx))
+    _SUPPORTED.add(idx)
 
 
 # ---------------------------------------------------------------------------------------------------------------

@@ -625,14 +625,13 @@ static int grouped_run(const void* A, int64_t lda, int fmt_a, const void* B, int
       p.epilogue = p.patch_nonfinite = 1;
       p.group_stride_b = group_stride_b;
       p.sa_stride = sa_stride; p.sb_stride = sb_stride;
-      const size_t need = fused_bytes(p, nfma, m_splits, groups, E);
       const bool named = kernel == MMB200_KERNEL_FAST && !(mmb::staged_vector_supports(p, nfma) && !(group_stride_b & 15));
-      if (need && workspace_bytes >= need && !named) {
+      if (groups.any && !named) {
         int launches = 0;
-        const cudaError_t err = mmb::launch_grouped(p, nfma, m_splits, groups.use, E, workspace, workspace_bytes, st, &launches);
+        const cudaError_t err = mmb::launch_grouped(p, nfma, m_splits, groups.use, E, workspace, workspace_bytes, GROUPED_SCRATCH_LIMIT, st,
+                                                    &launches, &fused);
         g_launches.fetch_add(launches, std::memory_order_relaxed);
         if (err != cudaSuccess) return cuda_fail(err);
-        fused = true;
       }
     }
     if (!fused) {

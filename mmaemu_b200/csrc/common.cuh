@@ -355,11 +355,12 @@ cudaError_t launch_fast(const Params& p, int nfma, cudaStream_t stream);
 cudaError_t launch_umma(const Params& p, int nfma, cudaStream_t stream, int* launches);
 cudaError_t launch_umma_grouped(const Params& p, int nfma, cudaStream_t stream, int* launches);
 // Ragged groups with unsplit plans on the tensor cores: scratch bytes (0: not served; the caller goes group by group), and the
-// launch. `rows`: rows of each of the E groups, `use`: whether the launch takes the group (null: all of them). p: the operands,
-// K, N and formats of the call, p.M its rows.
+// launch (*served: whether it took the call; not with more than `most` bytes or without the scratch memory). `rows`: rows of
+// each of the E groups, `use`: whether the launch takes the group (null: all of them). p: the operands, K, N and formats of the
+// call, p.M its rows.
 size_t grouped_workspace_bytes(const Params& p, int nfma, const int* rows, const unsigned char* use, int E);
 cudaError_t launch_grouped(const Params& p, int nfma, const int* rows, const unsigned char* use, int E, void* workspace,
-                           size_t workspace_bytes, cudaStream_t stream, int* launches);
+                           size_t workspace_bytes, size_t most, cudaStream_t stream, int* launches, bool* served);
 bool fast_supports(const Params& p, int nfma);
 // Staged fast kernel: scratch bytes it needs for a shape (0: a shape it does not take), and the launch (pre-decode of both
 // operands, then the GEMM).

@@ -1611,9 +1611,10 @@ GroupedPlan grouped_plan(const Params& p, int nfma, const int* rows, const unsig
   const int k_tiles = (p.K + KT - 1) / KT, tiles_n = (p.N + BN - 1) / BN;
   const int chains = p.fast ? 1 : (k_tiles + 3) / 4;
   double least = 0.0;
+  const bool no_row_groups = env_off("MMAEMU_B200_ROW_GROUPS"), no_slices = env_off("MMAEMU_B200_SLICES");
   const int choices[] = {16, 32, 64, 0x7FFFFFFF};
   for (int few : choices) {
-    if (few > 16 && env_off("MMAEMU_B200_ROW_GROUPS")) break;
+    if (few > 16 && no_row_groups) break;
     GroupedPlan g;
     g.few = few;
     g.tiles_n = tiles_n;
@@ -1641,7 +1642,7 @@ GroupedPlan grouped_plan(const Params& p, int nfma, const int* rows, const unsig
     if (g.n16) {
       const long long ctas = g.n16 * tiles_n;
       double t16 = kt.waves16(ctas, sms) * k_tiles;
-      long long s = env_off("MMAEMU_B200_SLICES") ? 1 : SLICE_CTA_TARGET / ctas;
+      long long s = no_slices ? 1 : SLICE_CTA_TARGET / ctas;
       s = s > MMB200_MAX_SLICES ? MMB200_MAX_SLICES : s;
       s = s > chains ? chains : s;
       if (s > 1 && (size_t)ctas * chains * 2 * TN * THREADS * sizeof(float) <= SLICE_SCRATCH_LIMIT) {
@@ -1679,10 +1680,12 @@ size_t grouped_workspace_bytes(const Params& p, int nfma, const int* rows, const
 }
 
 cudaError_t launch_grouped(const Params& p_in, int nfma, const int* rows, const unsigned char* use, int E, void* workspace,
-                           size_t workspace_bytes, cudaStream_t stream, int* launches) {
+                           size_t workspace_bytes, size_t most, cudaStream_t stream, int* launches, bool* served) {
   Params p = p_in;
+  *served = false;
   const GroupedPlan g = grouped_plan(p, nfma, rows, use, E);
-  if (!g.total || !workspace || workspace_bytes < g.total || (reinterpret_cast<uintptr_t>(workspace) & 127)) return cudaErrorInvalidValue;
+  if (!g.total || g.total > most || !workspace || workspace_bytes < g.total || (reinterpret_cast<uintptr_t>(workspace) & 127)) return cudaSuccess;
+  *served = true;
   unsigned char* base = static_cast<unsigned char*>(workspace);
   p.status = reinterpret_cast<int*>(base);
   p.ws_flag_a = reinterpret_cast<int*>(base + g.flag_a);

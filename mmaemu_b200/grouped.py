@@ -17,7 +17,7 @@ from . import _lib
 from .api import (_check_argument_types, _check_like_cublas, _check_like_torch, _check_scope, _emit_maturity, _kernel_choice,
                   _kernel_code, _on_device, _require_device, _scalar_ptr, _stream_ptr)
 from .errors import ReferenceRejectsError
-from .formats import OUT_DTYPE_NAMES, fmt_of
+from .formats import E5M2, NAME_OF, OUT_DTYPE_NAMES, fmt_of
 from .numerics import check_plan, get_preset
 from .platforms import get_profile
 from .splitk import resolve_splitk
@@ -25,6 +25,7 @@ from .splitk import resolve_splitk
 __all__ = ["grouped_scaled_mm"]
 
 MAX_GROUPS = 4096
+_PLAIN_OUT = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _sizes(m_splits, E: int, T: int) -> list:
@@ -54,6 +55,20 @@ def _group_scale(name: str, t: torch.Tensor, E: int) -> int:
     return t.stride(0)
 
 
+def _plainly_valid(input, mat2, scale_a, scale_b, scale_result, out_dtype, out) -> bool:
+    """Whether the checks of a scaled_mm call would let every group pass as it is, seen from the whole call: the usual layouts
+    and dtypes. False says nothing; the checks themselves decide then (15 us more)."""
+    if input.dim() != 2 or scale_result is not None or out is not None or out_dtype not in _PLAIN_OUT or input.dtype not in NAME_OF or \
+            mat2.dtype not in NAME_OF or (input.dtype == E5M2 and mat2.dtype == E5M2):
+        return False
+    (T, K), (E, K2, N) = input.shape, mat2.shape
+    (lda, unit), (gsb, unit2, ldb) = input.stride(), mat2.stride()
+    index = input.get_device()
+    return (K == K2 and K % 16 == 0 and N % 16 == 0 and T > 1 and N > 1 and K > 1 and unit == 1 and unit2 == 1 and lda >= K and ldb >= K
+            and not (lda | ldb | gsb | input.data_ptr() | mat2.data_ptr()) & 15 and index >= 0 and index == mat2.get_device()
+            and index == scale_a.get_device() and index == scale_b.get_device() and scale_a.dtype == scale_b.dtype == torch.float32)
+
+
 def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None, out_dtype=None, use_fast_accum=False, *,
                       out=None, profile=None, splitk="auto", backend="auto"):
     """scaled_mm of every group of rows, bit for bit: the first m_splits[0] rows of input [T, K] with mat2[0], the next
@@ -74,10 +89,13 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
         raise ValueError(f"grouped_scaled_mm(): between 1 and {MAX_GROUPS} groups, got {E}")
     sizes = _sizes(m_splits, E, T)
     sa, sb = _group_scale("scale_a", scale_a, E), _group_scale("scale_b", scale_b, E)
-    w0 = mat2[0]
-    scaling, od = _check_like_torch(input, w0, scale_a if scale_a.numel() == 1 else scale_a[:1],
-                                    scale_b if scale_b.numel() == 1 else scale_b[:1], None, scale_result,
-                                    out_dtype, out)
+    plain = _plainly_valid(input, mat2, scale_a, scale_b, scale_result, out_dtype, out)
+    if plain:
+        scaling, od = "tensorwise", out_dtype
+    else:
+        w0 = mat2[0]
+        scaling, od = _check_like_torch(input, w0, scale_a if scale_a.numel() == 1 else scale_a[:1],
+                                        scale_b if scale_b.numel() == 1 else scale_b[:1], None, scale_result, out_dtype, out)
     prof = get_profile(profile)
     preset = get_preset(prof.preset)
     if out is not None and (tuple(out.shape) != (T, N) or (N > 1 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N)):
@@ -85,7 +103,7 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
                          f"strides {tuple(out.stride())}")
     if T == 0 or N == 0 or K == 0:
         return torch.zeros((T, N), dtype=od, device=input.device) if out is None else out.zero_()
-    mat1 = _check_like_cublas(input, w0, scaling, od)
+    mat1 = input if plain else _check_like_cublas(input, w0, scaling, od)
     if E > 1 and mat2.stride(0) % 16:
         raise ReferenceRejectsError("CUBLAS_STATUS_NOT_SUPPORTED when calling cublasLtMatmul (operand pointer not 16-byte aligned)")
     fa, fb = fmt_of(mat1.dtype), fmt_of(mat2.dtype)
@@ -94,7 +112,7 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
         raise ReferenceRejectsError(f"{rule.message} [profile {prof.name}]")
     _check_scope(scaling, None, (mat1, mat2, scale_a, scale_b, scale_result))
     _emit_maturity(prof, preset)
-    layout_std = mat1.is_contiguous() and w0.t().is_contiguous()
+    layout_std = mat1.is_contiguous() and mat2.stride(1) == 1 and (mat2.stride(2) == K or N == 1)
 
     def plan_of(m):
         d = resolve_splitk(m, N, K, a_dtype=mat1.dtype, b_dtype=mat2.dtype, out_dtype=od, use_fast_accum=fast, profile=prof, splitk=splitk,
@@ -102,7 +120,10 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
         return d.S, check_plan(preset, K, d.S, d.scheme, fast)
 
     # (splits, scheme) of the groups by their rows; a split given by the caller holds for all of them
-    if isinstance(splitk, str) and splitk == "auto":
+    split, plans = False, None
+    if type(splitk) is int and splitk == 1:
+        check_plan(preset, K, 1, "none", fast)
+    elif isinstance(splitk, str) and splitk == "auto":
         plans = {m: plan_of(m) for m in set(sizes) if m}
         split = any(S > 1 for S, _ in plans.values())
     else:
@@ -112,10 +133,9 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
     kernel = _kernel_choice(backend)
     dev = mat1.device
     _require_device(dev)
-    a, w = mat1.detach(), mat2.detach()
-    lda = a.stride(0) if T > 1 else K
-    ldb = w.stride(2) if N > 1 else K
-    y = torch.empty((T, N), dtype=od, device=dev) if out is None else out
+    lda = mat1.stride(0) if T > 1 else K
+    ldb = mat2.stride(2) if N > 1 else K
+    y = input.new_empty((T, N), dtype=od) if out is None else out
     ints = ctypes.c_int * E
     rows, splits, schemes = ints(*sizes), None, None
     if split:
@@ -130,13 +150,13 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
                                                      int(fast)))
             if n:
                 try:
-                    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+                    ws = input.new_empty(n, dtype=torch.uint8)
                     ws_ptr = ws.data_ptr()
                 except torch.OutOfMemoryError:
                     if kernel != "auto":
                         raise                            # a request for the fast kernels by name
                     n = 0
-        rc = L.mmb200_grouped_scaled_mm(a.data_ptr(), lda, _lib.FMT_CODES[fa], w.data_ptr(), ldb, w.stride(0) if E > 1 else 0,
+        rc = L.mmb200_grouped_scaled_mm(mat1.data_ptr(), lda, _lib.FMT_CODES[fa], mat2.data_ptr(), ldb, mat2.stride(0) if E > 1 else 0,
                                         _lib.FMT_CODES[fb], y.data_ptr(), y.stride(0) if T > 1 else N,
                                         _lib.OUT_CODES[OUT_DTYPE_NAMES[od]], rows, splits, schemes, E, N, K, preset.code, int(fast),
                                         scale_a.data_ptr(), sa, scale_b.data_ptr(), sb, pr, _kernel_code(kernel), ws_ptr, n,

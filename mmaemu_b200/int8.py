@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .api import _STAY, _require_device
+from .api import _STAY, _SUPPORTED, _require_device
 from .errors import UnsupportedFeatureError
 
 __all__ = ["quantize_int8", "int8_scaled_mm", "int8_grouped_scaled_mm"]
@@ -29,12 +29,6 @@ MAX_ROWS = 1 << 23
 MAX_GROUPS = 4096
 _REAL_CODES = {torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}           # MMB200_HP_*
 _OUT_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # MMB200_OUT_*
-_supported: set = set()            # indices of devices that have been checked
-
-
-def _device(t: torch.Tensor) -> None:
-    _require_device(t.device)
-    _supported.add(t.get_device())
 
 
 def _not_a_tensor(who: str, name: str, t) -> TypeError:
@@ -63,8 +57,8 @@ def quantize_int8(x):
     if x.requires_grad and torch.is_grad_enabled():
         raise _no_grad("quantize_int8")
     index = x.get_device()
-    if index not in _supported:
-        _device(x)
+    if index not in _SUPPORTED:
+        _require_device(x.device)
     K = shape[-1]
     rows, n = x, shape[0]
     if len(shape) != 2:
@@ -207,8 +201,8 @@ def int8_scaled_mm(input, mat2, scale_a, scale_b, bias=None, out_dtype=None, *, 
     if bias is not None:
         bias, bias_code = _bias(who, bias, (N,))
     y, ldd, code = _output(who, input, out, out_dtype, M, N)
-    if index not in _supported:
-        _device(input)
+    if index not in _SUPPORTED:
+        _require_device(input.device)
     if M == 0 or N == 0:
         return y
     a, lda = _rows_of(input, M, K)
@@ -259,8 +253,8 @@ def int8_grouped_scaled_mm(input, mat2, offs, scale_a, scale_b, bias=None, out_d
     if bias is not None:
         bias, bias_code = _bias(who, bias, (E, N))
     y, ldd, code = _output(who, input, out, out_dtype, T, N)
-    if index not in _supported:
-        _device(input)
+    if index not in _SUPPORTED:
+        _require_device(input.device)
     if T == 0 or N == 0:
         return y
     if E == 0:
