@@ -746,8 +746,9 @@ Choice choose(const Int8Params& p) {
     if (kind == TILE && most_row_tiles(p, rows) > 65535) return;          // grid y
     const int ctas_per_tile = kind == PAIR ? 2 : 1, occupancy = kind == TILE ? 2 : 1;
     const long long tiles_n = ((long long)p.N + CH * ctas_per_tile - 1) / (CH * ctas_per_tile);
-    // every group ends in a tile that is half full on average
-    const double tiles_t = p.offs ? (double)p.T / rows + 0.5 * used : (double)(((long long)p.T + rows - 1) / rows);
+    // every group has a tile, and ends in one that is half full on average
+    const double ragged = (double)p.T / rows + 0.5 * used;
+    const double tiles_t = !p.offs ? (double)(((long long)p.T + rows - 1) / rows) : ragged > used ? ragged : (double)used;
     const double tiles = tiles_t * tiles_n, workers = (double)(n_sm / ctas_per_tile);
     auto waves = [](double n, double at_once) { return n <= at_once ? 1.0 : (double)(long long)(n / at_once + 0.999); };
     // rows that a tile copies: its own, a one-tile CTA all

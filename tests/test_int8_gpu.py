@@ -74,7 +74,7 @@ KERNELS = [((0, 16, 1), 40, 300, 100), ((0, 16, 2), 1, 5000, 2000), ((0, 16, 4),
            ((0, 64, 1), 33, 20000, 17), ((0, 64, 2), 3000, 16, 5000), ((0, 64, 4), 1500, 16, 2000), ((0, 64, 8), 700, 16, 5000),
            ((1, 64, 1), 65, 20000, 130), ((1, 128, 1), 1000, 2064, 1936), ((1, 128, 1), 1030, 5000, 300), ((1, 256, 1), 5000, 500, 1000),
            ((2, 256, 1), 2050, 5000, 300), ((2, 256, 1), 2000, 8200, 528)]
-RAGGED = [((0, 16, 8), [0, 33, 0, 1], 16, 5000), ((0, 64, 1), [16, 0, 5], 20000, 40), ((1, 64, 1), [25, 0, 70, 3] * 10, 2000, 500),
+RAGGED = [((0, 16, 8), [0, 33, 0, 1], 16, 5000), ((0, 32, 8), [100, 0, 200], 16, 5000), ((0, 64, 1), [60, 0, 40], 9000, 16), ((1, 64, 1), [25, 0, 70, 3] * 10, 2000, 500),
           ((1, 128, 1), [300, 0, 1, 128, 129, 900, 42, 600], 4100, 300), ((1, 256, 1), [3, 257, 256, 0, 484, 0, 0, 0], 2000, 1000),
           ((2, 256, 1), [1, 800, 256, 0, 1300, 33, 1610], 2050, 1040)]
 
