@@ -320,8 +320,8 @@ struct Epilogue {
 // ---------------------------------------------------------------------------------------------------------------
 // Programmatic dependent launch: a kernel launched this way starts while the previous one of the stream is still running, and
 // every thread of it waits, before its first access to memory, until that has completed -- so a kernel is never complete before
-// its predecessors are. The next kernel may start as soon as every CTA of this one has called dependent_launch_next; a kernel
-// with tensor memory does so after its allocation, so that the next one cannot take what it still needs.
+// its predecessors are. The next kernel may start as soon as every CTA of this one has called dependent_launch_next. Tensor memory
+// is allocated between the two: a kernel that waits holds none, and the next one cannot take what this one still needs.
 __device__ __forceinline__ void dependent_launch_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void dependent_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // cluster: CTAs per cluster (0: the kernel's own).

@@ -250,11 +250,11 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
     mbar_init(&sm.done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  dependent_launch_wait();
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "n"(COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  dependent_launch_wait();
   if (warp == 2) {
     const Group found = find_group<BT>(p, (int)blockIdx.y);
     if (lane == 0) sm.group = found;
@@ -463,6 +463,7 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
     mbar_init(&sm.drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  dependent_launch_wait();
   if (warp == 1) {
     if constexpr (CTAS == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "n"(W::COLS) : "memory");
@@ -479,7 +480,6 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
     cluster_wait();
   }
   fence_after();
-  dependent_launch_wait();
   dependent_launch_next();
   const uint32_t tmem = sm.tmem;
   bool ok = true;

@@ -147,6 +147,43 @@ def test_environment_switches(env, sizes, monkeypatch):
         check(ta, tw, sizes, *group_scales(len(sizes)), out_dtype=torch.bfloat16, profile="hopper", splitk=1, use_fast_accum=fast)
 
 
+def test_late_accumulator_profile():
+    """The experimental preset runs group by group on the integer kernel; slow accumulation is refused as in scaled_mm."""
+    sizes = [5, 0, 30]
+    _, _, ta, tw = operands(sizes, 48, 256, seed=15)
+    kw = dict(out_dtype=torch.bfloat16, profile="b200-mma-sync-experimental", splitk=1)
+    check(ta, tw, sizes, *group_scales(3), use_fast_accum=True, **kw)
+    with pytest.raises(mm.UnsupportedFeatureError), warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, *group_scales(3), **kw)
+
+
+def test_many_groups():
+    """More groups than one launch of the list kernel takes (512)."""
+    rng = np.random.default_rng(16)
+    sizes = [int(m) for m in rng.integers(0, 4, 1100)]
+    sizes[700] = 40
+    _, _, ta, tw = operands(sizes, 16, 64, seed=17)
+    sa, sb = group_scales(len(sizes))
+    y = mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, out_dtype=torch.bfloat16, profile="hopper", splitk=1)
+    z = mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, out_dtype=torch.bfloat16, profile="hopper", splitk=1,
+                             backend="cuda:b200-integer")
+    assert np.array_equal(bits(y), bits(z))
+
+
+@pytest.mark.parametrize("fast", [True, False])
+@pytest.mark.parametrize("profile,fa", [("hopper", "e4m3"), ("hopper", "e5m2"), ("ada", "e4m3"), ("ada", "e5m2")])
+def test_wide_outputs_and_mixed_sizes(profile, fa, fast):
+    """Enough tiles for 256 columns per CTA, groups of few rows beside long ones."""
+    sizes = [700, 3, 0, 128, 16, 300, 33, 900]
+    _, _, ta, tw = operands(sizes, 2064, 144, fa=fa, seed=18)
+    sa, sb = group_scales(8)
+    y = mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, out_dtype=torch.float32, profile=profile, splitk=1, use_fast_accum=fast)
+    z = mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, out_dtype=torch.float32, profile=profile, splitk=1, use_fast_accum=fast,
+                             backend="cuda:b200-integer")
+    assert np.array_equal(bits(y), bits(z))
+
+
 def test_layouts():
     """Row strides of both operands, a group stride that leaves gaps, an input that is a view; out= with a row stride."""
     sizes, N, K = [5, 0, 140, 30], 144, 272

@@ -7,6 +7,10 @@ the product of the scales (2^-24), the fused multiply-add (2^-24) and the output
     |y - y64| <= eps_out / 2 |y64| + 3 * 2^-24 (|acc sa sb| + |y64|), and a little for the products of these errors."""
 import ctypes
 import math
+import subprocess
+import sys
+import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -198,7 +202,10 @@ def test_empty_sizes():
     bias = torch.arange(24, device=DEV, dtype=torch.float32)
     y = mm.int8_scaled_mm(codes(20, 0), codes(24, 0).t(), one, one, bias, torch.float32)
     assert torch.equal(y, bias.expand(20, 24))                       # an empty sum is zero
-    assert not mm.int8_scaled_mm(codes(300, 0), codes(24, 0).t(), one, one).any()
+    for M, N in ((300, 24), (1000, 2064), (2050, 5000)):
+        assert not mm.int8_scaled_mm(codes(M, 0), codes(N, 0).t(), one, one).any()
+    ends = torch.tensor([3, 900], dtype=torch.int32, device=DEV)
+    assert not mm.int8_grouped_scaled_mm(codes(1000, 0), codes(2, 2000, 0).transpose(1, 2), ends, one, one).any()
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -433,6 +440,81 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         got = y.clone()
         same(got, step())
+
+
+FRESH = """
+import torch, mmaemu_b200 as mm
+dev = torch.device("cuda:0")
+x = torch.randn(70, 256, device=dev, dtype=torch.bfloat16)
+w = torch.randint(-127, 128, (3, 192, 256), device=dev).to(torch.int8)
+big = torch.randint(-127, 128, (2064, 256), device=dev).to(torch.int8)
+ends = torch.tensor([20, 20, 70], dtype=torch.int32, device=dev)
+one = torch.full((1,), 0.01, device=dev)
+f8 = torch.float8_e4m3fn
+xa, wa = x.to(f8), w.to(torch.bfloat16).to(f8)
+xb = torch.randint(-127, 128, (1000, 256), device=dev).to(torch.int8)
+def step():
+    xq, sx = mm.quantize_int8(x)
+    return (mm.int8_grouped_scaled_mm(xq, w.transpose(1, 2), ends, sx, one), mm.int8_scaled_mm(xq, w[0].t(), sx, one),
+            mm.int8_scaled_mm(xb, big.t(), one, one),
+            mm.grouped_scaled_mm(xa, wa.transpose(1, 2), [20, 0, 50], one, one, None, torch.bfloat16, profile="hopper", splitk=1))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("same")
+"""
+
+
+def test_the_first_calls_of_a_process_can_be_captured():
+    """Nothing that a first call looks up or sets breaks a capture."""
+    root = Path(__file__).resolve().parents[1]
+    r = subprocess.run([sys.executable, "-c", FRESH], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("same"), r.stderr[-2000:]
+
+
+def test_calls_on_two_streams_at_once():
+    """Two threads on streams of their own, every kind of kernel: no call sees the other's scratch memory or barriers."""
+    shapes = [(7, 130, 2001), (65, 2000, 130), (300, 1000, 333), (1000, 2064, 520)]
+    work = [(codes(M, K, seed=i), codes(N, K, seed=i + 9), scales(M, 1, seed=i), scales(1, N, seed=i + 1)) for i, (M, N, K) in enumerate(shapes)]
+    want = [want_bits(*w, torch.bfloat16) for w in work]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[k] = [[mm.int8_scaled_mm(a, w.t(), sa, sb) for a, w, sa, sb in work] for _ in range(20)]
+        stream.synchronize()
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(2):
+        for round_ in got[k]:
+            for y, w in zip(round_, want):
+                same(y, w)
+
+
+@pytest.mark.parametrize("M,N,K", [(4, 512, 2048)])
+def test_status_check_after_every_call(M, N, K, monkeypatch):
+    """$MMAEMU_B200_CHECK_STATUS=1: the call itself raises."""
+    monkeypatch.setenv("MMAEMU_B200_CHECK_STATUS", "1")
+    a, w, one = codes(M, K, seed=1), codes(N, K, seed=2), torch.ones(1, device=DEV)
+    want = mm.int8_scaled_mm(a, w.t(), one, one)
+    L = _lib.load()
+    L.mmb200_test_hooks(200, 16)
+    try:
+        with pytest.raises(_lib.NativeError) as e:
+            mm.int8_scaled_mm(a, w.t(), one, one)
+        assert e.value.status == _lib.ERR_TIMEOUT
+    finally:
+        L.mmb200_test_hooks(0, 0)
+    same(mm.int8_scaled_mm(a, w.t(), one, one), want)
 
 
 @pytest.mark.parametrize("M,N,K", [(4, 512, 2048), (100, 512, 2048), (400, 512, 2048), (65, 20000, 1300), (1000, 2064, 1936), (5000, 500, 1000),
