@@ -76,9 +76,20 @@ __device__ __forceinline__ uint32_t code_at_border(float x, const RowScale& r) {
   const int c = q + (twice > mid || (twice == mid && (q & 1)) ? 1 : 0);
   return (uint32_t)(x < 0.0f ? -c : c);
 }
+// Two fp32 FMAs in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long x, y, z, d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(z) : "f"(c.x), "f"(c.y));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
+}
 // The codes of N values, packed. In [2^23, 2^24) one ulp is 1, so RN(x inv + 1.5 * 2^23) holds the nearest integer in its
-// low bits (ties to even, two's complement): four instructions per value, none on the quarter-rate conversion pipe. `off`
-// collects the largest distance from the integer, so that borders cost one test per vector.
+// low bits (ties to even, two's complement): two and a half instructions per value, none on the quarter-rate conversion pipe.
+// `off` collects the largest distance from the integer, so that borders cost one test per vector.
 template <int N>
 __device__ __forceinline__ void codes_of(float (&x)[N], const RowScale& r, uint32_t (&w)[N / 4]) {
   constexpr float MAGIC = 12582912.0f, NEAR = 0.49998f;
@@ -88,11 +99,14 @@ __device__ __forceinline__ void codes_of(float (&x)[N], const RowScale& r, uint3
 #pragma unroll
     for (int q = 0; q < N; ++q) x[q] = __fmul_rn(x[q], RAISE);
   }
+  const float2 inv = make_float2(r.inv, r.inv), magic = make_float2(MAGIC, MAGIC), minus = make_float2(-1.0f, -1.0f);
 #pragma unroll
-  for (int q = 0; q < N; ++q) {
-    const float m = __fmaf_rn(x[q], r.inv, MAGIC);
-    off = fmaxf(off, fabsf(__fmaf_rn(x[q], r.inv, -__fsub_rn(m, MAGIC))));
-    b[q] = __float_as_uint(m);
+  for (int q = 0; q < N; q += 2) {
+    const float2 v = make_float2(x[q], x[q + 1]), m = fma2(v, inv, magic);
+    const float2 d = fma2(v, inv, fma2(m, minus, magic));          // x inv - (m - MAGIC); the difference is exact
+    off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
+    b[q] = __float_as_uint(m.x);
+    b[q + 1] = __float_as_uint(m.y);
   }
   if (off > NEAR) {
 #pragma unroll
