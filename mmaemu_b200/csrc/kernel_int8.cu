@@ -5,12 +5,20 @@
 // and the rows (tokens) its columns, so few rows make a narrow tile instead of an empty one, the channel's scale and bias are
 // one register per thread, and the stores of a warp cover 32 consecutive outputs of a row.
 //
-// int8_tile_kernel: one tile of 128 channels x BT rows per cluster; the CTAs of a cluster each take a part of K and add their
-// int32 sums through distributed shared memory. Integer sums are exact in any order, so the split changes no bit.
+// int8_tile_kernel: few rows. One tile of 128 channels x 16, 32 or 64 rows per cluster; the CTAs of a cluster each take a part of
+// K and add their int32 sums through distributed shared memory. Integer sums are exact in any order, so the split changes no
+// bit. Bound by reading the weights: 16 x 8192 x 28672 at 6.1 TB/s (38.5 us); 16 x 4096 x 8192 in 9.2 us, of which 3.5 are
+// launch, first copies and the cluster's sum (13 us more while a thread read the sums one by one).
 //
-// int8_pair_kernel: many rows. Two CTAs on neighbouring SMs (cta_group::2) work on a tile of 256 channels x 256 rows, each
-// holding half of both operands, so a byte of shared memory feeds twice the products; persistent, and TMEM holds two
-// accumulators, so the output of a tile leaves while the next one is multiplied.
+// int8_single_kernel, int8_pair_kernel: more rows. Persistent; TMEM holds two accumulators, so the output of a tile leaves while
+// the next one is multiplied. A CTA works on 128 channels x 64, 128 or 256 rows, a pair of CTAs on neighbouring SMs
+// (cta_group::2) on 256 x 256, each holding half of both operands, so that a byte of shared memory feeds twice the products.
+// Large products are bound by power: 8192 x 24576 x 8192 takes 1.13 ms, 2.9 POP/s, with operands of zeros 4.1 POP/s. 4096 rows
+// in 64 groups on 1536 x 2048 weights: 48 us for 201 MB of weights (one-tile CTAs: 55 us, and 66 with tiles of 128 rows).
+//
+// An MMA of 128 channels takes about 120 cycles up to 128 rows, so a CTA needs 0.25 us per 128 bytes of K however few rows it
+// has. The output loop must not wait: with a scale loaded per row instead of handed round by shuffles it took 27 us per tile
+// and was most of every product with K below 4096.
 #include <cuda.h>
 #include <cuda_fp16.h>
 

@@ -216,6 +216,37 @@ def test_layouts():
     assert np.array_equal(bits(y), bits(loop(ta, shared, sizes, sa, sb, **kw)))
 
 
+@pytest.mark.parametrize("K,lda,ldb,shift", [(67, 70, 69, 1), (400, 400, 401, 0), (128, 144, 128, 3), (1, 1, 1, 0)])
+@pytest.mark.parametrize("sizes", [[5, 0, 140, 30], [3, 1, 2]])
+def test_c_entry_point_takes_operands_of_any_alignment(K, lda, ldb, shift, sizes):
+    """K, leading dimensions, group stride and base addresses that no 16-byte load fits (the Python entry point refuses them, as
+    the emulated platform does)."""
+    N, E, T = 50, len(sizes), sum(sizes)
+    rng = np.random.default_rng(K)
+    a, w = datagen.codes(rng, T, K, "e4m3", "gauss40"), datagen.codes(rng, E * N, K, "e4m3", "gauss40", 1)
+    ha = torch.zeros(T * lda + 8, dtype=torch.uint8, device=DEV)
+    hw = torch.zeros(E * (N * ldb + 5) + 8, dtype=torch.uint8, device=DEV)
+    ha.as_strided((T, K), (lda, 1), shift).copy_(torch.from_numpy(a))
+    hw.as_strided((E, N, K), (N * ldb + 5, ldb, 1), shift).copy_(torch.from_numpy(w).view(E, N, K))
+    sa, sb = group_scales(E)
+    L = _lib.load()
+    ints = (ctypes.c_int * E)(*sizes)
+    for fast in (0, 1):
+        n = L.mmb200_grouped_workspace_bytes(ints, None, E, N, K, 0, 0, 32, fast)
+        ws = torch.empty(max(n, 1), dtype=torch.uint8, device=DEV)
+        y = torch.zeros(T, N, dtype=torch.float32, device=DEV)
+        rc = L.mmb200_grouped_scaled_mm(ha.data_ptr() + shift, lda, 0, hw.data_ptr() + shift, ldb, N * ldb + 5, 0, y.data_ptr(), N, 0, ints, None,
+                                        None, E, N, K, 32, fast, sa.data_ptr(), 1, sb.data_ptr(), 1, None, 0, ws.data_ptr(), n,
+                                        ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        _lib.check("mmb200_grouped_scaled_mm", rc)
+        start = 0
+        for e, m in enumerate(sizes):
+            if m:
+                want = oracle.scaled_mm(a[start:start + m], w.reshape(E, N, K)[e], float(sa[e]), float(sb[e]), out="float32", preset="hopper", fast=bool(fast))
+                assert np.array_equal(bits(y[start:start + m]), want), (fast, e)
+            start += m
+
+
 def test_empty_results():
     one = torch.ones(1, device=DEV)
     f = torch.float8_e4m3fn
