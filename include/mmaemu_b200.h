@@ -244,8 +244,8 @@ size_t mmb200_grouped_workspace_bytes(const int *m_splits, const int *splits, in
 int mmb200_grouped_scaled_mm(const void *A_dev, int64_t lda, int fmt_a, const void *B_dev, int64_t ldb,
                              int64_t group_stride_b, int fmt_b, void *D_dev, int64_t ldd, int out_dtype,
                              const int *m_splits, const int *splits, const int *schemes, int E, int N, int K, int nfma,
-                             int fast, const float *scale_a_dev, int sa_stride, const float *scale_b_dev, int sb_stride,
-                             const float *scale_result_dev, int kernel, void *workspace_dev, size_t workspace_bytes,
+                             int fast, const float *scale_a_dev, int64_t sa_stride, const float *scale_b_dev,
+                             int64_t sb_stride, const float *scale_result_dev, int kernel, void *workspace_dev, size_t workspace_bytes,
                              void *stream);
 int mmb200_grouped_status(const void *workspace_dev, void *stream);
 
@@ -258,7 +258,7 @@ int mmb200_quantize_int8(const void *X_dev, int64_t ldx, int x_dtype, int8_t *co
                          int64_t rows, int K, void *stream);
 
 /* D[r][n] = out(fma(RN32(acc), RN32(sa sb), bias)), acc = sum_k A[r][k] W[g][n][k] (exact; K <= MMB200_INT8_MAX_K,
- * T <= MMB200_INT8_MAX_ROWS), rounded
+ * T <= MMB200_INT8_MAX_ROWS, N <= MMB200_INT8_MAX_N), rounded
  * to fp32 and then to out_dtype (F32, BF16 or F16; canonical NaN). A is [T, K] int8 with row stride lda, W [E, N, K] with row
  * stride ldw and group stride group_stride_w. sa = scale_a_dev[r * sa_stride], sb = scale_b_dev[g * sb_group_stride +
  * n * sb_stride], bias = bias_dev[g * bias_group_stride + n] of bias_dtype (MMB200_HP_*; bias_dev NULL: none).
@@ -268,12 +268,13 @@ int mmb200_quantize_int8(const void *X_dev, int64_t ldx, int x_dtype, int8_t *co
  * memory of mmb200_int8_workspace_bytes first (16-byte aligned; 0 bytes: none needed). */
 #define MMB200_INT8_MAX_K 131071
 #define MMB200_INT8_MAX_ROWS (1 << 23)
+#define MMB200_INT8_MAX_N (1 << 30)
 size_t mmb200_int8_workspace_bytes(const int8_t *A_dev, int64_t lda, const int8_t *W_dev, int64_t ldw,
                                    int64_t group_stride_w, int T, int N, int K, int E);
 int mmb200_int8_scaled_mm(const int8_t *A_dev, int64_t lda, const int8_t *W_dev, int64_t ldw, int64_t group_stride_w,
                           void *D_dev, int64_t ldd, int out_dtype, int T, int N, int K, int E, const int *offs_dev,
-                          const float *scale_a_dev, int sa_stride, const float *scale_b_dev, int64_t sb_group_stride,
-                          int sb_stride, const void *bias_dev, int bias_dtype, int64_t bias_group_stride, int zero_rest,
+                          const float *scale_a_dev, int64_t sa_stride, const float *scale_b_dev, int64_t sb_group_stride,
+                          int64_t sb_stride, const void *bias_dev, int bias_dtype, int64_t bias_group_stride, int zero_rest,
                           void *workspace_dev, size_t workspace_bytes, void *stream);
 /* The kernel that a call of this shape runs on: kind << 16 | rows of a tile << 4 | parts of K, kind 0: one tile per CTA (a
  * cluster of `parts` CTAs shares a tile), 1: persistent CTAs, 2: persistent pairs of CTAs. ragged: whether offs_dev is given.

@@ -106,8 +106,8 @@ def load():
         sz = ctypes.c_size_t
         L.mmb200_grouped_workspace_bytes.argtypes = [vp, vp, ci, ci, ci, ci, ci, ci, ci]
         L.mmb200_grouped_workspace_bytes.restype = sz
-        L.mmb200_grouped_scaled_mm.argtypes = [vp, i64, ci, vp, i64, i64, ci, vp, i64, ci, vp, vp, vp, ci, ci, ci, ci, ci, vp, ci,
-                                               vp, ci, vp, ci, vp, sz, vp]
+        L.mmb200_grouped_scaled_mm.argtypes = [vp, i64, ci, vp, i64, i64, ci, vp, i64, ci, vp, vp, vp, ci, ci, ci, ci, ci, vp, i64,
+                                               vp, i64, vp, ci, vp, sz, vp]
         L.mmb200_grouped_scaled_mm.restype = ci
         L.mmb200_grouped_status.argtypes = [vp, vp]
         L.mmb200_grouped_status.restype = ci
@@ -115,7 +115,7 @@ def load():
         L.mmb200_quantize_int8.restype = ci
         L.mmb200_int8_workspace_bytes.argtypes = [vp, i64, vp, i64, i64, ci, ci, ci, ci]
         L.mmb200_int8_workspace_bytes.restype = sz
-        L.mmb200_int8_scaled_mm.argtypes = [vp, i64, vp, i64, i64, vp, i64, ci, ci, ci, ci, ci, vp, vp, ci, vp, i64, ci, vp, ci,
+        L.mmb200_int8_scaled_mm.argtypes = [vp, i64, vp, i64, i64, vp, i64, ci, ci, ci, ci, ci, vp, vp, i64, vp, i64, i64, vp, ci,
                                             i64, ci, vp, sz, vp]
         L.mmb200_int8_scaled_mm.restype = ci
         L.mmb200_int8_kernel_for.argtypes = [ci, ci, ci, ci, ci]

@@ -590,7 +590,7 @@ int mmb200_grouped_status(const void* workspace, void* stream) {
 
 static int grouped_run(const void* A, int64_t lda, int fmt_a, const void* B, int64_t ldb, int64_t group_stride_b, int fmt_b, void* D,
                        int64_t ldd, int out_dtype, const int* m_splits, const int* splits, const int* schemes, int E, int N, int K,
-                       int nfma, int fast, const float* scale_a, int sa_stride, const float* scale_b, int sb_stride,
+                       int nfma, int fast, const float* scale_a, int64_t sa_stride, const float* scale_b, int64_t sb_stride,
                        const float* scale_result, int kernel, void* workspace, size_t workspace_bytes, void* stream) {
   if (E < 0 || N < 0 || K < 0 || (E > 0 && !m_splits) || !splits != !schemes) return MMB200_ERR_BAD_ARG;
   if (E > MMB200_MAX_GROUPS) return MMB200_ERR_TOO_LARGE;
@@ -662,8 +662,8 @@ static int grouped_run(const void* A, int64_t lda, int fmt_a, const void* B, int
 
 int mmb200_grouped_scaled_mm(const void* A, int64_t lda, int fmt_a, const void* B, int64_t ldb, int64_t group_stride_b, int fmt_b,
                              void* D, int64_t ldd, int out_dtype, const int* m_splits, const int* splits, const int* schemes,
-                             int E, int N, int K, int nfma, int fast, const float* scale_a, int sa_stride, const float* scale_b,
-                             int sb_stride, const float* scale_result, int kernel, void* workspace, size_t workspace_bytes,
+                             int E, int N, int K, int nfma, int fast, const float* scale_a, int64_t sa_stride, const float* scale_b,
+                             int64_t sb_stride, const float* scale_result, int kernel, void* workspace, size_t workspace_bytes,
                              void* stream) {
   try {                                      // the lists of K slices are host memory
     return grouped_run(A, lda, fmt_a, B, ldb, group_stride_b, fmt_b, D, ldd, out_dtype, m_splits, splits, schemes, E, N, K, nfma, fast,
@@ -705,15 +705,15 @@ size_t mmb200_int8_workspace_bytes(const int8_t* A, int64_t lda, const int8_t* W
 }
 
 int mmb200_int8_scaled_mm(const int8_t* A, int64_t lda, const int8_t* W, int64_t ldw, int64_t group_stride_w, void* D, int64_t ldd,
-                          int out_dtype, int T, int N, int K, int E, const int* offs, const float* scale_a, int sa_stride,
-                          const float* scale_b, int64_t sb_group_stride, int sb_stride, const void* bias, int bias_dtype,
+                          int out_dtype, int T, int N, int K, int E, const int* offs, const float* scale_a, int64_t sa_stride,
+                          const float* scale_b, int64_t sb_group_stride, int64_t sb_stride, const void* bias, int bias_dtype,
                           int64_t bias_group_stride, int zero_rest, void* workspace, size_t workspace_bytes, void* stream) {
   if (T < 0 || N < 0 || K < 0 || E < 1 || (!offs && E != 1)) return MMB200_ERR_BAD_ARG;
   if (out_dtype < MMB200_OUT_F32 || out_dtype > MMB200_OUT_F16) return MMB200_ERR_BAD_ARG;
   if (bias && (bias_dtype < MMB200_HP_F32 || bias_dtype > MMB200_HP_F16)) return MMB200_ERR_BAD_ARG;
   if (!scale_a || !scale_b || sa_stride < 0 || sb_stride < 0 || sb_group_stride < 0 || bias_group_stride < 0 || group_stride_w < 0)
     return MMB200_ERR_BAD_ARG;
-  if (K > MMB200_INT8_MAX_K || T > MMB200_INT8_MAX_ROWS || E > MMB200_MAX_GROUPS) return MMB200_ERR_TOO_LARGE;
+  if (K > MMB200_INT8_MAX_K || T > MMB200_INT8_MAX_ROWS || N > MMB200_INT8_MAX_N || E > MMB200_MAX_GROUPS) return MMB200_ERR_TOO_LARGE;
   if (T == 0 || N == 0) return MMB200_OK;
   if (!D || (T > 1 && ldd < N)) return MMB200_ERR_BAD_ARG;
   if (K > 0 && (!A || !W || (T > 1 && lda < K) || (N > 1 && ldw < K))) return MMB200_ERR_BAD_ARG;

@@ -94,8 +94,7 @@ struct Params {
   const RowTile* ws_tiles;       // [tiles_m]
   const int* ws_slots;           // group of every decoded B
   int slots;                     // decoded Bs
-  long long group_stride_b;
-  int sa_stride, sb_stride;
+  long long group_stride_b, sa_stride, sb_stride;
 };
 
 // One tile of rows of a grouped launch: rows [m0, m_end) of group g, whose flags (and decoded tiles) of B are number `slot`.

@@ -28,9 +28,8 @@ struct Int8Params {
   const void* bias;       // null, or [E, N] (group stride bias_group)
   const int* offs;        // ends of the groups [E]; null: one group of all T rows
   int* status;            // device word: 1 when a bounded wait ran out
-  long long lda, ldw, gsw, ldd, sb_group, bias_group;
+  long long lda, ldw, gsw, ldd, sa_stride, sb_stride, sb_group, bias_group;
   int T, N, K, E;
-  int sa_stride, sb_stride;
   int bias_dtype, out_dtype;
   int zero_rest;          // rows behind the last group are set to zero
   int k_blocks, tiles_n, tiles_t;       // set by the launcher

@@ -181,40 +181,53 @@ __device__ __forceinline__ void write_sums(const Int8Params& p, const int* part,
 
 // ---- groups. Ends are taken as a running maximum, clamped to [0, T], so that no content of offs leads out of the operands.
 struct Group { int g, start, end, tile, last; };       // g < 0: no such tile; last: the end of the last group
-// The group of tile `slot` of BT rows, found by one warp (every lane returns it).
+// 32 groups at a time, one per lane of a warp: rows [start, end) and the tiles of BT rows up to the group's last. `last`: the end
+// of the groups before the chunk; `tiles`: their tiles.
 template <int BT>
-__device__ __forceinline__ Group find_group(const Int8Params& p, int slot) {
-  if (!p.offs) return Group{0, 0, p.T, slot, p.T};
-  const int lane = threadIdx.x % 32;
-  int tiles = 0, last = 0;
-  Group r{-1, 0, 0, 0, 0};
-  for (int base = 0; base < p.E; base += 32) {
-    int end = base + lane < p.E ? min(max(__ldg(p.offs + base + lane), 0), p.T) : 0;
+struct GroupChunk {
+  int start, end, upto;
+  __device__ __forceinline__ void load(const Int8Params& p, int base, int last, int tiles) {
+    const int lane = threadIdx.x % 32;
+    end = !p.offs ? p.T : base + lane < p.E ? min(max(__ldg(p.offs + base + lane), 0), p.T) : 0;
+    end = max(end, last);
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
       const int other = __shfl_up_sync(0xFFFFFFFFu, end, d);
       if (lane >= d) end = max(end, other);
     }
-    end = max(end, last);
-    int start = __shfl_up_sync(0xFFFFFFFFu, end, 1);
+    start = __shfl_up_sync(0xFFFFFFFFu, end, 1);
     if (lane == 0) start = last;
-    int upto = (end - start + BT - 1) / BT;
+    upto = (end - start + BT - 1) / BT + (lane == 0 ? tiles : 0);
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
       const int other = __shfl_up_sync(0xFFFFFFFFu, upto, d);
       if (lane >= d) upto += other;
     }
-    upto += tiles;
-    const unsigned after = __ballot_sync(0xFFFFFFFFu, upto > slot);
-    if (after && r.g < 0) {
+  }
+};
+// The group of tile `slot` of BT rows, found by one warp (every lane returns it).
+template <int BT>
+__device__ __forceinline__ Group find_group(const Int8Params& p, int slot) {
+  if (!p.offs) return Group{0, 0, p.T, slot, p.T};
+  int tiles = 0, last = 0, base = 0;
+  Group r{-1, 0, 0, 0, 0};
+  GroupChunk<BT> c;
+  for (; base < p.E && r.g < 0; base += 32) {
+    c.load(p, base, last, tiles);
+    const unsigned after = __ballot_sync(0xFFFFFFFFu, c.upto > slot);
+    if (after) {
       const int l = __ffs(after) - 1;
       r.g = base + l;
-      r.start = __shfl_sync(0xFFFFFFFFu, start, l);
-      r.end = __shfl_sync(0xFFFFFFFFu, end, l);
-      r.tile = slot - __shfl_sync(0xFFFFFFFFu, upto - (end - start + BT - 1) / BT, l);
+      r.start = __shfl_sync(0xFFFFFFFFu, c.start, l);
+      r.end = __shfl_sync(0xFFFFFFFFu, c.end, l);
+      r.tile = slot - __shfl_sync(0xFFFFFFFFu, c.upto - (c.end - c.start + BT - 1) / BT, l);
     }
-    tiles = __shfl_sync(0xFFFFFFFFu, upto, 31);
-    last = __shfl_sync(0xFFFFFFFFu, end, 31);
+    tiles = __shfl_sync(0xFFFFFFFFu, c.upto, 31);
+    last = __shfl_sync(0xFFFFFFFFu, c.end, 31);
+  }
+  if (p.zero_rest) {                         // the end of the last group
+    for (int e = base + threadIdx.x % 32; e < p.E; e += 32) last = max(last, min(max(__ldg(p.offs + e), 0), p.T));
+    last = __reduce_max_sync(0xFFFFFFFFu, last);
   }
   r.last = last;
   return r;
@@ -360,6 +373,8 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
 }
 
 // ---- persistent workers: one CTA per SM, or a pair of CTAs on neighbouring SMs
+// Ragged groups: the end of a group's rows and the tiles of BT rows up to it, in shared memory.
+struct GroupTable { int end, upto; };
 // A worker's tile is CH * CTAS channels x up to BT rows. In a pair each CTA holds its channels and half of the rows.
 template <int CTAS, int BT>
 struct Worker {
@@ -376,7 +391,9 @@ struct Worker {
     unsigned long long acc_empty[2];       // (first CTA) all output warps have read it
     unsigned long long drain;
     uint32_t tmem;
+    GroupTable groups[1];                  // as many as the launch has groups
   };
+  static size_t bytes(const Int8Params& p) { return sizeof(Smem) + 1024 + (p.offs ? sizeof(GroupTable) * (size_t)p.E : 0); }
 };
 constexpr int WORKER_THREADS = 320;        // warp 0: copies, warp 1: MMAs, warps 2 to 9: output (a quarter of the channels, half of the rows)
 constexpr int BAND_ROWS = 2048;            // rows that share a pass over the channels (16 MB of them at K = 8192 stay in L2)
@@ -424,23 +441,51 @@ __device__ __forceinline__ void commit_all(unsigned long long* bar) {        // 
                  ::"r"(smem_addr(bar)), "h"((uint16_t)3) : "memory");
 }
 
+// Written by one warp.
+template <int BT>
+__device__ __forceinline__ void write_groups(const Int8Params& p, GroupTable* table) {
+  const int lane = threadIdx.x % 32;
+  int tiles = 0, last = 0;
+  GroupChunk<BT> c;
+  for (int base = 0; base < p.E; base += 32) {
+    c.load(p, base, last, tiles);
+    if (base + lane < p.E) table[base + lane] = GroupTable{c.end, c.upto};
+    tiles = __shfl_sync(0xFFFFFFFFu, c.upto, 31);
+    last = __shfl_sync(0xFFFFFFFFu, c.end, 31);
+  }
+}
 // The tiles of a launch in order: group by group, inside a group bands of BAND_ROWS rows, inside a band channel tile by
 // channel tile. A worker walks an increasing sequence of indices; every role of a CTA has a walker of its own.
 template <int BT>
 struct Walker {
-  int g = -1, start = 0, end = 0, tiles_t = 0;
-  long long base = 0, count = 0;           // tiles before the group, tiles of the group
-  __device__ __forceinline__ bool find(const Int8Params& p, int tiles_n, long long t, int& row0, int& n_tile) {
+  int g = 0, end = 0;
+  __device__ __forceinline__ bool find(const Int8Params& p, const GroupTable* table, int tiles_n, long long t, int& row0, int& n_tile) {
     constexpr int BAND = BAND_ROWS / BT;
-    while (t >= base + count) {
-      base += count;
-      if (++g >= p.E) return false;
-      start = end;
-      end = p.offs ? max(end, min(max(__ldg(p.offs + g), 0), p.T)) : p.T;
-      tiles_t = (end - start + BT - 1) / BT;
-      count = (long long)tiles_t * tiles_n;
+    int start = 0, before = 0, upto;
+    if (p.offs) {
+      if ((long long)table[g].upto * tiles_n <= t) {       // the first group behind with more tiles up to it
+        int lo = g + 1, hi = p.E;
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if ((long long)table[mid].upto * tiles_n > t) hi = mid;
+          else lo = mid + 1;
+        }
+        if (lo >= p.E) return false;
+        g = lo;
+      }
+      if (g > 0) {
+        start = table[g - 1].end;
+        before = table[g - 1].upto;
+      }
+      end = table[g].end;
+      upto = table[g].upto;
+    } else {
+      end = p.T;
+      upto = (p.T + BT - 1) / BT;
+      if ((long long)upto * tiles_n <= t) return false;
     }
-    const long long i = t - base, per_band = (long long)BAND * tiles_n;
+    const int tiles_t = upto - before;
+    const long long i = t - (long long)before * tiles_n, per_band = (long long)BAND * tiles_n;
     const int band = (int)(i / per_band), j = (int)(i - band * per_band), width = min(BAND, tiles_t - band * BAND);
     n_tile = j / width;
     row0 = start + (band * BAND + j % width) * BT;
@@ -472,6 +517,7 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   dependent_launch_wait();
+  if (warp == 2 && p.offs) write_groups<BT>(p, sm.groups);
   if (warp == 1) {
     if constexpr (CTAS == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sm.tmem)), "n"(W::COLS) : "memory");
@@ -496,7 +542,7 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
   if (warp == 0) {
     if (lane == 0) {
       unsigned it = 0;
-      for (long long t = first; ok && walk.find(p, tiles_n, t, row0, n_tile); t += step) {
+      for (long long t = first; ok && walk.find(p, sm.groups, tiles_n, t, row0, n_tile); t += step) {
         const int mine = walk.template columns<CTAS>(row0) / CTAS, my_row = row0 + mine * rank, boxes = (mine + W::BOX - 1) / W::BOX;
         const uint32_t bytes = CTAS * (uint32_t)(sizeof(sm.stage[0].w) + boxes * W::BOX * KB);
         for (int kb = 0; kb < nk; ++kb, ++it) {
@@ -518,7 +564,7 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
     if (lane == 0 && rank == 0) {
       constexpr uint32_t SHAPE = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(CTAS * CH >> 4) << 24);
       unsigned it = 0, i = 0;
-      for (long long t = first; ok && walk.find(p, tiles_n, t, row0, n_tile); t += step, ++i) {
+      for (long long t = first; ok && walk.find(p, sm.groups, tiles_n, t, row0, n_tile); t += step, ++i) {
         const uint32_t acc = tmem + (i & 1) * BT, idesc = SHAPE | ((uint32_t)(walk.template columns<CTAS>(row0) >> 3) << 17);
         if (i >= 2 && !mbar_wait(&sm.acc_empty[i & 1], ((i >> 1) - 1) & 1, p.wait_polls)) { ok = false; break; }
         fence_after();
@@ -543,7 +589,7 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
     const int half = warp < 6 ? 0 : BT / 2;
     const uint32_t mine = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + half;
     unsigned i = 0;
-    for (long long t = first; walk.find(p, tiles_n, t, row0, n_tile); t += step, ++i) {
+    for (long long t = first; walk.find(p, sm.groups, tiles_n, t, row0, n_tile); t += step, ++i) {
       const int n = (CTAS * n_tile + rank) * CH + 32 * (warp % 4) + lane, rows = min(walk.end - row0 - half, BT / 2);
       const bool real = n < p.N;
       const float sb = real ? __ldg(p.scale_b + (long long)walk.g * p.sb_group + (long long)n * p.sb_stride) : 0.0f;
@@ -560,7 +606,8 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
         else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(first_cta<CTAS>(&sm.acc_empty[i & 1])) : "memory");
       }
     }
-    if (ok) zero_rows<OUT>(p, walk.end + (int)blockIdx.x, (int)gridDim.x, 0, p.N, threadIdx.x - 64, WORKER_THREADS - 64);   // (the walk has seen every group)
+    if (ok && p.zero_rest)
+      zero_rows<OUT>(p, sm.groups[p.E - 1].end + (int)blockIdx.x, (int)gridDim.x, 0, p.N, threadIdx.x - 64, WORKER_THREADS - 64);
   }
   if (!ok) atomicExch(p.status, 1);
   fence_before();
@@ -709,13 +756,14 @@ cudaError_t launch_worker(const Int8Params& p, const Maps& m, long long tiles, c
   void (*kern)(CUtensorMap, CUtensorMap, Int8Params);
   if constexpr (CTAS == 2) kern = int8_pair_kernel<OUT>;
   else kern = int8_single_kernel<BT, OUT>;
-  constexpr size_t SMEM = sizeof(typename Worker<CTAS, BT>::Smem) + 1024;
-  static_assert(SMEM <= 232448, "shared memory of a CTA");
+  constexpr size_t MOST = sizeof(typename Worker<CTAS, BT>::Smem) + 1024 + sizeof(GroupTable) * MMB200_MAX_GROUPS;
+  static_assert(MOST <= 232448, "shared memory of a CTA");
   static SmemLimit limit;
-  const cudaError_t err = limit.set(reinterpret_cast<const void*>(kern), SMEM);
+  const cudaError_t err = limit.set(reinterpret_cast<const void*>(kern), MOST);
   if (err != cudaSuccess) return err;
   const long long workers = sms() / CTAS;
-  return launch_dependent(kern, dim3((unsigned)(CTAS * (tiles < workers ? tiles : workers))), WORKER_THREADS, SMEM, st, m.w, m.a, p);
+  return launch_dependent(kern, dim3((unsigned)(CTAS * (tiles < workers ? tiles : workers))), WORKER_THREADS,
+                          Worker<CTAS, BT>::bytes(p), st, m.w, m.a, p);
 }
 template <int CTAS, int BT>
 cudaError_t launch_worker_out(const Int8Params& p, const Maps& m, long long tiles, cudaStream_t st) {

@@ -87,6 +87,8 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
     E, N, (T, K) = mat2.shape[0], mat2.shape[2], input.shape
     if E < 1 or E > MAX_GROUPS:
         raise ValueError(f"grouped_scaled_mm(): between 1 and {MAX_GROUPS} groups, got {E}")
+    if max(T, N, K) >= 1 << 31:
+        raise ValueError(f"grouped_scaled_mm(): sizes are below 2^31, got {T} rows, N = {N}, K = {K}")
     sizes = _sizes(m_splits, E, T)
     sa, sb = _group_scale("scale_a", scale_a, E), _group_scale("scale_b", scale_b, E)
     plain = _plainly_valid(input, mat2, scale_a, scale_b, scale_result, out_dtype, out)

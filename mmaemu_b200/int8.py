@@ -26,6 +26,7 @@ __all__ = ["quantize_int8", "int8_scaled_mm", "int8_grouped_scaled_mm"]
 
 MAX_K = 131071                     # 2^14 * K < 2^31: the int32 sums cannot overflow
 MAX_ROWS = 1 << 23
+MAX_N = 1 << 30                    # also of the values in a row of quantize_int8
 MAX_GROUPS = 4096
 _REAL_CODES = {torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}           # MMB200_HP_*
 _OUT_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # MMB200_OUT_*
@@ -56,10 +57,12 @@ def quantize_int8(x):
         raise ValueError("quantize_int8(): x must have at least one dimension")
     if x.requires_grad and torch.is_grad_enabled():
         raise _no_grad("quantize_int8")
+    K = shape[-1]
+    if K > MAX_N:
+        raise ValueError(f"quantize_int8(): a row has at most {MAX_N} values, got {K}")
     index = x.get_device()
     if index not in _SUPPORTED:
         _require_device(x.device)
-    K = shape[-1]
     rows, n = x, shape[0]
     if len(shape) != 2:
         n = shape[:-1].numel()
@@ -176,7 +179,7 @@ def int8_scaled_mm(input, mat2, scale_a, scale_b, bias=None, out_dtype=None, *, 
 
     scale_a: one element or [M, 1], scale_b: one element or [1, N], fp32. bias: [N] fp32, bf16 or fp16. out_dtype: bfloat16
     (default), float16 or float32. out: a row-major [M, N] tensor of the output dtype (any row stride) to write into.
-    K <= 131071, M <= 2^23. Rows of any alignment and stride are served; those that do not start on 16 bytes are copied
+    K <= 131071, M <= 2^23, N <= 2^30. Rows of any alignment and stride are served; those that do not start on 16 bytes are copied
     first."""
     who = "int8_scaled_mm"
     index = _check_operands(who, input, mat2, scale_a, scale_b, bias, out)
@@ -184,8 +187,9 @@ def int8_scaled_mm(input, mat2, scale_a, scale_b, bias=None, out_dtype=None, *, 
     if len(sizes) != 2 or len(sizes2) != 2 or sizes[1] != sizes2[0]:
         raise ValueError(f"{who}(): expected input [M, K] and mat2 [K, N], got {tuple(sizes)} and {tuple(sizes2)}")
     (M, K), N = sizes, sizes2[1]
-    if K > MAX_K or M > MAX_ROWS:
-        raise ValueError(f"{who}(): K is at most {MAX_K} (int32 sums) and M at most {MAX_ROWS}, got K = {K}, M = {M}")
+    if K > MAX_K or M > MAX_ROWS or N > MAX_N:
+        raise ValueError(f"{who}(): K is at most {MAX_K} (int32 sums), M at most {MAX_ROWS} and N at most {MAX_N}, got K = {K}, "
+                         f"M = {M}, N = {N}")
     unit, ldw = mat2.stride()
     if K > 1 and N > 0 and unit != 1:
         raise ValueError(f"{who}(): mat2 must be column-major (the transpose of a row-major [N, K] weight), got strides "
@@ -233,9 +237,9 @@ def int8_grouped_scaled_mm(input, mat2, offs, scale_a, scale_b, bias=None, out_d
     if len(sizes) != 2 or len(sizes2) != 3 or sizes[1] != sizes2[1]:
         raise ValueError(f"{who}(): expected input [T, K] and mat2 [E, K, N], got {tuple(sizes)} and {tuple(sizes2)}")
     (T, K), (E, _, N) = sizes, sizes2
-    if K > MAX_K or T > MAX_ROWS or E > MAX_GROUPS:
-        raise ValueError(f"{who}(): K is at most {MAX_K} (int32 sums), T at most {MAX_ROWS} and E at most {MAX_GROUPS}, got K = {K}, "
-                         f"T = {T}, E = {E}")
+    if K > MAX_K or T > MAX_ROWS or E > MAX_GROUPS or N > MAX_N:
+        raise ValueError(f"{who}(): K is at most {MAX_K} (int32 sums), T at most {MAX_ROWS}, E at most {MAX_GROUPS} and N at most "
+                         f"{MAX_N}, got K = {K}, T = {T}, E = {E}, N = {N}")
     if offs.dtype != torch.int32 or offs.dim() != 1 or offs.shape[0] != E:
         raise ValueError(f"{who}(): offs must be int32 of shape {(E,)}, got {offs.dtype} of shape {tuple(offs.shape)}")
     gsw, unit, ldw = mat2.stride()

@@ -222,7 +222,7 @@ def grouped_want(a, w, ends, sa, sb, out):
 
 
 GROUPS = [[1], [0, 0, 5], [16, 16, 16], [17, 0, 1, 31, 0], [128, 129, 127], [256, 1, 255, 300], [600, 3], [2] * 70, [0] * 40 + [9] + [0] * 30,
-          [33, 64, 65, 100, 0, 1], list(range(40))]
+          [33, 64, 65, 100, 0, 1], list(range(40)), [3, 0, 1] * 100]
 
 
 @pytest.mark.parametrize("sizes", GROUPS, ids=lambda s: f"{len(s)}groups{sum(s)}rows")
@@ -288,6 +288,29 @@ def test_grouped_operands_of_any_layout(make):
     sa, sb = scales(T, 1, seed=3), scales(E, 1, N, seed=4)
     ends = torch.tensor(sizes, device=DEV).cumsum(0).to(torch.int32)
     same(mm.int8_grouped_scaled_mm(a, w.transpose(1, 2), ends, sa, sb), grouped_want(a, w, ends.tolist(), sa, sb, torch.bfloat16))
+
+
+@pytest.mark.parametrize("T,N", [(5000, 16), (5000, 2000), (300000, 16)])
+def test_as_many_groups_as_there_may_be(T, N):
+    """4096 groups, most of them empty or of a row; tiles per CTA and persistent CTAs."""
+    E, K = 4096, 48
+    g = torch.Generator().manual_seed(T)
+    at = torch.sort(torch.randint(0, T + 1, (E,), generator=g))[0]
+    at[-1] = T - 3
+    at = at.clamp(max=T - 3)
+    a, w = codes(T, K, seed=1), codes(E, N, K, seed=2)
+    sa, sb = scales(T, 1, seed=3), scales(E, 1, N, seed=4)
+    y = mm.int8_grouped_scaled_mm(a, w.transpose(1, 2), at.to(torch.int32).to(DEV), sa, sb, out_dtype=torch.float32)
+    e = torch.searchsorted(at, torch.arange(T), right=True).to(DEV)
+    real = e < E
+    e = e.clamp(max=E - 1)
+    for lo in range(0, T, 4096):                                     # row by row in pieces: one weight matrix per row
+        rows = slice(lo, min(T, lo + 4096))
+        for c in range(0, N, 500):
+            cols = slice(c, min(N, c + 500))
+            acc = torch.einsum("tk,tnk->tn", a[rows].float(), w[:, cols][e[rows]].float())        # exact: at most 48 * 2^14
+            want = acc * (sa[rows] * sb[e[rows], 0, cols]) + 0.0
+            same(y[rows, cols], torch.where(real[rows, None], want, 0.0))
 
 
 def test_grouped_without_groups_or_rows():

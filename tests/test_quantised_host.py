@@ -69,6 +69,7 @@ def test_refusals(call, kw, exc):
 @pytest.mark.parametrize("kw", [
     dict(mat2=z(32, 16)), dict(scale_b=s(16, 1)), dict(scale_b=s(1, 15)), dict(mat2=z(16, 32)), dict(mat2=z(2, 16, 32).transpose(1, 2)),
     dict(input=z(1, 131072), mat2=z(1, 131072).t()), dict(input=torch.zeros(1, dtype=I8).expand((1 << 23) + 1, 1), mat2=z(1, 1)),
+    dict(input=z(1, 1), mat2=z(1, 1).expand(1, (1 << 30) + 1)),
 ])
 def test_refusals_of_the_dense_product(kw):
     with pytest.raises(ValueError):
@@ -98,7 +99,8 @@ def test_gradients_are_refused():
         dense(scale_a=w)
 
 
-@pytest.mark.parametrize("x,exc", [([1.0], TypeError), (z(3, 4), TypeError), (s(3, 4).double(), TypeError), (torch.tensor(1.0), ValueError)])
+@pytest.mark.parametrize("x,exc", [([1.0], TypeError), (z(3, 4), TypeError), (s(3, 4).double(), TypeError), (torch.tensor(1.0), ValueError),
+                                   (s(1, 1).expand(1, (1 << 30) + 1), ValueError)])
 def test_refusals_of_the_quantiser(x, exc):
     with pytest.raises(exc):
         mm.quantize_int8(x)
@@ -116,6 +118,7 @@ def test_refusals_of_the_quantiser(x, exc):
     (dict(mat2=z(3, 32, 16, dtype=torch.float8_e4m3fn)), mm.ReferenceRejectsError),
     (dict(out=z(4, 15, dtype=torch.bfloat16)), ValueError), (dict(out=z(16, 4, dtype=torch.bfloat16).t()), ValueError),
     (dict(out=z(4, 16, dtype=torch.float16)), mm.ReferenceRejectsError), (dict(use_fast_accum=1), TypeError),
+    (dict(input=z(1, 32, dtype=torch.float8_e4m3fn).expand(1 << 31, 32), m_splits=[1 << 31, 0, 0]), ValueError),
     (dict(profile="nothing"), Exception), (dict(splitk=(2, "serial")), ValueError), (dict(backend="cuda:h4"), mm.BackendUnavailableError),
     (dict(mat2=torch.zeros(3 * 520, dtype=torch.float8_e4m3fn).as_strided((3, 32, 16), (520, 1, 32))), mm.ReferenceRejectsError),
 ])
@@ -151,7 +154,7 @@ def test_argument_checks_of_the_entry_points(lib):
                dict(sb=None), dict(sas=-1), dict(sbs=-1), dict(sbg=-1), dict(gsw=-1), dict(bg=-1), dict(d=None), dict(a=None), dict(w=None),
                dict(lda=15), dict(ldw=15), dict(ldd=15), dict(d=p + 1)):
         assert i8(**kw) == _lib.ERR_BAD_ARG, kw
-    for kw in (dict(K=131072, lda=131072, ldw=131072), dict(T=(1 << 23) + 1), dict(E=4097, offs=p)):
+    for kw in (dict(K=131072, lda=131072, ldw=131072), dict(T=(1 << 23) + 1), dict(E=4097, offs=p), dict(N=(1 << 30) + 1, ldd=1 << 31)):
         assert i8(**kw) == _lib.ERR_TOO_LARGE, kw
     assert i8(T=0) == _lib.OK and i8(N=0) == _lib.OK
     q = lib.mmb200_quantize_int8
