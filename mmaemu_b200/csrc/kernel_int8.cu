@@ -601,9 +601,10 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
       write_rows<OUT, BT / 2>(p, mine + (i & 1) * BT, nk > 0, row0 + half, rows, n, real, sb, bias, scale);
       fence_before();
       __syncwarp();
+      // (relaxed: the accumulator's values are in registers; a release would wait for the tile's stores to reach memory)
       if (lane == 0) {
-        if constexpr (CTAS == 1) mbar_arrive(&sm.acc_empty[i & 1]);
-        else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(first_cta<CTAS>(&sm.acc_empty[i & 1])) : "memory");
+        if constexpr (CTAS == 1) asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&sm.acc_empty[i & 1])) : "memory");
+        else asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(first_cta<CTAS>(&sm.acc_empty[i & 1])) : "memory");
       }
     }
     if (ok && p.zero_rest)
