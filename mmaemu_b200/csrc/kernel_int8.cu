@@ -118,7 +118,11 @@ template <int OUT, int BT>
 __device__ __forceinline__ void write_rows(const Int8Params& p, uint32_t acc, bool products, long long row0, int rows, int n, bool real, float sb,
                                            float bias, float scale) {
   constexpr int CHUNK = BT < 32 ? BT : 32;
-  typename OutType<OUT>::type* out = static_cast<typename OutType<OUT>::type*>(p.d) + row0 * p.ldd + n;
+  using O = typename OutType<OUT>::type;
+  O* out = static_cast<O*>(p.d) + row0 * p.ldd + n;
+  auto value = [&](int sum, float s, int q) {
+    return out_bits<OUT>(__fmaf_rn(__int2float_rn(sum), __fmul_rn(__shfl_sync(0xFFFFFFFFu, s, q), sb), bias));
+  };
 #pragma unroll 1
   for (int c = 0; c < rows; c += CHUNK) {
     int r[CHUNK];
@@ -131,12 +135,23 @@ __device__ __forceinline__ void write_rows(const Int8Params& p, uint32_t acc, bo
     const float s = scale;
     scale = row_scales<CHUNK>(p, row0 + c + CHUNK, rows - c - CHUNK);
     const int left = rows - c;
+    if (left >= CHUNK && __all_sync(0xFFFFFFFFu, real)) {
 #pragma unroll
-    for (int q = 0; q < CHUNK; ++q) {
-      const float alpha = __fmul_rn(__shfl_sync(0xFFFFFFFFu, s, q), sb);
-      const auto y = out_bits<OUT>(__fmaf_rn(__int2float_rn(r[q]), alpha, bias));
-      if (real && q < left) *out = y;
-      out += p.ldd;
+      for (int q = 0; q < CHUNK; q += 8) {
+        O y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = value(r[q + j], s, q + j);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) out[j * p.ldd] = y[j];
+        out += 8 * p.ldd;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < CHUNK; ++q) {
+        const O y = value(r[q], s, q);
+        if (real && q < left) *out = y;
+        out += p.ldd;
+      }
     }
   }
 }
