@@ -13,12 +13,13 @@
 // int8_single_kernel, int8_pair_kernel: more rows. Persistent; TMEM holds two accumulators, so the output of a tile leaves while
 // the next one is multiplied. A CTA works on 128 channels x 64, 128 or 256 rows, a pair of CTAs on neighbouring SMs
 // (cta_group::2) on 256 x 256, each holding half of both operands, so that a byte of shared memory feeds twice the products.
-// Large products are bound by power: 8192 x 24576 x 8192 takes 1.13 ms, 2.9 POP/s, with operands of zeros 4.1 POP/s. 4096 rows
-// in 64 groups on 1536 x 2048 weights: 48 us for 201 MB of weights (one-tile CTAs: 55 us, and 66 with tiles of 128 rows).
+// Large products are bound by power: 8192 x 24576 x 8192 takes 1.11 ms, 2.95 POP/s; the 8192-cube 3.2 POP/s, with operands of
+// zeros 4.0. 4096 rows in 64 groups on 1536 x 2048 weights: 44 us for 201 MB of weights (one-tile CTAs: 55 us).
 //
 // An MMA of 128 channels takes about 120 cycles up to 128 rows, so a CTA needs 0.25 us per 128 bytes of K however few rows it
-// has. The output loop must not wait: with a scale loaded per row instead of handed round by shuffles it took 27 us per tile
-// and was most of every product with K below 4096.
+// has. The output loop must not wait: with a scale loaded per row instead of handed round by shuffles it took 27 us per tile of
+// 256 x 256, now 4.5 us, which still bounds products with K of 1024 and less (8192 x 8192 x 1024: 64 us, of which the MMAs would
+// take 37).
 #include <cuda.h>
 #include <cuda_fp16.h>
 

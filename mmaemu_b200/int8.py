@@ -19,11 +19,12 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .api import _STAY, _SUPPORTED, _require_device
+from .api import _SUPPORTED, _require_device
 from .errors import UnsupportedFeatureError
 
 __all__ = ["quantize_int8", "int8_scaled_mm", "int8_grouped_scaled_mm"]
 
+_Tensor, _INT8, _F32 = torch.Tensor, torch.int8, torch.float32
 MAX_K = 131071                     # 2^14 * K < 2^31: the int32 sums cannot overflow
 MAX_ROWS = 1 << 23
 MAX_N = 1 << 30                    # also of the values in a row of quantize_int8
@@ -38,6 +39,13 @@ def _not_a_tensor(who: str, name: str, t) -> TypeError:
 
 def _no_grad(who: str) -> UnsupportedFeatureError:
     return UnsupportedFeatureError(f"{who}(): inference only: an input requires grad while grad mode is enabled")
+
+
+def _quantise(rows, ld, code, codes, scale, n, K, index) -> None:
+    rc = _lib.load().mmb200_quantize_int8(rows.data_ptr(), ld, code, codes.data_ptr(), K, scale.data_ptr(), n, K,
+                                          torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check("mmb200_quantize_int8", rc)
 
 
 def quantize_int8(x):
@@ -76,36 +84,32 @@ def quantize_int8(x):
     scale = x.new_empty((n, 1) if len(shape) == 2 else (*shape[:-1], 1), dtype=torch.float32)
     if n == 0:
         return codes, scale
-    with _STAY if index == torch._C._cuda_getDevice() else torch.cuda.device(index):
-        rc = _lib.load().mmb200_quantize_int8(rows.data_ptr(), ld, code, codes.data_ptr(), K, scale.data_ptr(), n, K,
-                                              torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        _lib.check("mmb200_quantize_int8", rc)
+    if index == torch._C._cuda_getDevice():
+        _quantise(rows, ld, code, codes, scale, n, K, index)
+    else:
+        with torch.cuda.device(index):
+            _quantise(rows, ld, code, codes, scale, n, K, index)
     return codes, scale
 
 
 def _check_operands(who, input, mat2, scale_a, scale_b, bias, out) -> int:
     """Types, one device (its index; -1: no GPU), no gradients."""
-    for name, t in (("input", input), ("mat2", mat2), ("scale_a", scale_a), ("scale_b", scale_b)):
-        if not isinstance(t, torch.Tensor):
-            raise _not_a_tensor(who, name, t)
-    if input.dtype != torch.int8 or mat2.dtype != torch.int8:
+    if not (isinstance(input, _Tensor) and isinstance(mat2, _Tensor) and isinstance(scale_a, _Tensor) and isinstance(scale_b, _Tensor)
+            and (bias is None or isinstance(bias, _Tensor)) and (out is None or isinstance(out, _Tensor))):
+        for name, t in (("input", input), ("mat2", mat2), ("scale_a", scale_a), ("scale_b", scale_b), ("bias", bias), ("out", out)):
+            if not isinstance(t, _Tensor) and (t is not None or name not in ("bias", "out")):
+                raise _not_a_tensor(who, name, t)
+    if input.dtype is not _INT8 or mat2.dtype is not _INT8:
         raise TypeError(f"{who}(): input and mat2 must be int8, got {input.dtype} and {mat2.dtype}")
     index = input.get_device()
-    grad = scale_a.requires_grad or scale_b.requires_grad
-    same = mat2.get_device() == index and scale_a.get_device() == index and scale_b.get_device() == index
-    for name, t in (("bias", bias), ("out", out)):
-        if t is not None:
-            if not isinstance(t, torch.Tensor):
-                raise _not_a_tensor(who, name, t)
-            grad = grad or t.requires_grad
-            same = same and t.get_device() == index
-    if not same:
+    if not (index == mat2.get_device() == scale_a.get_device() == scale_b.get_device() and (bias is None or bias.get_device() == index)
+            and (out is None or out.get_device() == index)):
         raise ValueError(f"{who}(): expected all tensors on one device, found "
                          f"{sorted({str(t.device) for t in (input, mat2, scale_a, scale_b, bias, out) if t is not None})}")
-    if grad and torch.is_grad_enabled():
+    if (scale_a.requires_grad or scale_b.requires_grad or (bias is not None and bias.requires_grad)
+            or (out is not None and out.requires_grad)) and torch.is_grad_enabled():
         raise _no_grad(who)
-    if scale_a.dtype != torch.float32 or scale_b.dtype != torch.float32:
+    if scale_a.dtype is not _F32 or scale_b.dtype is not _F32:
         raise ValueError(f"{who}(): scale_a and scale_b must be float32, got {scale_a.dtype} and {scale_b.dtype}")
     return index
 
@@ -155,22 +159,21 @@ def _bias(who, bias, shape):
     return bias.detach().contiguous(), code
 
 
-def _run(index, ap, lda, wp, ldw, gsw, y, ldd, code, T, N, K, E, offs, scale_a, sa, scale_b, sb_group, sb, bias, bias_code, bias_group,
-         zero_rest):
+def _run(index, ap, lda, wp, ldw, gsw, y, *rest) -> None:
+    """The call into the library. rest: what follows D_dev in mmb200_int8_scaled_mm, up to zero_rest."""
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _run(index, ap, lda, wp, ldw, gsw, y, *rest)
     L = _lib.load()
-    with _STAY if index == torch._C._cuda_getDevice() else torch.cuda.device(index):
-        ws, ws_ptr, n = None, None, 0
-        if (ap | wp | lda | ldw | gsw) & 15 or (E > 1 and not gsw):     # rows that TMA cannot read in place: room for copies
-            n = L.mmb200_int8_workspace_bytes(ap, lda, wp, ldw, gsw, T, N, K, E)
-            if n:
-                ws = y.new_empty(n, dtype=torch.uint8)
-                ws_ptr = ws.data_ptr()
-        rc = L.mmb200_int8_scaled_mm(ap, lda, wp, ldw, gsw, y.data_ptr(), ldd, code, T, N, K, E, offs, scale_a.data_ptr(), sa,
-                                     scale_b.data_ptr(), sb_group, sb, None if bias is None else bias.data_ptr(), bias_code, bias_group,
-                                     zero_rest, ws_ptr, n, torch._C._cuda_getCurrentRawStream(index))
-        if rc:
-            _lib.check("mmb200_int8_scaled_mm", rc)
-    return y
+    ws, ws_ptr, n = None, None, 0
+    if (ap | wp | lda | ldw | gsw) & 15 or (rest[5] > 1 and not gsw):   # rows that TMA cannot read in place: room for copies
+        n = L.mmb200_int8_workspace_bytes(ap, lda, wp, ldw, gsw, *rest[2:6])
+        if n:
+            ws = y.new_empty(n, dtype=torch.uint8)
+            ws_ptr = ws.data_ptr()
+    rc = L.mmb200_int8_scaled_mm(ap, lda, wp, ldw, gsw, y.data_ptr(), *rest, ws_ptr, n, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check("mmb200_int8_scaled_mm", rc)
 
 
 def int8_scaled_mm(input, mat2, scale_a, scale_b, bias=None, out_dtype=None, *, out=None):
@@ -214,8 +217,9 @@ def int8_scaled_mm(input, mat2, scale_a, scale_b, bias=None, out_dtype=None, *, 
         ldw = K
     elif ldw < K:                                        # overlapping rows
         mat2, ldw = mat2.t().contiguous(), K
-    return _run(index, a.data_ptr(), lda, mat2.data_ptr(), ldw, 0, y, ldd, code, M, N, K, 1, None, scale_a, sa, scale_b, 0, sb, bias,
-                bias_code, 0, 0)
+    _run(index, a.data_ptr(), lda, mat2.data_ptr(), ldw, 0, y, ldd, code, M, N, K, 1, None, scale_a.data_ptr(), sa, scale_b.data_ptr(), 0,
+         sb, None if bias is None else bias.data_ptr(), bias_code, 0, 0)
+    return y
 
 
 def int8_grouped_scaled_mm(input, mat2, offs, scale_a, scale_b, bias=None, out_dtype=None, *, out=None):
@@ -268,8 +272,10 @@ def int8_grouped_scaled_mm(input, mat2, offs, scale_a, scale_b, bias=None, out_d
         mat2 = mat2.transpose(1, 2).contiguous()
         gsw, ldw = N * K, K
     offs = offs.contiguous()
-    return _run(index, a.data_ptr(), lda, mat2.data_ptr(), ldw if N > 1 else K, gsw if E > 1 else 0, y, ldd, code, T, N, K, E,
-                offs.data_ptr(), scale_a, sa, scale_b, sb_group, sb, bias, bias_code, N, int(out is None))
+    _run(index, a.data_ptr(), lda, mat2.data_ptr(), ldw if N > 1 else K, gsw if E > 1 else 0, y, ldd, code, T, N, K, E, offs.data_ptr(),
+         scale_a.data_ptr(), sa, scale_b.data_ptr(), sb_group, sb, None if bias is None else bias.data_ptr(), bias_code, N,
+         int(out is None))
+    return y
 
 
 # torch.compile must not trace into these entry points (they call a foreign library through ctypes)
