@@ -8,7 +8,7 @@
 // int8_tile_kernel: few rows. One tile of 128 channels x 16, 32 or 64 rows per cluster; the CTAs of a cluster each take a part of
 // K and add their int32 sums through distributed shared memory. Integer sums are exact in any order, so the split changes no
 // bit. Bound by reading the weights: 16 x 8192 x 28672 at 6.1 TB/s (38.5 us); 16 x 4096 x 8192 in 9.2 us, of which 3.5 are
-// launch, first copies and the cluster's sum (13 us more while a thread read the sums one by one).
+// launch, first copies and the cluster's sum (64 rows, 512 channels, K = 512 in 4 us; 13 while a thread read the sums one by one).
 //
 // int8_single_kernel, int8_pair_kernel: more rows. Persistent; TMEM holds two accumulators, so the output of a tile leaves while
 // the next one is multiplied. A CTA works on 128 channels x 64, 128 or 256 rows, a pair of CTAs on neighbouring SMs
