@@ -271,11 +271,26 @@ int mmb200_quantize_int8(const void *X_dev, int64_t ldx, int x_dtype, int8_t *co
 #define MMB200_INT8_MAX_N (1 << 30)
 size_t mmb200_int8_workspace_bytes(const int8_t *A_dev, int64_t lda, const int8_t *W_dev, int64_t ldw,
                                    int64_t group_stride_w, int T, int N, int K, int E);
-int mmb200_int8_scaled_mm(const int8_t *A_dev, int64_t lda, const int8_t *W_dev, int64_t ldw, int64_t group_stride_w,
-                          void *D_dev, int64_t ldd, int out_dtype, int T, int N, int K, int E, const int *offs_dev,
-                          const float *scale_a_dev, int64_t sa_stride, const float *scale_b_dev, int64_t sb_group_stride,
-                          int64_t sb_stride, const void *bias_dev, int bias_dtype, int64_t bias_group_stride, int zero_rest,
-                          void *workspace_dev, size_t workspace_bytes, void *stream);
+/* (25 fields of 64 bits, so that a binding can pack them in one go) */
+typedef struct mmb200_int8_args {
+  const int8_t *A_dev;
+  int64_t lda;
+  const int8_t *W_dev;
+  int64_t ldw, group_stride_w;
+  void *D_dev;
+  int64_t ldd, out_dtype, T, N, K, E;
+  const int *offs_dev;
+  const float *scale_a_dev;
+  int64_t sa_stride;
+  const float *scale_b_dev;
+  int64_t sb_group_stride, sb_stride;
+  const void *bias_dev;
+  int64_t bias_dtype, bias_group_stride, zero_rest;
+  void *workspace_dev;
+  uint64_t workspace_bytes;
+  void *stream;
+} mmb200_int8_args;
+int mmb200_int8_scaled_mm(const mmb200_int8_args *args);
 /* The kernel that a call of this shape runs on: kind << 16 | rows of a tile << 4 | parts of K, kind 0: one tile per CTA (a
  * cluster of `parts` CTAs shares a tile), 1: persistent CTAs, 2: persistent pairs of CTAs. ragged: whether offs_dev is given.
  * Pure host logic (148 SMs are assumed where no device answers). */

@@ -6,6 +6,7 @@ There is no fallback: if the shared object is missing or a call fails, an except
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -27,6 +28,9 @@ EXPORTS = ("mmb200_abi_version", "mmb200_status_string", "mmb200_last_cuda_error
            "mmb200_workspace_status", "mmb200_scaled_mm_static_status", "mmb200_test_hooks", "mmb200_scaled_mm_peers", "mmb200_probe_issue_rate",
            "mmb200_grouped_workspace_bytes", "mmb200_grouped_scaled_mm", "mmb200_grouped_status", "mmb200_quantize_int8", "mmb200_int8_workspace_bytes",
            "mmb200_int8_scaled_mm", "mmb200_int8_kernel_for", "mmb200_int8_status")
+
+# mmb200_int8_args as bytes: one argument instead of 25, whose conversion took 3 us of a call
+int8_args = struct.Struct("25q").pack
 
 _lock = threading.Lock()
 _lib = None
@@ -115,8 +119,7 @@ def load():
         L.mmb200_quantize_int8.restype = ci
         L.mmb200_int8_workspace_bytes.argtypes = [vp, i64, vp, i64, i64, ci, ci, ci, ci]
         L.mmb200_int8_workspace_bytes.restype = sz
-        L.mmb200_int8_scaled_mm.argtypes = [vp, i64, vp, i64, i64, vp, i64, ci, ci, ci, ci, ci, vp, vp, i64, vp, i64, i64, vp, ci,
-                                            i64, ci, vp, sz, vp]
+        L.mmb200_int8_scaled_mm.argtypes = [ctypes.c_char_p]         # int8_args
         L.mmb200_int8_scaled_mm.restype = ci
         L.mmb200_int8_kernel_for.argtypes = [ci, ci, ci, ci, ci]
         L.mmb200_int8_kernel_for.restype = ci

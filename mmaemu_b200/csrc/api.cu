@@ -704,40 +704,41 @@ size_t mmb200_int8_workspace_bytes(const int8_t* A, int64_t lda, const int8_t* W
   return mmb::int8_workspace_bytes(p);
 }
 
-int mmb200_int8_scaled_mm(const int8_t* A, int64_t lda, const int8_t* W, int64_t ldw, int64_t group_stride_w, void* D, int64_t ldd,
-                          int out_dtype, int T, int N, int K, int E, const int* offs, const float* scale_a, int64_t sa_stride,
-                          const float* scale_b, int64_t sb_group_stride, int64_t sb_stride, const void* bias, int bias_dtype,
-                          int64_t bias_group_stride, int zero_rest, void* workspace, size_t workspace_bytes, void* stream) {
-  if (T < 0 || N < 0 || K < 0 || E < 1 || (!offs && E != 1)) return MMB200_ERR_BAD_ARG;
-  if (out_dtype < MMB200_OUT_F32 || out_dtype > MMB200_OUT_F16) return MMB200_ERR_BAD_ARG;
-  if (bias && (bias_dtype < MMB200_HP_F32 || bias_dtype > MMB200_HP_F16)) return MMB200_ERR_BAD_ARG;
-  if (!scale_a || !scale_b || sa_stride < 0 || sb_stride < 0 || sb_group_stride < 0 || bias_group_stride < 0 || group_stride_w < 0)
+int mmb200_int8_scaled_mm(const mmb200_int8_args* a) {
+  static_assert(sizeof(mmb200_int8_args) == 25 * 8, "packed by bindings");
+  if (!a || a->T < 0 || a->N < 0 || a->K < 0 || a->E < 1 || (!a->offs_dev && a->E != 1)) return MMB200_ERR_BAD_ARG;
+  if (a->out_dtype < MMB200_OUT_F32 || a->out_dtype > MMB200_OUT_F16) return MMB200_ERR_BAD_ARG;
+  if (a->bias_dev && (a->bias_dtype < MMB200_HP_F32 || a->bias_dtype > MMB200_HP_F16)) return MMB200_ERR_BAD_ARG;
+  if (!a->scale_a_dev || !a->scale_b_dev || a->sa_stride < 0 || a->sb_stride < 0 || a->sb_group_stride < 0 || a->bias_group_stride < 0 ||
+      a->group_stride_w < 0)
     return MMB200_ERR_BAD_ARG;
-  if (K > MMB200_INT8_MAX_K || T > MMB200_INT8_MAX_ROWS || N > MMB200_INT8_MAX_N || E > MMB200_MAX_GROUPS) return MMB200_ERR_TOO_LARGE;
-  if (T == 0 || N == 0) return MMB200_OK;
-  if (!D || (T > 1 && ldd < N)) return MMB200_ERR_BAD_ARG;
-  if (K > 0 && (!A || !W || (T > 1 && lda < K) || (N > 1 && ldw < K))) return MMB200_ERR_BAD_ARG;
-  const uintptr_t es = out_dtype == MMB200_OUT_F32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(D) % es) return MMB200_ERR_BAD_ARG;
+  if (a->K > MMB200_INT8_MAX_K || a->T > MMB200_INT8_MAX_ROWS || a->N > MMB200_INT8_MAX_N || a->E > MMB200_MAX_GROUPS)
+    return MMB200_ERR_TOO_LARGE;
+  if (a->T == 0 || a->N == 0) return MMB200_OK;
+  if (!a->D_dev || (a->T > 1 && a->ldd < a->N)) return MMB200_ERR_BAD_ARG;
+  if (a->K > 0 && (!a->A_dev || !a->W_dev || (a->T > 1 && a->lda < a->K) || (a->N > 1 && a->ldw < a->K))) return MMB200_ERR_BAD_ARG;
+  const uintptr_t es = a->out_dtype == MMB200_OUT_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(a->D_dev) % es) return MMB200_ERR_BAD_ARG;
   const int rc = current_device_ok();
   if (rc != MMB200_OK) return rc;
   mmb::Int8Params p;
   std::memset(&p, 0, sizeof(p));
-  p.a = A; p.w = W; p.d = D;
-  p.scale_a = scale_a; p.scale_b = scale_b; p.bias = bias; p.offs = offs;
-  p.lda = lda; p.ldw = ldw; p.gsw = group_stride_w; p.ldd = ldd; p.sb_group = sb_group_stride; p.bias_group = bias_group_stride;
-  p.T = T; p.N = N; p.K = K; p.E = E;
-  p.sa_stride = sa_stride; p.sb_stride = sb_stride;
-  p.bias_dtype = bias_dtype; p.out_dtype = out_dtype;
-  p.zero_rest = zero_rest;
+  p.a = a->A_dev; p.w = a->W_dev; p.d = a->D_dev;
+  p.scale_a = a->scale_a_dev; p.scale_b = a->scale_b_dev; p.bias = a->bias_dev; p.offs = a->offs_dev;
+  p.lda = a->lda; p.ldw = a->ldw; p.gsw = a->group_stride_w; p.ldd = a->ldd;
+  p.sa_stride = a->sa_stride; p.sb_stride = a->sb_stride; p.sb_group = a->sb_group_stride; p.bias_group = a->bias_group_stride;
+  p.T = (int)a->T; p.N = (int)a->N; p.K = (int)a->K; p.E = (int)a->E;
+  p.bias_dtype = (int)a->bias_dtype; p.out_dtype = (int)a->out_dtype;
+  p.zero_rest = a->zero_rest != 0;
   const size_t need = mmb::int8_workspace_bytes(p);
-  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) return MMB200_ERR_BAD_ARG;
+  if (need && (!a->workspace_dev || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace_dev) & 15)))
+    return MMB200_ERR_BAD_ARG;
   int launches = 0;
-  const cudaError_t err = mmb::launch_int8(p, workspace, static_cast<cudaStream_t>(stream), &launches);
+  const cudaError_t err = mmb::launch_int8(p, a->workspace_dev, static_cast<cudaStream_t>(a->stream), &launches);
   g_launches.fetch_add(launches, std::memory_order_relaxed);
   if (err != cudaSuccess) return cuda_fail(err);
   const char* check = std::getenv("MMAEMU_B200_CHECK_STATUS");
-  return check && check[0] == '1' && !check[1] ? mmb200_int8_status(stream) : MMB200_OK;
+  return check && check[0] == '1' && !check[1] ? mmb200_int8_status(a->stream) : MMB200_OK;
 }
 
 int mmb200_int8_kernel_for(int T, int N, int K, int E, int ragged) {

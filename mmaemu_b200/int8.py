@@ -160,18 +160,19 @@ def _bias(who, bias, shape):
 
 
 def _run(index, ap, lda, wp, ldw, gsw, y, *rest) -> None:
-    """The call into the library. rest: what follows D_dev in mmb200_int8_scaled_mm, up to zero_rest."""
+    """The call into the library. rest: what follows D_dev in mmb200_int8_args, up to zero_rest."""
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return _run(index, ap, lda, wp, ldw, gsw, y, *rest)
     L = _lib.load()
-    ws, ws_ptr, n = None, None, 0
+    ws, ws_ptr, n = None, 0, 0
     if (ap | wp | lda | ldw | gsw) & 15 or (rest[5] > 1 and not gsw):   # rows that TMA cannot read in place: room for copies
         n = L.mmb200_int8_workspace_bytes(ap, lda, wp, ldw, gsw, *rest[2:6])
         if n:
             ws = y.new_empty(n, dtype=torch.uint8)
             ws_ptr = ws.data_ptr()
-    rc = L.mmb200_int8_scaled_mm(ap, lda, wp, ldw, gsw, y.data_ptr(), *rest, ws_ptr, n, torch._C._cuda_getCurrentRawStream(index))
+    rc = L.mmb200_int8_scaled_mm(_lib.int8_args(ap, lda, wp, ldw, gsw, y.data_ptr(), *rest, ws_ptr, n,
+                                                torch._C._cuda_getCurrentRawStream(index)))
     if rc:
         _lib.check("mmb200_int8_scaled_mm", rc)
 
@@ -217,8 +218,8 @@ def int8_scaled_mm(input, mat2, scale_a, scale_b, bias=None, out_dtype=None, *, 
         ldw = K
     elif ldw < K:                                        # overlapping rows
         mat2, ldw = mat2.t().contiguous(), K
-    _run(index, a.data_ptr(), lda, mat2.data_ptr(), ldw, 0, y, ldd, code, M, N, K, 1, None, scale_a.data_ptr(), sa, scale_b.data_ptr(), 0,
-         sb, None if bias is None else bias.data_ptr(), bias_code, 0, 0)
+    _run(index, a.data_ptr(), lda, mat2.data_ptr(), ldw, 0, y, ldd, code, M, N, K, 1, 0, scale_a.data_ptr(), sa, scale_b.data_ptr(), 0,
+         sb, 0 if bias is None else bias.data_ptr(), bias_code, 0, 0)
     return y
 
 
@@ -273,7 +274,7 @@ def int8_grouped_scaled_mm(input, mat2, offs, scale_a, scale_b, bias=None, out_d
         gsw, ldw = N * K, K
     offs = offs.contiguous()
     _run(index, a.data_ptr(), lda, mat2.data_ptr(), ldw if N > 1 else K, gsw if E > 1 else 0, y, ldd, code, T, N, K, E, offs.data_ptr(),
-         scale_a.data_ptr(), sa, scale_b.data_ptr(), sb_group, sb, None if bias is None else bias.data_ptr(), bias_code, N,
+         scale_a.data_ptr(), sa, scale_b.data_ptr(), sb_group, sb, 0 if bias is None else bias.data_ptr(), bias_code, N,
          int(out is None))
     return y
 

@@ -146,15 +146,18 @@ def test_argument_checks_of_the_entry_points(lib):
     buf = ctypes.create_string_buffer(1024)
     p = (ctypes.addressof(buf) + 15) // 16 * 16
 
-    def i8(a=p, lda=16, w=p, ldw=16, gsw=0, d=p, ldd=16, out=1, T=2, N=16, K=16, E=1, offs=None, sa=p, sas=0, sb=p, sbg=0, sbs=0, bias=None,
+    def i8(a=p, lda=16, w=p, ldw=16, gsw=0, d=p, ldd=16, out=1, T=2, N=16, K=16, E=1, offs=0, sa=p, sas=0, sb=p, sbg=0, sbs=0, bias=0,
            bt=0, bg=0):
-        return lib.mmb200_int8_scaled_mm(a, lda, w, ldw, gsw, d, ldd, out, T, N, K, E, offs, sa, sas, sb, sbg, sbs, bias, bt, bg, 0, None, 0, None)
+        return lib.mmb200_int8_scaled_mm(_lib.int8_args(a, lda, w, ldw, gsw, d, ldd, out, T, N, K, E, offs, sa, sas, sb, sbg, sbs, bias, bt, bg, 0,
+                                                        0, 0, 0))
 
-    for kw in (dict(T=-1), dict(N=-1), dict(K=-1), dict(E=-1), dict(E=2), dict(out=3), dict(out=-1), dict(bias=p, bt=0), dict(sa=None),
-               dict(sb=None), dict(sas=-1), dict(sbs=-1), dict(sbg=-1), dict(gsw=-1), dict(bg=-1), dict(d=None), dict(a=None), dict(w=None),
+    assert lib.mmb200_int8_scaled_mm(None) == _lib.ERR_BAD_ARG
+    for kw in (dict(T=-1), dict(N=-1), dict(K=-1), dict(E=-1), dict(E=2), dict(out=3), dict(out=-1), dict(bias=p, bt=0), dict(sa=0),
+               dict(sb=0), dict(sas=-1), dict(sbs=-1), dict(sbg=-1), dict(gsw=-1), dict(bg=-1), dict(d=0), dict(a=0), dict(w=0),
                dict(lda=15), dict(ldw=15), dict(ldd=15), dict(d=p + 1)):
         assert i8(**kw) == _lib.ERR_BAD_ARG, kw
-    for kw in (dict(K=131072, lda=131072, ldw=131072), dict(T=(1 << 23) + 1), dict(E=4097, offs=p), dict(N=(1 << 30) + 1, ldd=1 << 31)):
+    for kw in (dict(K=131072, lda=131072, ldw=131072), dict(T=(1 << 23) + 1), dict(E=4097, offs=p), dict(N=(1 << 30) + 1, ldd=1 << 31),
+               dict(N=(1 << 32) + 16), dict(T=1 << 40)):
         assert i8(**kw) == _lib.ERR_TOO_LARGE, kw
     assert i8(T=0) == _lib.OK and i8(N=0) == _lib.OK
     q = lib.mmb200_quantize_int8
