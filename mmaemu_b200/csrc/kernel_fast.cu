@@ -646,8 +646,8 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const __grid_constant_
 }
 
 #if !defined(MMB_PART) || MMB_PART == 0
-// By one block of THREADS threads: writes the tile sequence and, behind it (`events`, when not null), the entries that matter to the second pass of
-// K-sliced execution in the same order: those after which a chain or a split is complete.
+// By one block of THREADS threads: writes the tile sequence and, behind it (`events`, when not null), the entries that matter to
+// the second pass of K-sliced execution in the same order: those after which a chain or a split is complete.
 __device__ __forceinline__ void write_sequence(const Plan& plan, int K, uint32_t* out, uint32_t* events) {
   const int n = plan_sequence(plan, K, out, (int)threadIdx.x, (int)blockDim.x);
   if (!events) return;
@@ -1637,10 +1637,12 @@ GroupedPlan grouped_plan(const Params& p, int nfma, const int* rows, const unsig
     double time = 0.0;
     if (g.n128) {
       const long long tiles = g.n128 * tiles_n, wide = g.n128 * ((tiles_n + 1) / 2);
-      const double narrow_waves = (double)((tiles + sms - 1) / sms), wide_waves = (double)((wide + sms - 1) / sms) * KernelTimes::wide_wave(p.fast != 0);
+      const double narrow_waves = (double)((tiles + sms - 1) / sms);
+      const double wide_waves = (double)((wide + sms - 1) / sms) * KernelTimes::wide_wave(p.fast != 0);
       g.wide = kt.one_sum && wide_waves < narrow_waves;
       // the decode passes read 4 KB and write 16 KB per 128 rows and k-tile, at about 5 TB/s
-      time += (g.wide ? wide_waves : narrow_waves) * kt.umma * k_tiles + kt.predecode + (double)(g.n128 + (long long)g.slots128 * tiles_n) * k_tiles * 20480.0 / 5e6;
+      time += (g.wide ? wide_waves : narrow_waves) * kt.umma * k_tiles + kt.predecode;
+      time += (double)(g.n128 + (long long)g.slots128 * tiles_n) * k_tiles * 20480.0 / 5e6;
     }
     if (g.n16) {
       const long long ctas = g.n16 * tiles_n;
