@@ -619,8 +619,10 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
       __syncwarp();
       // (relaxed: the accumulator's values are in registers; a release would wait for the tile's stores to reach memory)
       if (lane == 0) {
-        if constexpr (CTAS == 1) asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&sm.acc_empty[i & 1])) : "memory");
-        else asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(first_cta<CTAS>(&sm.acc_empty[i & 1])) : "memory");
+        if constexpr (CTAS == 1)
+          asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&sm.acc_empty[i & 1])) : "memory");
+        else
+          asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(first_cta<CTAS>(&sm.acc_empty[i & 1])) : "memory");
       }
     }
     if (ok && p.zero_rest)
@@ -802,15 +804,18 @@ cudaError_t launch_out(const Int8Params& p, const Maps& m, int parts, unsigned t
 // Kernel, rows of a tile and parts of K by estimated time, in microseconds. A CTA takes TAU per 128 bytes of K and tile (MMAs of
 // 128 channels take about 120 cycles up to 128 rows); all of them together get L2_RATE out of the caches and HBM_RATE out of
 // memory; the slowest of the three counts, and a part of the first (REST), as they overlap only in part. START and the output of
-// the last tile (OUT per row) come on top, the cluster's sum (SUM, PART each) and every further wave of one-tile CTAs (WAVE). Measured on whole calls, replayed from a graph: 1 to 2048 rows, 512 to 24576 channels, K from 512 to
-// 28672; the choice was within 5 % of the best of all of them for most, within 20 % for all.
+// the last tile (OUT per row) come on top, the cluster's sum (SUM, and PART and SUM_ROW each) and every further wave of one-tile
+// CTAs (WAVE). Two one-tile CTAs on an SM take SHARE times as long as one; memory is up to SPARE slower with few CTAs. Measured
+// on whole calls, replayed from a graph: 117 shapes of 1 to 2048 rows, 512 to 24576 channels, K from 512 to 28672; the choice was
+// within 5 % of the best of all of them for 102, within 15 % for all.
 enum Kind { TILE, SINGLE, PAIR };
 struct Choice { Kind kind; int rows, parts; };
 long long most_row_tiles(const Int8Params& p, int rows) {               // of all groups: every one may end in a partial tile
   return p.offs ? (long long)p.T / rows + (p.E < p.T ? p.E : p.T) : ((long long)p.T + rows - 1) / rows;
 }
 Choice choose(const Int8Params& p) {
-  constexpr double L2_RATE = 14e6, HBM_RATE = 6.1e6, OUT = 0.011, SUM = 1.8, PART = 0.1, WAVE = 2.0, REST = 0.15;
+  constexpr double L2_RATE = 14e6, HBM_RATE = 6.1e6, OUT = 0.011, SUM = 1.8, PART = 0.1, SUM_ROW = 0.02;
+  constexpr double WAVE = 2.0, REST = 0.15, SHARE = 1.6, SPARE = 0.1;
   const long long n_sm = sms(), used = p.E < p.T ? p.E : p.T;             // groups with rows, at most
   const double hbm = ((double)used * p.N + p.T) * p.K / HBM_RATE;
   Choice best{TILE, 16, 1};
@@ -827,10 +832,18 @@ Choice choose(const Int8Params& p) {
     // rows that a tile copies: its own, a one-tile CTA all
     const double copied = kind == TILE ? rows : (double)p.T / tiles_t + (p.T > 64 ? 32 : 0);
     const double l2 = tiles * p.k_blocks * KB * (CH * ctas_per_tile + copied) / L2_RATE;
-    const double mma = tau * p.k_blocks / parts * waves(tiles * parts, workers);
+    const double ctas = tiles * parts;
+    double turns = waves(ctas, workers);                                 // of an SM's tensor pipe
+    if (kind == TILE) {                                                  // two CTAs on an SM overlap
+      const double rounds = waves(ctas, 2.0 * n_sm), rest = ctas - (rounds - 1.0) * 2.0 * n_sm;
+      turns = (rounds - 1.0) * SHARE + (rest <= n_sm ? 1.0 : SHARE);
+    }
+    const double mma = tau * p.k_blocks / parts * turns;
     double t = mma > l2 ? mma : l2;
-    t = t > hbm ? t : hbm;
-    t += REST * mma + start + OUT * rows + (parts > 1 ? SUM + PART * parts : 0.0) + (kind == TILE ? WAVE * (waves(tiles * parts, workers * occupancy) - 1.0) : 0.0);
+    const double memory = hbm * (ctas < 2.0 * n_sm ? 1.0 + SPARE * (1.0 - ctas / (2.0 * n_sm)) : 1.0);
+    t = t > memory ? t : memory;
+    t += REST * mma + start + OUT * rows + (parts > 1 ? SUM + PART * parts + SUM_ROW * rows : 0.0);
+    if (kind == TILE) t += WAVE * (waves(tiles * parts, workers * occupancy) - 1.0);
     if (parts > 1 && tiles * parts > 2.0 * n_sm) return;                 // clusters that wait for room cost more than they save
     if (t < least) {
       least = t;

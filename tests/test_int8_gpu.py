@@ -73,9 +73,10 @@ def test_product_bits(M, N, K, out):
 
 # every kernel, by the rule's choice: (kind, rows of a tile, parts of K) -> rows, channels, K; a worker's second and third tile,
 # ragged rows, channels and K among them
-KERNELS = [((0, 16, 1), 40, 300, 100), ((0, 16, 2), 1, 5000, 2000), ((0, 16, 4), 300, 16, 2000), ((0, 16, 8), 7, 130, 2001),
-           ((0, 32, 1), 3000, 16, 48), ((0, 32, 2), 17, 5000, 2000), ((0, 32, 4), 700, 16, 2000), ((0, 32, 8), 300, 17, 5000),
-           ((0, 64, 1), 33, 20000, 17), ((0, 64, 2), 3000, 16, 5000), ((0, 64, 4), 1500, 16, 2000), ((0, 64, 8), 700, 16, 5000),
+KERNELS = [((0, 16, 1), 40, 300, 100), ((0, 16, 2), 1, 5622, 2083), ((0, 16, 4), 1, 5000, 2000), ((0, 16, 4), 300, 16, 2000), ((0, 16, 8), 7, 130, 2001),
+           ((0, 16, 1), 3000, 16, 48), ((0, 16, 1), 17, 5000, 2000), ((0, 16, 1), 1500, 16, 2000), ((0, 32, 1), 5000, 16, 40),
+           ((0, 32, 2), 17, 5676, 2475), ((0, 32, 4), 700, 16, 2000), ((0, 32, 8), 300, 17, 5000), ((0, 32, 8), 700, 16, 5000),
+           ((0, 64, 1), 33, 20000, 17), ((0, 64, 2), 4631, 16, 3445), ((0, 64, 4), 3000, 16, 5000), ((0, 64, 8), 1500, 16, 5000),
            ((1, 64, 1), 65, 20000, 130), ((1, 128, 1), 1000, 2064, 1936), ((1, 128, 1), 1030, 5000, 300), ((1, 256, 1), 5000, 500, 1000),
            ((2, 256, 1), 2050, 5000, 300), ((2, 256, 1), 2000, 8200, 528)]
 RAGGED = [((0, 16, 8), [0, 33, 0, 1], 16, 5000), ((0, 32, 8), [100, 0, 200], 16, 5000), ((0, 64, 1), [60, 0, 40], 9000, 16), ((1, 64, 1), [25, 0, 70, 3] * 10, 2000, 500),
