@@ -114,9 +114,10 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
         raise ReferenceRejectsError(f"{rule.message} [profile {prof.name}]")
     _check_scope(scaling, None, (mat1, mat2, scale_a, scale_b, scale_result))
     _emit_maturity(prof, preset)
-    layout_std = mat1.is_contiguous() and mat2.stride(1) == 1 and (mat2.stride(2) == K or N == 1)
+    rows_std, weights_std = mat1.is_contiguous(), mat2.stride(1) == 1 and (mat2.stride(2) == K or N == 1)
 
     def plan_of(m):
+        layout_std = weights_std and (rows_std or m == 1)      # one row is contiguous whatever the input's row stride
         d = resolve_splitk(m, N, K, a_dtype=mat1.dtype, b_dtype=mat2.dtype, out_dtype=od, use_fast_accum=fast, profile=prof, splitk=splitk,
                            layout_std=layout_std, dry=False)
         return d.S, check_plan(preset, K, d.S, d.scheme, fast)

@@ -307,3 +307,19 @@ def test_a_wait_that_runs_out_is_reported(sizes, monkeypatch):
     finally:
         L.mmb200_test_hooks(0, 0)
     check(ta, tw, sizes, sa, sb, **kw)
+
+
+@pytest.mark.parametrize("profile,fast,N,K,sizes", [("hopper", False, 2048, 8192, [1, 300, 0, 1]), ("hopper-te", True, 2048, 8192, [300, 1]),
+                                                    ("ada", True, 512, 8192, [1, 600, 1]), ("ada", False, 128, 8192, [1, 0, 1, 1])])
+def test_split_decisions_with_a_padded_input(profile, fast, N, K, sizes):
+    """Rows of a wider buffer: a group of one row is contiguous for scaled_mm and split by the table, a longer one is not."""
+    T = sum(sizes)
+    _, _, ta, tw = operands(sizes, N, K, cls="gauss1", seed=19)
+    home = torch.zeros(T, K + 32, dtype=torch.uint8, device=DEV)
+    home[:, :K] = ta.view(torch.uint8)
+    a2 = home[:, :K].view(ta.dtype)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        assert mm.resolve_splitk(1, N, K, a_dtype=ta.dtype, b_dtype=tw.dtype, out_dtype=torch.bfloat16, use_fast_accum=fast, profile=profile,
+                                 dry=True).S > 1
+    check(a2, tw, sizes, *group_scales(len(sizes)), out_dtype=torch.bfloat16, profile=profile, use_fast_accum=fast)

@@ -205,3 +205,37 @@ def test_argument_checks_of_the_emulated_grouped_entry_point(lib):
     # the decoded operands of all groups would take 16 GB: group by group
     most = (ctypes.c_int * 64)(*[100] * 64)
     assert need(most, None, 64, 8192, 8192, 0, 0, 32, 1) < 1 << 30
+
+
+@pytest.mark.parametrize("profile", ["hopper", "hopper-te", "ada"])
+@pytest.mark.parametrize("pad", [0, 16])
+@pytest.mark.parametrize("sizes", [[1, 1], [1, 128], [128, 0, 1], [16, 64, 1, 1], [1]])
+def test_split_decisions_are_those_of_the_loop(sizes, pad, profile, monkeypatch):
+    """splitk="auto": the layout that the decision goes by is each group's own (one row of a padded input is contiguous). What every
+    group resolves to, or the error that the first undecided one raises, is what scaled_mm of the group has."""
+    from mmaemu_b200 import api
+    from mmaemu_b200 import grouped as grouped_module
+    f, N, K = torch.float8_e4m3fn, 2048, 2048
+    a, w = z(sum(sizes), K + pad, dtype=f)[:, :K], z(len(sizes), N, K, dtype=f)
+    kw = dict(out_dtype=torch.bfloat16, profile=profile)
+    seen = {}
+
+    def record(M, *args, **kwargs):
+        seen[M] = None
+        d = mm.resolve_splitk(M, *args, **kwargs)
+        seen[M] = (d.S, d.scheme, d.source)
+        return d
+
+    monkeypatch.setattr(api, "resolve_splitk", record)
+    monkeypatch.setattr(grouped_module, "resolve_splitk", record)
+    loop, start = {}, 0
+    for e, m in enumerate(sizes):
+        if m:
+            with pytest.raises((mm.BackendUnavailableError, mm.SplitKUnknownError)):
+                mm.scaled_mm(a[start:start + m], w[e].t(), ONE, ONE, **kw)
+        start += m
+    loop, seen = seen, {}
+    undecided = any(d is None for d in loop.values())
+    with pytest.raises(mm.SplitKUnknownError if undecided else mm.BackendUnavailableError):
+        mm.grouped_scaled_mm(a, w.transpose(1, 2), sizes, ONE, ONE, **kw)
+    assert undecided or seen == loop
