@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define MMB200_ABI_VERSION 5
+#define MMB200_ABI_VERSION 6
 
 /* status codes */
 #define MMB200_OK 0
@@ -235,12 +235,14 @@ int mmb200_kernel_for(const void *A_dev, int64_t lda, const void *B_dev, int64_t
  * mmb200_scaled_mm_ws calls, whatever kernel runs. m_splits, splits and schemes are HOST arrays of E entries, read during
  * the call (the split decision of the emulated platform depends on a group's rows). With scratch memory the unsplit groups
  * run in one pass of launches (up to 8 GiB of decoded operands), the others one after the other. Scratch memory as there:
- * mmb200_grouped_workspace_bytes; mmb200_grouped_status synchronises `stream` and reports whether a bounded wait of the call
+ * mmb200_grouped_workspace_bytes, or, where that much is not to be had, mmb200_grouped_workspace_bytes_one_by_one, with which
+ * every group runs by itself on the scratch-memory kernels; mmb200_grouped_status synchronises `stream` and reports whether a bounded wait of the call
  * that last used it ran out (the outputs of that group then keep their previous contents). The reference has no grouped
  * call. */
 #define MMB200_MAX_GROUPS 4096
 size_t mmb200_grouped_workspace_bytes(const int *m_splits, const int *splits, int E, int N, int K, int fmt_a, int fmt_b,
                                       int nfma, int fast);
+size_t mmb200_grouped_workspace_bytes_one_by_one(const int *m_splits, const int *splits, int E, int N, int K);
 int mmb200_grouped_scaled_mm(const void *A_dev, int64_t lda, int fmt_a, const void *B_dev, int64_t ldb,
                              int64_t group_stride_b, int fmt_b, void *D_dev, int64_t ldd, int out_dtype,
                              const int *m_splits, const int *splits, const int *schemes, int E, int N, int K, int nfma,

@@ -13,7 +13,7 @@ from pathlib import Path
 from .errors import BackendUnavailableError
 
 LIB_PATH = Path(__file__).resolve().parent / "libmmaemu_b200.so"
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 FMT_CODES = {"e4m3": 0, "e5m2": 1}
 OUT_CODES = {"float32": 0, "bfloat16": 1, "float16": 2, "float8_e4m3fn": 3, "float8_e5m2": 4}
@@ -26,7 +26,8 @@ EXPORTS = ("mmb200_abi_version", "mmb200_status_string", "mmb200_last_cuda_error
            "mmb200_launch_count", "mmb200_workspace_bytes", "mmb200_workspace_bytes_split", "mmb200_scaled_mm_ws", "mmb200_accumulate_ws",
            "mmb200_scaled_mm_static", "mmb200_quantize_scaled_mm_ws", "mmb200_workspace_status_offset",
            "mmb200_workspace_status", "mmb200_scaled_mm_static_status", "mmb200_test_hooks", "mmb200_scaled_mm_peers", "mmb200_probe_issue_rate",
-           "mmb200_grouped_workspace_bytes", "mmb200_grouped_scaled_mm", "mmb200_grouped_status", "mmb200_quantize_int8", "mmb200_int8_workspace_bytes",
+           "mmb200_grouped_workspace_bytes", "mmb200_grouped_workspace_bytes_one_by_one", "mmb200_grouped_scaled_mm", "mmb200_grouped_status",
+           "mmb200_quantize_int8", "mmb200_int8_workspace_bytes",
            "mmb200_int8_scaled_mm", "mmb200_int8_kernel_for", "mmb200_int8_status")
 
 # mmb200_int8_args as bytes: one argument instead of 25, whose conversion took 3 us of a call
@@ -110,6 +111,8 @@ def load():
         sz = ctypes.c_size_t
         L.mmb200_grouped_workspace_bytes.argtypes = [vp, vp, ci, ci, ci, ci, ci, ci, ci]
         L.mmb200_grouped_workspace_bytes.restype = sz
+        L.mmb200_grouped_workspace_bytes_one_by_one.argtypes = [vp, vp, ci, ci, ci]
+        L.mmb200_grouped_workspace_bytes_one_by_one.restype = sz
         L.mmb200_grouped_scaled_mm.argtypes = [vp, i64, ci, vp, i64, i64, ci, vp, i64, ci, vp, vp, vp, ci, ci, ci, ci, ci, vp, i64,
                                                vp, i64, vp, ci, vp, sz, vp]
         L.mmb200_grouped_scaled_mm.restype = ci

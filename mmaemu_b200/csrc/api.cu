@@ -559,6 +559,17 @@ size_t fused_bytes(const mmb::Params& p, int nfma, const int* m_splits, const Fu
 }
 }  // namespace
 
+// Scratch memory of the groups that the fused launches do not take, one after the other (fused null: of all groups).
+static size_t one_by_one_bytes(const int* m_splits, const int* splits, const FusedGroups* fused, int E, int N, int K) {
+  size_t most = 0;
+  for (int e = 0; e < E; ++e) {
+    if (m_splits[e] <= 0 || (fused && fused->use[e])) continue;
+    const size_t n = mmb::staged_workspace_bytes(m_splits[e], N, K, splits ? splits[e] : 1, true, false, mmb::tensor_cores_off());
+    if (n > most) most = n;
+  }
+  return most ? GROUPED_HEADER + most : 0;
+}
+
 size_t mmb200_grouped_workspace_bytes(const int* m_splits, const int* splits, int E, int N, int K, int fmt_a, int fmt_b, int nfma,
                                       int fast) {
   if (!m_splits || E <= 0 || E > MMB200_MAX_GROUPS || N <= 0 || K <= 0) return 0;
@@ -568,14 +579,13 @@ size_t mmb200_grouped_workspace_bytes(const int* m_splits, const int* splits, in
   const mmb::Params p = grouped_params(rows, N, K, fmt_a, fmt_b, fast);
   const FusedGroups groups(m_splits, splits, E);
   const size_t fused = fused_bytes(p, nfma, m_splits, groups, E);
-  size_t most = 0;
-  for (int e = 0; e < E; ++e) {
-    if (m_splits[e] <= 0 || (fused && groups.use[e])) continue;
-    const size_t n = mmb::staged_workspace_bytes(m_splits[e], N, K, splits ? splits[e] : 1, true, false, mmb::tensor_cores_off());
-    if (n > most) most = n;
-  }
-  most = most ? GROUPED_HEADER + most : 0;
+  const size_t most = one_by_one_bytes(m_splits, splits, fused ? &groups : nullptr, E, N, K);
   return fused > most ? fused : most;
+}
+
+size_t mmb200_grouped_workspace_bytes_one_by_one(const int* m_splits, const int* splits, int E, int N, int K) {
+  if (!m_splits || E <= 0 || E > MMB200_MAX_GROUPS || N <= 0 || K <= 0) return 0;
+  return one_by_one_bytes(m_splits, splits, nullptr, E, N, K);
 }
 
 int mmb200_grouped_status(const void* workspace, void* stream) {

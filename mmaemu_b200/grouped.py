@@ -69,6 +69,22 @@ def _plainly_valid(input, mat2, scale_a, scale_b, scale_result, out_dtype, out) 
             and index == scale_a.get_device() and index == scale_b.get_device() and scale_a.dtype == scale_b.dtype == torch.float32)
 
 
+def _scratch(L, input, kernel, sizes, plan):
+    """(tensor or None, pointer or None, bytes) of the scratch memory: for all groups at once (about four times the operands), where
+    the device has too little left for that for one group after the other, as a loop of scaled_mm calls would have it, else none."""
+    n = L.mmb200_grouped_workspace_bytes(*sizes, *plan)
+    while n:
+        try:
+            ws = input.new_empty(n, dtype=torch.uint8)
+            return ws, ws.data_ptr(), n
+        except torch.OutOfMemoryError:
+            one_by_one = L.mmb200_grouped_workspace_bytes_one_by_one(*sizes)
+            if one_by_one >= n and kernel != "auto":
+                raise                                    # a request for the fast kernels by name
+            n = one_by_one if one_by_one < n else 0
+    return None, None, 0
+
+
 def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None, out_dtype=None, use_fast_accum=False, *,
                       out=None, profile=None, splitk="auto", backend="auto"):
     """scaled_mm of every group of rows, bit for bit: the first m_splits[0] rows of input [T, K] with mat2[0], the next
@@ -149,16 +165,8 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
     with _on_device(dev):
         ws, ws_ptr, n = None, None, 0
         if kernel not in ("integer", "direct") and not preset.late_c and os.environ.get("MMAEMU_B200_WORKSPACE", "1") != "0":
-            n = int(L.mmb200_grouped_workspace_bytes(rows, splits, E, N, K, _lib.FMT_CODES[fa], _lib.FMT_CODES[fb], preset.code,
-                                                     int(fast)))
-            if n:
-                try:
-                    ws = input.new_empty(n, dtype=torch.uint8)
-                    ws_ptr = ws.data_ptr()
-                except torch.OutOfMemoryError:
-                    if kernel != "auto":
-                        raise                            # a request for the fast kernels by name
-                    n = 0
+            ws, ws_ptr, n = _scratch(L, input, kernel, (rows, splits, E, N, K), (_lib.FMT_CODES[fa], _lib.FMT_CODES[fb], preset.code,
+                                                                                int(fast)))
         rc = L.mmb200_grouped_scaled_mm(mat1.data_ptr(), lda, _lib.FMT_CODES[fa], mat2.data_ptr(), ldb, mat2.stride(0) if E > 1 else 0,
                                         _lib.FMT_CODES[fb], y.data_ptr(), y.stride(0) if T > 1 else N,
                                         _lib.OUT_CODES[OUT_DTYPE_NAMES[od]], rows, splits, schemes, E, N, K, preset.code, int(fast),

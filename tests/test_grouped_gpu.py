@@ -323,3 +323,45 @@ def test_split_decisions_with_a_padded_input(profile, fast, N, K, sizes):
         assert mm.resolve_splitk(1, N, K, a_dtype=ta.dtype, b_dtype=tw.dtype, out_dtype=torch.bfloat16, use_fast_accum=fast, profile=profile,
                                  dry=True).S > 1
     check(a2, tw, sizes, *group_scales(len(sizes)), out_dtype=torch.bfloat16, profile=profile, use_fast_accum=fast)
+
+
+@pytest.mark.parametrize("splitk", [1, (2, "contiguous")])
+@pytest.mark.parametrize("fast", [True, False])
+def test_without_memory_for_the_scratch_of_all_groups(fast, splitk, monkeypatch):
+    """Where the decoded operands of all groups do not fit, every group runs on the scratch-memory kernels by itself; without memory
+    for that either, on the kernels that need none. The allocations fail because the test makes them fail."""
+    monkeypatch.setenv("MMAEMU_B200_ROW_GROUPS", "0")                # 128-row tiles, whose operands are decoded into scratch memory
+    sizes = [130, 0, 200, 40] * 6
+    E = len(sizes)
+    _, _, ta, tw = operands(sizes, 400, 272, seed=20)
+    sa, sb = group_scales(E)
+    kw = dict(out_dtype=torch.bfloat16, profile="hopper", splitk=splitk, use_fast_accum=fast)
+    L = _lib.load()
+    want = loop(ta, tw, sizes, sa, sb, **kw)
+    before = L.mmb200_launch_count()
+    loop(ta, tw, sizes, sa, sb, **kw)
+    launches_of_loop = L.mmb200_launch_count() - before
+    new_empty, asked, most = torch.Tensor.new_empty, [], [0]
+
+    def limited(self, size, *args, dtype=None, **kwargs):
+        if dtype is torch.uint8:
+            asked.append(size)
+            if size > most[0]:
+                raise torch.OutOfMemoryError("no memory left")
+        return new_empty(self, size, *args, dtype=dtype, **kwargs)
+
+    monkeypatch.setattr(torch.Tensor, "new_empty", limited)
+    one_by_one = L.mmb200_grouped_workspace_bytes_one_by_one((ctypes.c_int * E)(*sizes), None if splitk == 1 else (ctypes.c_int * E)(*[2, 1, 2, 2] * 6),
+                                                             E, 400, 272)
+    for backend in ("auto", "cuda:b200-fast"):
+        most[0] = one_by_one
+        asked.clear()
+        before = L.mmb200_launch_count()
+        y = mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, backend=backend, **kw)
+        assert asked[-1] == one_by_one and (len(asked) == 2 or splitk != 1)
+        assert L.mmb200_launch_count() - before == launches_of_loop
+        assert np.array_equal(bits(y), bits(want))
+    most[0] = 0
+    assert np.array_equal(bits(mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, **kw)), bits(want))
+    with pytest.raises(torch.OutOfMemoryError):
+        mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, backend="cuda:b200-fast", **kw)

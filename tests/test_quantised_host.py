@@ -239,3 +239,16 @@ def test_split_decisions_are_those_of_the_loop(sizes, pad, profile, monkeypatch)
     with pytest.raises(mm.SplitKUnknownError if undecided else mm.BackendUnavailableError):
         mm.grouped_scaled_mm(a, w.transpose(1, 2), sizes, ONE, ONE, **kw)
     assert undecided or seen == loop
+
+
+def test_scratch_memory_of_groups_one_after_the_other(lib):
+    """What a call asks for where there is no room for the decoded operands of all groups: the largest group's, by itself."""
+    ints = lambda *v: (ctypes.c_int * len(v))(*v)  # noqa: E731
+    one = lib.mmb200_grouped_workspace_bytes_one_by_one
+    alone = [lib.mmb200_workspace_bytes_split(m, 4096, 4096, 1) for m in (128, 300)]
+    assert one(ints(128, 0, 300, 128), None, 4, 4096, 4096) == 256 + max(alone)
+    many = ints(*[128] * 32)
+    assert one(many, None, 32, 4096, 4096) == 256 + alone[0] < lib.mmb200_grouped_workspace_bytes(many, None, 32, 4096, 4096, 0, 0, 32, 0) / 8
+    split = lib.mmb200_workspace_bytes_split(128, 4096, 4096, 4)
+    assert one(ints(128, 300), ints(4, 1), 2, 4096, 4096) == 256 + max(split, alone[1])
+    assert one(ints(0, 0), None, 2, 64, 64) == 0 and one(None, None, 2, 64, 64) == 0 and one(ints(5), None, 0, 64, 64) == 0
