@@ -7,7 +7,7 @@
  * status, never throw and never abort. Mutable state of the library: per-device function attributes that are set once;
  * the per-device memory pool, internal streams and events of mmb200_scaled_mm_host; the fixed scratch array of mmb200_scaled_mm_static with its
  * cached per-device address; the launch counter; the process-wide test hooks of mmb200_test_hooks; the per-device status
- * word of the int8 kernels (mmb200_int8_status).
+ * words of the int8 kernels (mmb200_int8_status).
  *
  * Operands are FP8 code bytes: A is [M, K] row-major with leading dimension lda (bytes), B is [N, K] row-major with
  * leading dimension ldb -- that is mat2.t() of torch._scaled_mm's column-major [K, N] operand.
@@ -297,9 +297,10 @@ int mmb200_int8_scaled_mm(const mmb200_int8_args *args);
  * cluster of `parts` CTAs shares a tile), 1: persistent CTAs, 2: persistent pairs of CTAs. ragged: whether offs_dev is given.
  * Pure host logic (148 SMs are assumed where no device answers). */
 int mmb200_int8_kernel_for(int T, int N, int K, int E, int ragged);
-/* Synchronises `stream`, reads and clears the current device's status word of the int8 kernels: MMB200_ERR_TIMEOUT when a
- * bounded wait has run out since the word was last read (outputs of that call are unspecified), else MMB200_OK. With
- * MMAEMU_B200_CHECK_STATUS=1 in the environment mmb200_int8_scaled_mm ends with this call. */
+/* Synchronises `stream`: MMB200_ERR_TIMEOUT when a bounded wait of an int8 kernel has run out on the current device since the
+ * last such call, else MMB200_OK. One word for the calls of all streams and threads: it does not say whose outputs are unspecified.
+ * With MMAEMU_B200_CHECK_STATUS=1 in the environment mmb200_int8_scaled_mm counts on a word of its own instead, synchronises its
+ * stream and returns MMB200_ERR_TIMEOUT itself (up to 64 such calls at once on a device; the next one waits for one of them). */
 int mmb200_int8_status(void *stream);
 
 /* Issue-rate probe for roofline denominators: launches `ctas` blocks of 256 threads in which every thread executes

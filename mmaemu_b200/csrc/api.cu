@@ -1,5 +1,7 @@
 // Host side of the C ABI (include/mmaemu_b200.h): argument checks, kernel choice, launches. No allocation except in
 // mmb200_scaled_mm_host, which stages host operands through the stream-ordered allocator.
+#include <sched.h>
+
 #include <atomic>
 #include <mutex>
 #include <cstdlib>
@@ -714,6 +716,45 @@ size_t mmb200_int8_workspace_bytes(const int8_t* A, int64_t lda, const int8_t* W
   return mmb::int8_workspace_bytes(p);
 }
 
+namespace {
+// The status words of the int8 kernels on one device. A word only counts up; `seen` is what it was when it was last read, so that
+// no count is lost between a reader's copy and its note, whatever streams the two run on. Words 1 and up belong to one call each
+// while it runs (`busy`).
+struct Int8Status {
+  std::atomic<uint64_t> busy{0};
+  std::atomic<int> seen[mmb::INT8_STATUS_WORDS] = {};
+};
+static_assert(mmb::INT8_STATUS_WORDS == 65, "a bit of `busy` for each but the first");
+Int8Status* int8_status_here() {
+  static Int8Status devices[64];
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? &devices[dev] : nullptr;
+}
+// After the stream has drained: whether the word has gone up since it was last read.
+int read_int8_status(Int8Status& s, int index, cudaStream_t st) {
+  int* words = nullptr;
+  int now = 0;
+  cudaError_t err = mmb::int8_status_words(&words);
+  if (err == cudaSuccess) err = cudaMemcpyAsync(&now, words + index, sizeof(int), cudaMemcpyDeviceToHost, st);
+  if (err == cudaSuccess) err = cudaStreamSynchronize(st);
+  if (err != cudaSuccess) return cuda_fail(err);
+  int last = s.seen[index].load();
+  while ((int)((unsigned)now - (unsigned)last) > 0)
+    if (s.seen[index].compare_exchange_weak(last, now)) return MMB200_ERR_TIMEOUT;
+  return MMB200_OK;
+}
+// A word for one call; with 64 checked calls in flight on the device, the next one waits for one of them.
+int take_int8_word(Int8Status& s) {
+  for (;;) {
+    uint64_t busy = s.busy.load();
+    const int bit = ~busy ? __builtin_ctzll(~busy) : -1;
+    if (bit >= 0 && s.busy.compare_exchange_weak(busy, busy | (1ull << bit))) return 1 + bit;
+    if (bit < 0) sched_yield();
+  }
+}
+void release_int8_word(Int8Status& s, int index) { s.busy.fetch_and(~(1ull << (index - 1))); }
+}  // namespace
+
 int mmb200_int8_scaled_mm(const mmb200_int8_args* a) {
   static_assert(sizeof(mmb200_int8_args) == 25 * 8, "packed by bindings");
   if (!a || a->T < 0 || a->N < 0 || a->K < 0 || a->E < 1 || (!a->offs_dev && a->E != 1)) return MMB200_ERR_BAD_ARG;
@@ -743,12 +784,25 @@ int mmb200_int8_scaled_mm(const mmb200_int8_args* a) {
   const size_t need = mmb::int8_workspace_bytes(p);
   if (need && (!a->workspace_dev || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace_dev) & 15)))
     return MMB200_ERR_BAD_ARG;
+  const char* check = std::getenv("MMAEMU_B200_CHECK_STATUS");
+  Int8Status* checked = check && check[0] == '1' && !check[1] ? int8_status_here() : nullptr;
+  int word = 0;
+  if (checked) {
+    int* words = nullptr;
+    const cudaError_t err = mmb::int8_status_words(&words);
+    if (err != cudaSuccess) return cuda_fail(err);
+    word = take_int8_word(*checked);
+    p.status = words + word;
+  }
   int launches = 0;
   const cudaError_t err = mmb::launch_int8(p, a->workspace_dev, static_cast<cudaStream_t>(a->stream), &launches);
   g_launches.fetch_add(launches, std::memory_order_relaxed);
-  if (err != cudaSuccess) return cuda_fail(err);
-  const char* check = std::getenv("MMAEMU_B200_CHECK_STATUS");
-  return check && check[0] == '1' && !check[1] ? mmb200_int8_status(a->stream) : MMB200_OK;
+  int result = err == cudaSuccess ? MMB200_OK : cuda_fail(err);
+  if (checked) {
+    if (result == MMB200_OK) result = read_int8_status(*checked, word, static_cast<cudaStream_t>(a->stream));
+    release_int8_word(*checked, word);
+  }
+  return result;
 }
 
 int mmb200_int8_kernel_for(int T, int N, int K, int E, int ragged) {
@@ -764,15 +818,8 @@ int mmb200_int8_kernel_for(int T, int N, int K, int E, int ragged) {
 int mmb200_int8_status(void* stream) {
   const int rc = current_device_ok();
   if (rc != MMB200_OK) return rc;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int* word = nullptr;
-  int seen = 0;
-  cudaError_t err = mmb::int8_status_word(&word);
-  if (err == cudaSuccess) err = cudaMemcpyAsync(&seen, word, sizeof(int), cudaMemcpyDeviceToHost, st);
-  if (err == cudaSuccess) err = cudaMemsetAsync(word, 0, sizeof(int), st);
-  if (err == cudaSuccess) err = cudaStreamSynchronize(st);
-  if (err != cudaSuccess) return cuda_fail(err);
-  return seen ? MMB200_ERR_TIMEOUT : MMB200_OK;
+  Int8Status* s = int8_status_here();
+  return s ? read_int8_status(*s, 0, static_cast<cudaStream_t>(stream)) : MMB200_ERR_UNSUPPORTED;
 }
 
 int mmb200_kernel_for(const void* A, int64_t lda, const void* B, int64_t ldb, int K, int nfma, int S) {

@@ -27,7 +27,7 @@ struct Int8Params {
   const float* scale_b;   // [E, N] (sb_group, sb_stride), [N] or one
   const void* bias;       // null, or [E, N] (group stride bias_group)
   const int* offs;        // ends of the groups [E]; null: one group of all T rows
-  int* status;            // device word: 1 when a bounded wait ran out
+  int* status;            // device word that bounded waits count up when they run out; null: the device's common one
   long long lda, ldw, gsw, ldd, sa_stride, sb_stride, sb_group, bias_group;
   int T, N, K, E;
   int bias_dtype, out_dtype;
@@ -39,7 +39,9 @@ struct Int8Params {
 size_t int8_workspace_bytes(const Int8Params& p);
 cudaError_t launch_int8(const Int8Params& p, void* workspace, cudaStream_t st, int* launches);
 int int8_kernel_for(const Int8Params& p);       // mmb200_int8_kernel_for
-// The device's status word (zero until a bounded wait of an int8 kernel runs out).
-cudaError_t int8_status_word(int** word);
+// The current device's status words, which bounded waits of the int8 kernels count up when they run out (and nobody clears): the
+// common one, then those of the calls that check their own waits.
+constexpr int INT8_STATUS_WORDS = 65;
+cudaError_t int8_status_words(int** words);
 
 }  // namespace mmb

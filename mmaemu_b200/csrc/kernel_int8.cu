@@ -32,7 +32,7 @@
 namespace mmb {
 namespace {
 
-__device__ int g_int8_status;
+__device__ int g_int8_status[INT8_STATUS_WORDS];
 
 constexpr int CH = 128;                    // output channels of a tile
 constexpr int KB = 128;                    // bytes of K per stage: one 128-byte swizzle atom
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
     if (!mbar_wait(&sm.done, 0, p.wait_polls)) ok = false;
     fence_after();
   }
-  if (!ok) atomicExch(p.status, 1);
+  if (!ok) atomicAdd(p.status, 1);
   const bool bad = __syncthreads_or(ok ? 0 : 1) != 0;
   const int lane_ch = 32 * (warp % 4) + lane, n = n0 + lane_ch;
   const uint32_t mine = tmem + ((uint32_t)(32 * (warp % 4)) << 16);
@@ -628,7 +628,7 @@ __device__ __forceinline__ void int8_worker(const CUtensorMap& map_w, const CUte
     if (ok && p.zero_rest)
       zero_rows<OUT>(p, sm.groups[p.E - 1].end + (int)blockIdx.x, (int)gridDim.x, 0, p.N, threadIdx.x - 64, WORKER_THREADS - 64);
   }
-  if (!ok) atomicExch(p.status, 1);
+  if (!ok) atomicAdd(p.status, 1);
   fence_before();
   __syncthreads();
   if constexpr (CTAS == 2) {
@@ -864,14 +864,14 @@ Choice choose(const Int8Params& p) {
 
 }  // namespace
 
-cudaError_t int8_status_word(int** word) {
+cudaError_t int8_status_words(int** words) {
   static std::atomic<int*> cached[64];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  if (dev >= 0 && dev < 64 && (*word = cached[dev].load(std::memory_order_acquire)) != nullptr) return cudaSuccess;
-  err = cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_int8_status);
-  if (err == cudaSuccess && dev >= 0 && dev < 64) cached[dev].store(*word, std::memory_order_release);
+  if (dev >= 0 && dev < 64 && (*words = cached[dev].load(std::memory_order_acquire)) != nullptr) return cudaSuccess;
+  err = cudaGetSymbolAddress(reinterpret_cast<void**>(words), g_int8_status);
+  if (err == cudaSuccess && dev >= 0 && dev < 64) cached[dev].store(*words, std::memory_order_release);
   return err;
 }
 
@@ -893,7 +893,7 @@ int int8_kernel_for(const Int8Params& p_in) {
 cudaError_t launch_int8(const Int8Params& p_in, void* workspace, cudaStream_t st, int* launches) {
   Int8Params p = p_in;
   staged_wait_limits(&p.wait_polls, &p.announce_extra);
-  cudaError_t err = int8_status_word(&p.status);
+  cudaError_t err = p.status ? cudaSuccess : int8_status_words(&p.status);
   if (err != cudaSuccess) return err;
   int8_t* ws = static_cast<int8_t*>(workspace);
   if (p.K > 0) {

@@ -12,7 +12,8 @@ with one rounding for the product and the bias together (+0 without one, so a ze
 `scaled_mm` with a scale for each row and column.
 The reference has no int8 path. Errors are TypeError for argument types, ValueError for shapes, layouts and devices,
 UnsupportedFeatureError for inputs that require grad, BackendUnavailableError without an sm_100 device. Calls run on the
-current stream of the operands' device, do not synchronise and can be captured into CUDA graphs.
+current stream of the operands' device, do not synchronise and can be captured into CUDA graphs. With
+$MMAEMU_B200_CHECK_STATUS=1 a product waits for its own kernels and raises when one of their bounded waits has run out.
 """
 from __future__ import annotations
 

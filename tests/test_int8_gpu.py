@@ -560,3 +560,45 @@ def test_a_wait_that_runs_out_is_reported(M, N, K):
     assert L.mmb200_int8_status(st) == _lib.ERR_TIMEOUT
     assert L.mmb200_int8_status(st) == _lib.OK                       # read once
     same(mm.int8_scaled_mm(a, w.t(), one, one), want)
+
+
+def test_a_checked_call_reports_its_own_waits_only(monkeypatch):
+    """A wait that has run out in another call is neither raised by a checked call nor taken from the device's word by it, and
+    the other way round."""
+    M, N, K = 4, 512, 2048
+    a, w, one = codes(M, K, seed=1), codes(N, K, seed=2), torch.ones(1, device=DEV)
+    want = mm.int8_scaled_mm(a, w.t(), one, one)
+    L = _lib.load()
+    st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert L.mmb200_int8_status(st) == _lib.OK
+    L.mmb200_test_hooks(200, 16)
+    try:
+        mm.int8_scaled_mm(a, w.t(), one, one)
+        torch.cuda.synchronize()
+    finally:
+        L.mmb200_test_hooks(0, 0)
+    monkeypatch.setenv("MMAEMU_B200_CHECK_STATUS", "1")
+    got = []
+
+    def run():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got.extend(mm.int8_scaled_mm(a, w.t(), one, one) for _ in range(10))
+
+    threads = [threading.Thread(target=run) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 40
+    for y in got:
+        same(y, want)
+    assert L.mmb200_int8_status(st) == _lib.ERR_TIMEOUT              # the unchecked call's
+    L.mmb200_test_hooks(200, 16)
+    try:
+        for _ in range(70):                                          # more calls than there are words
+            with pytest.raises(_lib.NativeError):
+                mm.int8_scaled_mm(a, w.t(), one, one)
+    finally:
+        L.mmb200_test_hooks(0, 0)
+    assert L.mmb200_int8_status(st) == _lib.OK
+    same(mm.int8_scaled_mm(a, w.t(), one, one), want)
