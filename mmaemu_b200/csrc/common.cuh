@@ -43,7 +43,7 @@ struct Params {
   int* ws_flag_a;
   int* ws_flag_b;
   int* status;
-  int* status_word;      // caller's status word instead of the one in the scratch memory (a word for several launches), or null
+  int* status_word;      // a word for all launches of the call besides the launch's own in the scratch memory, or null
   int k_tiles;
   // B decoded by an earlier launch (the host-buffer entry point decodes B once and runs the rows of A slab by slab):
   // shared_b holds B's tile images followed by its column flags (staged_shared_b_bytes); the launch then neither

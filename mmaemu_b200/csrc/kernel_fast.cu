@@ -584,7 +584,8 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(const __grid_constant_
   const RowTile rt = row_tile<GROUPED, BM>(p, tile_m);
   const int gm = rt.m0 + (p.umma ? lin % BM : ln.row(i)), gn = tile_n * BN + (p.umma ? lin / BM : ln.col(j));
   if (gm >= rt.m_end || gn >= p.N) return;
-  if (p.status && *reinterpret_cast<volatile int*>(p.status)) return;   // a slice gave up waiting: no output, as in the other modes
+  // a slice gave up waiting: no output, as in the other modes (the 16-row kernels of ragged groups do not wait)
+  if (!GROUPED && p.status && *reinterpret_cast<volatile int*>(p.status)) return;
   constexpr size_t STRIDE = (size_t)(GROUPED ? 2 : TM) * TN * THREADS;
   const float* src = p.ws_chains + (size_t)blockIdx.x * p.n_chains * STRIDE + (size_t)idx * THREADS + tid;
   const bool slow = p.plan_group != 0;
@@ -891,7 +892,7 @@ __device__ __forceinline__ void staged_body(const Params& p, unsigned char* smem
   for (int t = 0; t < T; ++t) {
     if (ok && !mbar_wait(&sm.full[t % NST], (t / NST) & 1, p.wait_polls)) {
       ok = false;                          // give up: no further reads of the ring, the output is not written
-      if (p.status) atomicExch(p.status, 1);
+      record_timeout(p);
     }
     if (ok) {
       landed = t + 1;
@@ -914,7 +915,7 @@ __device__ __forceinline__ void staged_body(const Params& p, unsigned char* smem
     if (tid == 0 && r >= 0 && r + NST < T) {
       if (ok && !mbar_wait(&sm.empty[r % NST], (r / NST) & 1, p.wait_polls)) {
         ok = false;
-        if (p.status) atomicExch(p.status, 1);
+        record_timeout(p);
       }
       if (ok) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // order the generic reads before the async writes
@@ -1524,7 +1525,7 @@ cudaError_t launch_staged(const Params& p_in, int nfma, void* workspace, size_t 
   }
   p.only_b = 0;
   p.byte_loads = vector_loads(p) ? 0 : 1;
-  p.status = p.status_word ? p.status_word : reinterpret_cast<int*>(base + w.status);
+  p.status = reinterpret_cast<int*>(base + w.status);
   p.plan_group = plan.group;
   staged_wait_limits(&p.wait_polls, &p.test_announce_extra);
   cudaError_t err = cudaMemsetAsync(base + w.flag_a, 0, w.a - w.flag_a, stream);     // row flags and status word

@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) umma_kernel(const __grid_cons
     }
   }
   // One decision for the whole CTA; after it no MMA and no copy touches the stages.
-  if (!ok && p.status) atomicExch(p.status, 1);
+  if (!ok) record_timeout(p);
   const bool bad = __syncthreads_or(ok ? 0 : 1) != 0;
   if (!SLICED && !bad && warp < EPI_WARPS) {           // a K slice has stored its chains; the combine kernel writes the output
     Epilogue epi;

@@ -180,6 +180,12 @@ __device__ __forceinline__ bool mbar_wait(unsigned long long* bar, uint32_t pari
   }
   return false;
 }
+// A bounded wait has run out: noted in the launch's own word, by which its second pass goes, and in the call's, if it has several
+// launches.
+__device__ __forceinline__ void record_timeout(const Params& p) {
+  if (p.status) atomicExch(p.status, 1);
+  if (p.status_word) atomicExch(p.status_word, 1);
+}
 // Bulk copy global -> shared (both 16-byte aligned, size a multiple of 16), completion counted on `bar`.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, unsigned long long* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"

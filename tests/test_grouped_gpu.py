@@ -365,3 +365,43 @@ def test_without_memory_for_the_scratch_of_all_groups(fast, splitk, monkeypatch)
     assert np.array_equal(bits(mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, **kw)), bits(want))
     with pytest.raises(torch.OutOfMemoryError):
         mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, backend="cuda:b200-fast", **kw)
+
+
+@pytest.mark.parametrize("one_by_one", [False, True])
+@pytest.mark.parametrize("sizes", [[300, 5, 0, 3], [2, 130, 16]])
+def test_a_wait_that_runs_out_in_one_group_leaves_the_others_written(sizes, one_by_one, monkeypatch):
+    """The test hook makes the waits of the 128-row tiles run out; groups of few rows (K slices and their combination) do not wait
+    and are written, in the fused launches and one after the other. The call's status word tells."""
+    from mmaemu_b200 import grouped as grouped_module
+    monkeypatch.setenv("MMAEMU_B200_ROW_GROUPS", "0")                # more than 16 rows: 128-row tiles, whose copies are waited for
+    E, N, K = len(sizes), 256, 1024
+    _, _, ta, tw = operands(sizes, N, K, seed=21)
+    sa, sb = group_scales(E)
+    kw = dict(profile="hopper", splitk=1)
+    want = loop(ta, tw, sizes, sa, sb, out_dtype=torch.float32, **kw)
+    out = torch.full((sum(sizes), N), 7.0, device=DEV)
+    L = _lib.load()
+    kept = []
+
+    def scratch(L, input, kernel, shape, plan):
+        n = L.mmb200_grouped_workspace_bytes_one_by_one(*shape) if one_by_one else L.mmb200_grouped_workspace_bytes(*shape, *plan)
+        kept.append(torch.empty(n, dtype=torch.uint8, device=DEV))
+        return kept[-1], kept[-1].data_ptr(), n
+
+    monkeypatch.setattr(grouped_module, "_scratch", scratch)
+    L.mmb200_test_hooks(200, 16)
+    try:
+        mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, out=out, **kw)
+        torch.cuda.synchronize()
+    finally:
+        L.mmb200_test_hooks(0, 0)
+    start = 0
+    for m in sizes:
+        rows = slice(start, start + m)
+        assert np.array_equal(bits(out[rows]), bits(want[rows])) if m <= 16 else (out[rows] == 7.0).all(), m
+        start += m
+    st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert L.mmb200_grouped_status(kept[0].data_ptr(), st) == _lib.ERR_TIMEOUT
+    mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, out=out, **kw)
+    assert np.array_equal(bits(out), bits(want))
+    assert L.mmb200_grouped_status(kept[1].data_ptr(), st) == _lib.OK
