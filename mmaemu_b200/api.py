@@ -297,6 +297,8 @@ def _stream_ptr(device) -> ctypes.c_void_p:
 def _scalar_ptr(t: torch.Tensor, device) -> tuple:
     """(keep-alive tensor, device pointer) of a one-element fp32 tensor on `device`."""
     t = t.detach()
+    if t.is_neg():                       # the imaginary part of a conjugate: its sign is a bit of the tensor, not of the memory
+        t = t.resolve_neg()
     if t.device != device or not t.is_contiguous():
         t = t.to(device).contiguous()
     return t, t.data_ptr()

@@ -106,6 +106,8 @@ def grouped_scaled_mm(input, mat2, m_splits, scale_a, scale_b, scale_result=None
     if max(T, N, K) >= 1 << 31:
         raise ValueError(f"grouped_scaled_mm(): sizes are below 2^31, got {T} rows, N = {N}, K = {K}")
     sizes = _sizes(m_splits, E, T)
+    if scale_a.is_neg() or scale_b.is_neg():
+        scale_a, scale_b = scale_a.resolve_neg(), scale_b.resolve_neg()
     sa, sb = _group_scale("scale_a", scale_a, E), _group_scale("scale_b", scale_b, E)
     plain = _plainly_valid(input, mat2, scale_a, scale_b, scale_result, out_dtype, out)
     if plain:

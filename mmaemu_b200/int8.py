@@ -61,6 +61,8 @@ def quantize_int8(x):
     code = _REAL_CODES.get(x.dtype)
     if code is None:
         raise TypeError(f"quantize_int8(): x must be float32, bfloat16 or float16, got {x.dtype}")
+    if x.is_neg():                       # the imaginary part of a conjugate: its sign is a bit of the tensor, not of the memory
+        x = x.resolve_neg()
     shape = x.shape
     if not shape:
         raise ValueError("quantize_int8(): x must have at least one dimension")
@@ -144,7 +146,7 @@ def _output(who, input, out, out_dtype, rows, N):
         raise ValueError(f"{who}(): the output is float32, bfloat16 or float16, got {dtype}")
     if out is None:
         return (input.new_empty((rows, N), dtype=dtype) if input.is_cuda else None), N, code
-    if tuple(out.shape) != (rows, N) or (N > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < N):
+    if tuple(out.shape) != (rows, N) or (N > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < N) or out.is_neg():
         raise ValueError(f"{who}(): out must be a row-major tensor of shape {(rows, N)}, got shape {tuple(out.shape)} with strides "
                          f"{tuple(out.stride())}")
     return out, (out.stride(0) if rows > 1 else N), code
@@ -188,6 +190,8 @@ def int8_scaled_mm(input, mat2, scale_a, scale_b, bias=None, out_dtype=None, *, 
     first."""
     who = "int8_scaled_mm"
     index = _check_operands(who, input, mat2, scale_a, scale_b, bias, out)
+    if scale_a.is_neg() or scale_b.is_neg() or (bias is not None and bias.is_neg()):
+        scale_a, scale_b, bias = scale_a.resolve_neg(), scale_b.resolve_neg(), None if bias is None else bias.resolve_neg()
     sizes, sizes2 = input.shape, mat2.shape
     if len(sizes) != 2 or len(sizes2) != 2 or sizes[1] != sizes2[0]:
         raise ValueError(f"{who}(): expected input [M, K] and mat2 [K, N], got {tuple(sizes)} and {tuple(sizes2)}")
@@ -237,6 +241,8 @@ def int8_grouped_scaled_mm(input, mat2, offs, scale_a, scale_b, bias=None, out_d
     if not isinstance(offs, torch.Tensor):
         raise _not_a_tensor(who, "offs", offs)
     index = _check_operands(who, input, mat2, scale_a, scale_b, bias, out)
+    if scale_a.is_neg() or scale_b.is_neg() or (bias is not None and bias.is_neg()):
+        scale_a, scale_b, bias = scale_a.resolve_neg(), scale_b.resolve_neg(), None if bias is None else bias.resolve_neg()
     if offs.get_device() != index:
         raise ValueError(f"{who}(): expected all tensors on one device, found {input.device} and {offs.device}")
     sizes, sizes2 = input.shape, mat2.shape

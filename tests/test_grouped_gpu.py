@@ -405,3 +405,17 @@ def test_a_wait_that_runs_out_in_one_group_leaves_the_others_written(sizes, one_
     mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, out=out, **kw)
     assert np.array_equal(bits(out), bits(want))
     assert L.mmb200_grouped_status(kept[1].data_ptr(), st) == _lib.OK
+
+
+def test_scales_whose_sign_is_a_bit():
+    """Scales that are the imaginary part of a conjugate: the sign is a bit of the tensor, not of the memory."""
+    sizes, N, K = [5, 0, 140], 144, 272
+    a, w, ta, tw = operands(sizes, N, K, seed=22)
+    z = torch.complex(torch.zeros(3, device=DEV), torch.tensor([0.5, -2.0, 0.25], device=DEV)).conj().imag
+    assert z.is_neg()
+    plain = torch.tensor([-0.5, 2.0, -0.25], device=DEV)
+    kw = dict(out_dtype=torch.float32, profile="hopper", splitk=1)
+    want = loop(ta, tw, sizes, plain, plain[1:2], **kw)
+    assert np.array_equal(bits(want[:5]), oracle.scaled_mm(a[:5], w[0], -0.5, 2.0, out="float32", preset="hopper", fast=False))
+    assert np.array_equal(bits(mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, z, z[1:2], **kw)), bits(want))
+    assert np.array_equal(bits(loop(ta, tw, sizes, z, z[1:2], **kw)), bits(want))

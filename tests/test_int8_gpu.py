@@ -602,3 +602,29 @@ def test_a_checked_call_reports_its_own_waits_only(monkeypatch):
         L.mmb200_test_hooks(0, 0)
     assert L.mmb200_int8_status(st) == _lib.OK
     same(mm.int8_scaled_mm(a, w.t(), one, one), want)
+
+
+def negated(*shape, seed=0):
+    """The imaginary part of a conjugate: a view whose sign is a bit of the tensor, and the same values in memory."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    v = torch.randn(*shape, dtype=torch.complex64, generator=g, device=DEV).conj().imag
+    assert v.is_neg()
+    return v, v.resolve_neg().contiguous()
+
+
+def test_views_whose_sign_is_a_bit():
+    for shape in ((6, 1), (6, 40)):
+        x, plain = negated(*shape, seed=1)
+        for got, want in zip(mm.quantize_int8(x), mm.quantize_int8(plain)):
+            assert torch.equal(got, want)
+        check_quantised(plain)
+    M, N, K, E = 7, 33, 64, 2
+    a, w, w3 = codes(M, K, seed=1), codes(N, K, seed=2), codes(E, N, K, seed=3)
+    (va, sa), (vb, sb), (vc, sc), (v3, s3) = negated(M, 1, seed=2), negated(1, N, seed=3), negated(1, seed=4), negated(E, 1, N, seed=5)
+    same(mm.int8_scaled_mm(a, w.t(), va, vb), want_bits(a, w, sa, sb, torch.bfloat16))
+    same(mm.int8_scaled_mm(a, w.t(), vc, sb), want_bits(a, w, sc, sb, torch.bfloat16))
+    same(mm.int8_scaled_mm(a, w[:1].t(), sa, sb[:, :1], vc), mm.int8_scaled_mm(a, w[:1].t(), sa, sb[:, :1], sc))
+    ends = torch.tensor([3, 7], dtype=torch.int32, device=DEV)
+    same(mm.int8_grouped_scaled_mm(a, w3.transpose(1, 2), ends, va, v3), grouped_want(a, w3, [3, 7], sa, s3, torch.bfloat16))
+    with pytest.raises(ValueError):
+        mm.int8_scaled_mm(a, w[:1].t(), sa, sb[:, :1], out=negated(M, 1)[0])
