@@ -419,3 +419,25 @@ def test_scales_whose_sign_is_a_bit():
     assert np.array_equal(bits(want[:5]), oracle.scaled_mm(a[:5], w[0], -0.5, 2.0, out="float32", preset="hopper", fast=False))
     assert np.array_equal(bits(mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, z, z[1:2], **kw)), bits(want))
     assert np.array_equal(bits(loop(ta, tw, sizes, z, z[1:2], **kw)), bits(want))
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^32 bytes of weights and more than 2^31 outputs."""
+    E, N, K = 5, 16384, 65536
+    base = operands([1], 256, K, seed=23)
+    tw = base[3].view(torch.uint8).repeat(E, N // 256, 1)
+    tw[-1] = 0x3C                                                    # the last group's weights: 1.5
+    tw = tw.view(F8["e4m3"])
+    assert tw.numel() > 2 ** 32
+    sizes = [1, 0, 2, 0, 2]
+    _, _, ta, _ = operands(sizes, 16, K, seed=24)
+    check(ta, tw, sizes, *group_scales(E), out_dtype=torch.float32, profile="hopper", splitk=1)
+    del tw, base
+    sizes, N, K = [130000, 3, 1100], 16512, 32
+    _, _, ta, tw = operands(sizes, N, K, seed=25)
+    sa, sb = group_scales(3)
+    kw = dict(out_dtype=torch.bfloat16, profile="hopper", splitk=1, use_fast_accum=True)
+    y = mm.grouped_scaled_mm(ta, tw.transpose(1, 2), sizes, sa, sb, **kw)
+    assert y.numel() > 2 ** 31
+    for e, lo, hi in ((0, 0, 100), (0, 129900, 130000), (1, 130000, 130003), (2, 130003, 131103)):
+        assert np.array_equal(bits(y[lo:hi]), bits(mm.scaled_mm(ta[lo:hi], tw[e].t(), sa[e], sb[e], **kw)))

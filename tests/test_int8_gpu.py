@@ -628,3 +628,49 @@ def test_views_whose_sign_is_a_bit():
     same(mm.int8_grouped_scaled_mm(a, w3.transpose(1, 2), ends, va, v3), grouped_want(a, w3, [3, 7], sa, s3, torch.bfloat16))
     with pytest.raises(ValueError):
         mm.int8_scaled_mm(a, w[:1].t(), sa, sb[:, :1], out=negated(M, 1)[0])
+
+
+@pytest.mark.parametrize("layout", ["groups inside rows", "gap between groups", "overlapping groups", "one channel, strided groups"])
+@pytest.mark.parametrize("sizes", [[5, 0, 40, 3], [300, 0, 129, 600]])
+def test_grouped_weights_in_place_with_any_group_stride(layout, sizes):
+    """Group strides that are below the row stride, no multiple of it, or below a matrix: read in place all the same."""
+    E, T, N, K = 4, sum(sizes), 1 if "one channel" in layout else 272, 320
+    strides = {"groups inside rows": (K, E * K), "gap between groups": (N * K + 48, K), "overlapping groups": (16, K),
+               "one channel, strided groups": (48 + K, K)}[layout]
+    a, home = codes(T, K, seed=1), codes(E * (N * K + 400), seed=2)
+    w = home.as_strided((E, N, K), (*strides, 1))
+    sa, sb = scales(T, 1, seed=3), scales(E, 1, N, seed=4)
+    ends = torch.tensor(sizes, device=DEV).cumsum(0).to(torch.int32)
+    assert _lib.load().mmb200_int8_workspace_bytes(a.data_ptr(), K, w.data_ptr(), strides[1], strides[0], T, N, K, E) == 0
+    same(mm.int8_grouped_scaled_mm(a, w.transpose(1, 2), ends, sa, sb), grouped_want(a, w, ends.tolist(), sa, sb, torch.bfloat16))
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 outputs, input codes and quantised values; the first, middle and last rows are compared."""
+    T, N, K = 131079, 20000, 48
+    a, w = codes(T, K, seed=1), codes(N, K, seed=2)
+    sa, sb = scales(T, 1, seed=3), scales(1, N, seed=4)
+    ends = torch.tensor([70001, T - 5], dtype=torch.int32, device=DEV)
+    y, z = mm.int8_scaled_mm(a, w.t(), sa, sb), mm.int8_grouped_scaled_mm(a, torch.stack([w, w.flip(0)]).transpose(1, 2), ends, sa, sb[0, 0])
+    assert y.numel() > 2 ** 31
+    for lo in (0, 69990, T - 40):
+        rows = slice(lo, min(lo + 40, T))
+        same(y[rows], want_bits(a[rows], w, sa[rows], sb, torch.bfloat16))
+        first, second = (want_bits(a[rows], v, sa[rows], sb[0, 0], torch.bfloat16) for v in (w, w.flip(0)))
+        row = torch.arange(T, device=DEV)[rows, None]
+        same(z[rows], torch.where(row < 70001, first, torch.where(row < T - 5, second, 0.0)))
+    del y, z
+    T, K = 70001, 32768
+    x = torch.empty(T, K, dtype=torch.float16, device=DEV)
+    for lo in range(0, T, 10000):
+        x[lo:lo + 10000].normal_(generator=torch.Generator(device=DEV).manual_seed(lo))
+    xq, sx = mm.quantize_int8(x)
+    assert xq.numel() > 2 ** 31
+    for lo in (0, 65530, T - 20):
+        rows = slice(lo, min(lo + 20, T))
+        assert torch.equal(xq[rows], quantise_want(x[rows])[0]) and torch.equal(sx[rows], mm.quantize_int8(x[rows].clone())[1])
+    w, sb = codes(40, K, seed=5), scales(1, 40, seed=6)
+    y = mm.int8_scaled_mm(xq, w.t(), sx, sb)
+    for lo in (0, 65530, T - 20):
+        rows = slice(lo, min(lo + 20, T))
+        same(y[rows], want_bits(xq[rows], w, sx[rows], sb, torch.bfloat16))
