@@ -674,3 +674,13 @@ def test_offsets_beyond_32_bits():
     for lo in (0, 65530, T - 20):
         rows = slice(lo, min(lo + 20, T))
         same(y[rows], want_bits(xq[rows], w, sx[rows], sb, torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_quantise_rows_of_one_repeated_value(dtype):
+    """Rows of one value without a stride between them."""
+    one = torch.tensor([[-0.75]], dtype=DT[dtype], device=DEV)
+    check_quantised(one.expand(5, 1))
+    check_quantised(one.expand(2, 300, 1))
+    check_quantised(one.expand(5, 40))
+    check_quantised(one[0].expand(7))
