@@ -32,7 +32,7 @@ struct Int8Params {
   int T, N, K, E;
   int bias_dtype, out_dtype;
   int zero_rest;          // rows behind the last group are set to zero
-  int k_blocks, tiles_n, tiles_t;       // set by the launcher
+  int k_blocks, tiles_n;  // set by the launcher
   int wait_polls, announce_extra;
 };
 // Scratch memory for operands that TMA cannot read in place (0: none needed).

@@ -52,13 +52,24 @@ __device__ __forceinline__ void commit(unsigned long long* bar) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, unsigned long long* bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-               ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar)) : "memory");
+// Copies of a box of rows (channels) for a kernel of CTAS CTAs per worker; `bar`: shared address of the barrier they count on.
+template <int CTAS>
+__device__ __forceinline__ void load_rows(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if constexpr (CTAS == 1)
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-               ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
+template <int CTAS>
+__device__ __forceinline__ void load_channels(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if constexpr (CTAS == 1)
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -314,8 +325,8 @@ __global__ void __launch_bounds__(TILE_THREADS) int8_tile_kernel(const __grid_co
           const int s = t % STAGES;
           if (t >= STAGES && !mbar_wait(&sm.empty[s], ((t / STAGES) - 1) & 1, p.wait_polls)) { ok = false; break; }
           mbar_expect_tx(&sm.full[s], (uint32_t)sizeof(typename Smem::Stage) + (uint32_t)p.announce_extra);
-          tma_3d(sm.stage[s].w, &map_w, (kb0 + t) * KB, n0, g.g, &sm.full[s]);
-          tma_2d(sm.stage[s].a, &map_a, (kb0 + t) * KB, row0, &sm.full[s]);
+          load_channels<1>(sm.stage[s].w, &map_w, (kb0 + t) * KB, n0, g.g, smem_addr(&sm.full[s]));
+          load_rows<1>(sm.stage[s].a, &map_a, (kb0 + t) * KB, row0, smem_addr(&sm.full[s]));
           issued = t + 1;
         }
         // the CTA must not end while a copy may be in flight: wait for the last copy into every stage (bounded)
@@ -420,24 +431,6 @@ __device__ __forceinline__ uint32_t first_cta(const void* ptr) {
   uint32_t a;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(ptr)));
   return a;
-}
-template <int CTAS>
-__device__ __forceinline__ void load_rows(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  if constexpr (CTAS == 1)
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-  else
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
-template <int CTAS>
-__device__ __forceinline__ void load_channels(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  if constexpr (CTAS == 1)
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
-  else
-    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 template <int CTAS>
 __device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
