@@ -236,9 +236,9 @@ int mmb200_kernel_for(const void *A_dev, int64_t lda, const void *B_dev, int64_t
  * the call (the split decision of the emulated platform depends on a group's rows). With scratch memory the unsplit groups
  * run in one pass of launches (up to 8 GiB of decoded operands), the others one after the other. Scratch memory as there:
  * mmb200_grouped_workspace_bytes, or, where that much is not to be had, mmb200_grouped_workspace_bytes_one_by_one, with which
- * every group runs by itself on the scratch-memory kernels; mmb200_grouped_status synchronises `stream` and reports whether a bounded wait of the call
- * that last used it ran out (outputs of the groups whose waits ran out then keep their previous contents, all others are written). The reference has no grouped
- * call. */
+ * every group runs by itself on the scratch-memory kernels. mmb200_grouped_status synchronises `stream` and reports whether a
+ * bounded wait of the call that last used the memory ran out (outputs of the groups whose waits ran out then keep their
+ * previous contents, all others are written). The reference has no grouped call. */
 #define MMB200_MAX_GROUPS 4096
 size_t mmb200_grouped_workspace_bytes(const int *m_splits, const int *splits, int E, int N, int K, int fmt_a, int fmt_b,
                                       int nfma, int fast);

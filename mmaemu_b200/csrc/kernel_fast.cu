@@ -1563,8 +1563,8 @@ cudaError_t launch_staged(const Params& p_in, int nfma, void* workspace, size_t 
 
 // ---------------------------------------------------------------------------------------------------------------
 // Ragged groups, unsplit plans: all groups in one pass of launches. Groups of up to `few` rows run on 16-row tiles, the others
-// on 128-row tcgen05 tiles; both walk a list of row tiles that a small kernel writes from the group sizes. Against the launches
-// of one group after the other: 16 rows in 8 groups (1024 x 2048, slow) 32 us instead of 105, 1000 rows (1040 x 2064, fast) 125
+// on 128-row tcgen05 tiles; both walk a list of row tiles that a small kernel writes from the group sizes. Kernel times against
+// those of one group after the other: 16 rows in 8 groups (1024 x 2048, slow) 32 us instead of 105, 1000 rows (1040 x 2064, fast) 125
 // instead of 646, 4096 rows (2048 x 2048, slow) 346 instead of 824. What bounds them is what bounds the kernels of one call; the
 // smallest also its 16-row tiles, which hold one to four rows.
 namespace {

@@ -7,19 +7,21 @@
 //
 // int8_tile_kernel: few rows. One tile of 128 channels x 16, 32 or 64 rows per cluster; the CTAs of a cluster each take a part of
 // K and add their int32 sums through distributed shared memory. Integer sums are exact in any order, so the split changes no
-// bit. Bound by reading the weights: 16 x 8192 x 28672 at 6.1 TB/s (38.5 us); 16 x 4096 x 8192 in 9.2 us, of which 3.5 are
-// launch, first copies and the cluster's sum (64 rows, 512 channels, K = 512 in 4 us; 13 while a thread read the sums one by one).
+// bit. Bound by reading the weights: 16 x 8192 x 28672 in 40 us, 5.8 TB/s; 16 x 4096 x 8192 in 10.5 us (8.2 where the 33.5 MB of
+// weights are still in L2), of which 3.5 are launch, first copies and the cluster's sum (64 rows, 512 channels, K = 512 in 3.3 us;
+// 13 while a thread read the sums one by one). Times of this file: replayed from a graph over operands that do not stay in L2.
 //
 // int8_single_kernel, int8_pair_kernel: more rows. Persistent; TMEM holds two accumulators, so the output of a tile leaves while
 // the next one is multiplied. A CTA works on 128 channels x 64, 128 or 256 rows, a pair of CTAs on neighbouring SMs
 // (cta_group::2) on 256 x 256, each holding half of both operands, so that a byte of shared memory feeds twice the products.
-// Large products are bound by power: 8192 x 24576 x 8192 takes 1.11 ms, 2.95 POP/s; the 8192-cube 3.2 POP/s, with operands of
-// zeros 4.0. 4096 rows in 64 groups on 1536 x 2048 weights: 44 us for 201 MB of weights (one-tile CTAs: 55 us).
+// Large products are bound by power: 8192 x 24576 x 8192 takes 1.15 ms, 2.87 POP/s (a call among others 1.19 ms, 2.77); the 8192-cube
+// 2.9 POP/s, with operands of zeros 4.0. 4096 rows in 64 groups on 1536 x 2048 weights: 45 us for 201 MB of weights (one-tile
+// CTAs: 55 us).
 //
 // An MMA of 128 channels takes about 120 cycles up to 128 rows, so a CTA needs 0.25 us per 128 bytes of K however few rows it
 // has. The output loop must not wait: with a scale loaded per row instead of handed round by shuffles it took 27 us per tile of
-// 256 x 256, now 4.5 us, which still bounds products with K of 1024 and less (8192 x 8192 x 1024: 64 us, of which the MMAs would
-// take 37).
+// 256 x 256, now 4.5 us, which still bounds products with K of 1024 and less (8192 x 8192 x 1024: 64 to 72 us, of which the MMAs
+// would take 37).
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -799,8 +801,9 @@ cudaError_t launch_out(const Int8Params& p, const Maps& m, int parts, unsigned t
 // memory; the slowest of the three counts, and a part of the first (REST), as they overlap only in part. START and the output of
 // the last tile (OUT per row) come on top, the cluster's sum (SUM, and PART and SUM_ROW each) and every further wave of one-tile
 // CTAs (WAVE). Two one-tile CTAs on an SM take SHARE times as long as one; memory is up to SPARE slower with few CTAs. Measured
-// on whole calls, replayed from a graph: 117 shapes of 1 to 2048 rows, 512 to 24576 channels, K from 512 to 28672; the choice was
-// within 5 % of the best of all of them for 102, within 15 % for all.
+// on whole calls, replayed from a graph on three sets of operands in turn (so weights below about 40 MB came from L2): 117 shapes of 1
+// to 2048 rows, 512 to 24576 channels, K from 512 to 28672; the choice was within 5 % of the best of all of them for 102, within
+// 15 % for all.
 enum Kind { TILE, SINGLE, PAIR };
 struct Choice { Kind kind; int rows, parts; };
 long long most_row_tiles(const Int8Params& p, int rows) {               // of all groups: every one may end in a partial tile

@@ -7,11 +7,13 @@
 // row with a NaN or an infinity has scale NaN and codes 0, so every product with it is NaN.
 //
 // What bounds it: one read of x and one write of the codes. A row is read once into registers (16-byte loads) by as many
-// threads as hold it, the maximum is taken across them, and the codes leave from the registers. 8192 x 8192 bf16 takes 36.7 us,
-// 5.5 TB/s or 84 % of the measured copy rate; the issue slots are in use three quarters of the time (9 instructions per value
-// and 4 more of a thread's fixed work), so instructions count: conversions on the quarter-rate pipe took 80 us, single FMAs
-// 40. 1536 threads per SM at most 42 registers each (38.0 us at 44); blocks that keep a row ahead in registers took 49 us, 128
-// threads with twice the vectors 39.
+// threads as hold it, the maximum is taken across them, and the codes leave from the registers. 8192 x 8192 bf16 takes 36.8 us,
+// 5.5 TB/s or 83 % of the measured copy rate, fp32 58 us, 5.8 TB/s; for 16-bit values the issue slots are in use three quarters of the
+// time (9 instructions per value and 4 more of a thread's fixed work), so instructions count: conversions on the quarter-rate pipe
+// took 80 us, single FMAs 40. 1536 threads per SM leave 40 registers for each (the kernels take 32 to 39); blocks that keep a row
+// ahead in registers took 49 us, 128 threads with twice the vectors 39. Of rows beyond 8192 fp32 or 16384 16-bit values, which no
+// block holds, the rest is read a second time: 4096 x 16384 fp32 73 us, 4096 x 28672 bf16 82 us (4.6 and 4.3 TB/s of what has to
+// move).
 #include "common.cuh"
 #include "int8.h"
 
@@ -123,7 +125,7 @@ __device__ __forceinline__ void codes_of(float (&x)[N], const RowScale& r, uint3
 }
 
 // The row's threads (a warp, or the whole block) hold VPT 16-byte vectors each. The last vector of a row may be partial.
-// Rows longer than that are read twice.
+// What a row has beyond that is read twice.
 template <int T, int BLOCK, bool WARP_ROW, int VPT>
 __global__ void __launch_bounds__(BLOCK, 1536 / BLOCK) quantise_kernel(const __grid_constant__ QuantiseParams p) {
   using E = Elem<T>;
